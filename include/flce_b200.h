@@ -416,6 +416,36 @@ int flce_b200_jsd_rows(void* student, int64_t ld_student, const void* teacher, i
                        int64_t n_rows, int64_t vocab, const int64_t* labels, int64_t ignore_index, float beta,
                        float temperature, const float* count, float fixed_count, float* loss_rows, void* stream);
 
+/* ---- Layer norm and RMSNorm over the rows of a matrix (src/liger_kernel/ops/layer_norm.py, src/liger_kernel/ops/rms_norm.py).
+ *
+ *   layer norm  y = (x - mean) * rstd * (offset + weight) + bias,   rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+ *   RMSNorm     y = x * rstd * (offset + weight),                   rstd = 1 / sqrt(mean(x^2) + eps)
+ *
+ * Rows start ld_x elements apart (any pitch >= 0; 16-byte aligned rows of whole 16-byte vectors move fastest); results are
+ * dense.  weight == NULL: a gain of one (offset plays no part); bias may be NULL (always for RMSNorm).  round_xhat != 0 rounds
+ * the normalised value to the rows' type before it meets the weight.  n_rows may be 0. */
+typedef enum flce_norm_kind { FLCE_LAYER_NORM = 0, FLCE_RMS_NORM = 1 } flce_norm_kind_t;
+typedef struct flce_norm {
+  int64_t n_rows, hidden, ld_x;
+  int32_t kind;         /* flce_norm_kind_t */
+  int32_t dtype;        /* of x, y and their gradients */
+  int32_t weight_dtype; /* of weight, bias and their gradients: dtype or FLCE_FP32 */
+  int32_t round_xhat;
+  float eps, offset;
+  const void *x, *weight, *bias;
+} flce_norm_t;
+
+/* mean, rstd: [n_rows] fp32, needed by the backward call; either may be NULL (RMSNorm has no mean). */
+int flce_b200_norm_forward(const flce_norm_t* p, void* y, float* mean, float* rstd, void* stream);
+
+/* grad_weight / grad_bias [hidden] in weight_dtype, NULL where not wanted.  The workspace (4-byte aligned, of
+ * flce_b200_norm_workspace_bytes; only read by the call that wrote it) may be NULL when neither is.  Sums run in a fixed
+ * order: the same bits in every run. */
+size_t flce_b200_norm_workspace_bytes(const flce_norm_t* p);
+int flce_b200_norm_backward(const flce_norm_t* p, const void* grad_y, int64_t ld_grad, const float* mean, const float* rstd,
+                            void* grad_x, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
 /* Synchronises `stream`, then reports whether any kernel of this library abandoned a bounded wait
  * since the last call (FLCE_ERR_DEVICE_TIMEOUT) and clears the record.  For tests and debugging. */
 int flce_b200_check_device_status(void* stream);

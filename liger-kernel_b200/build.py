@@ -15,7 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "liger_kernel_b200", "libflce_b200.so")
-SOURCES = [os.path.join(CSRC, "flce_b200.cu")]
+SOURCES = [os.path.join(CSRC, name) for name in ("flce_b200.cu", "norm_b200.cu")]
 
 
 def _deps():
@@ -44,6 +44,7 @@ def build(force=False, verbose=False, trace=False):
     nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
     cmd = [
         nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
+        "--threads", "0",   # one compiler per source file
         "-shared", "-Xcompiler", "-fPIC", "-I", os.path.join(ROOT, "include"), "-I", CSRC,
         "-o", out,
     ] + (["-DFLCE_CLOCK_TRACE"] if trace else []) + SOURCES

@@ -15,6 +15,7 @@
 #include "epilogues.cuh"
 #include "gemm_sm100.cuh"
 #include "head_loss_kernels.cuh"
+#include "host_internal.hpp"
 #include "rmsnorm_rows.cuh"
 #include "row_kernels.cuh"
 
@@ -23,19 +24,13 @@ namespace flce {
 // ------------------------------------------------------------------ errors
 static thread_local char g_last_error[512] = "";
 
-static int fail(int code, const char* fmt, ...) {
+int fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
   va_end(ap);
   return code;
 }
-
-#define FLCE_CUDA(expr)                                                                             \
-  do {                                                                                              \
-    cudaError_t e__ = (expr);                                                                       \
-    if (e__ != cudaSuccess) return fail(FLCE_ERR_CUDA, "%s failed: %s", #expr, cudaGetErrorString(e__)); \
-  } while (0)
 
 // ------------------------------------------------------------------ process-wide options
 // (atomics: autograd calls backward from worker threads while another thread may still be setting options)
@@ -66,6 +61,8 @@ static int g_profile_created = 0;  // events exist for slots [0, created)
 static int g_profile_used = 0;
 static std::atomic<long long> g_kernel_launches{0};
 static std::mutex g_profile_mutex;
+
+void count_launches(int n) { g_kernel_launches += n; }
 
 static ProfileSlot* profile_begin(int kind, cudaStream_t stream) {
   if (!g_profile_on) return nullptr;
@@ -132,6 +129,23 @@ static int device_state(DeviceState** out) {
     g_sm_count_hint.compare_exchange_strong(expected, st.sm_count);
   }
   *out = &st;
+  return FLCE_OK;
+}
+
+int current_sm_count(int* sm_count) {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  FLCE_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return fail(FLCE_ERR_UNSUPPORTED, "device ordinal %d out of range", dev);
+  int count = known[dev].load(std::memory_order_relaxed);
+  if (count == 0) {
+    int major = 0;
+    FLCE_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev));
+    if (major != 10) return fail(FLCE_ERR_UNSUPPORTED, "this library is built for sm_100a only; device %d is sm_%d?", dev, major);
+    FLCE_CUDA(cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev));
+    known[dev].store(count, std::memory_order_relaxed);
+  }
+  *sm_count = count;
   return FLCE_OK;
 }
 

@@ -1,0 +1,34 @@
+// What the host sides of the library's translation units share.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "flce_b200.h"
+
+namespace flce {
+
+// keeps the message for flce_b200_last_error() (per thread) and returns `code`
+int fail(int code, const char* fmt, ...);
+
+#define FLCE_CUDA(expr)                                                                             \
+  do {                                                                                              \
+    cudaError_t e__ = (expr);                                                                       \
+    if (e__ != cudaSuccess) return fail(FLCE_ERR_CUDA, "%s failed: %s", #expr, cudaGetErrorString(e__)); \
+  } while (0)
+
+// adds to what flce_b200_kernel_launches() reports
+void count_launches(int n);
+
+// SM count of the current device; FLCE_ERR_UNSUPPORTED unless it is an sm_100 one.  Touches no device memory and no
+// stream, so the first call on a device may come while a stream is being captured.
+int current_sm_count(int* sm_count);
+
+// A launch that the host emulation of the tests can stand in for.  `kernel` is parenthesised: it holds commas.
+#ifndef FLCE_HOST_EMULATION
+#define FLCE_LAUNCH(kernel, grid, block, stream, ...) kernel<<<grid, block, 0, stream>>>(__VA_ARGS__)
+#else
+#define FLCE_LAUNCH(kernel, grid, block, stream, ...) \
+  emu::launch(emu_dim3(grid), emu_dim3(block), [&]() { (void)(stream), (kernel)(__VA_ARGS__); })
+#endif
+
+}  // namespace flce

@@ -11,12 +11,18 @@ from .ops.fused_linear_jsd import LigerFusedLinearJSDFunction  # noqa: F401
 from .ops.fused_linear_scaled_cross_entropy import LigerFusedLinearScaledCrossEntropyFunction  # noqa: F401
 from .ops.fused_rmsnorm_linear_cross_entropy import LigerFusedRMSNormLinearCrossEntropyFunction  # noqa: F401
 from .ops.fused_rmsnorm_linear_cross_entropy import liger_fused_rmsnorm_linear_cross_entropy  # noqa: F401
+from .ops.norm import LigerLayerNormFunction  # noqa: F401
+from .ops.norm import LigerRMSNormFunction  # noqa: F401
 from .transformers.cross_entropy import LigerCrossEntropyLoss  # noqa: F401
 from .transformers.functional import liger_cross_entropy  # noqa: F401
 from .transformers.functional import CrossEntropyOutput  # noqa: F401
 from .transformers.functional import liger_fused_linear_cross_entropy  # noqa: F401
 from .transformers.functional import liger_fused_linear_jsd  # noqa: F401
+from .transformers.functional import liger_layer_norm  # noqa: F401
+from .transformers.functional import liger_rms_norm  # noqa: F401
 from .transformers.fused_linear_jsd import LigerFusedLinearJSD  # noqa: F401
+from .transformers.layer_norm import LigerLayerNorm  # noqa: F401
+from .transformers.rms_norm import LigerRMSNorm  # noqa: F401
 from .transformers.fused_linear_cross_entropy import LigerFusedLinearCrossEntropyLoss  # noqa: F401
 from .transformers.model.loss_utils import LigerForCausalLMLoss  # noqa: F401
 from .transformers.monkey_patch import _apply_liger_kernel_to_instance  # noqa: F401

@@ -15,6 +15,7 @@ FLCE_MEAN, FLCE_SUM, FLCE_NONE = 0, 1, 2
 PHASE_FORWARD, PHASE_BACKWARD, PHASE_FUSED, PHASE_BACKWARD_SPLIT = 0, 1, 2, 3
 ROWSTAT_PLANES = 6
 FLAG_ARGMAX = 1
+FLCE_LAYER_NORM, FLCE_RMS_NORM = 0, 1
 # flce_status_t
 FLCE_OK, FLCE_ERR_INVALID_ARGUMENT, FLCE_ERR_UNSUPPORTED, FLCE_ERR_WORKSPACE, FLCE_ERR_CUDA, FLCE_ERR_DEVICE_TIMEOUT = range(6)
 
@@ -49,6 +50,9 @@ EXPORTS = (
     "flce_b200_sce_workspace_bytes",
     "flce_b200_sce_forward",
     "flce_b200_sce_backward",
+    "flce_b200_norm_forward",
+    "flce_b200_norm_workspace_bytes",
+    "flce_b200_norm_backward",
     "flce_b200_check_device_status",
     "flce_b200_profile_enable",
     "flce_b200_profile_read",
@@ -109,6 +113,15 @@ class SceProblem(C.Structure):
         ("dtype", C.c_int32), ("reserved", C.c_int32), ("ignore_index", C.c_int64),
         ("temperature", C.c_float), ("reserved2", C.c_float),
         ("x", C.c_void_p), ("w", C.c_void_p), ("target", C.c_void_p),
+    ]
+
+
+class Norm(C.Structure):
+    _fields_ = [
+        ("n_rows", C.c_int64), ("hidden", C.c_int64), ("ld_x", C.c_int64),
+        ("kind", C.c_int32), ("dtype", C.c_int32), ("weight_dtype", C.c_int32), ("round_xhat", C.c_int32),
+        ("eps", C.c_float), ("offset", C.c_float),
+        ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p),
     ]
 
 
@@ -197,6 +210,13 @@ def _load():
     lib.flce_b200_sce_forward.restype = C.c_int
     lib.flce_b200_sce_backward.argtypes = [SP, vp, vp, vp, vp, i32, vp, vp, vp, sz, sz, vp]
     lib.flce_b200_sce_backward.restype = C.c_int
+    NP = C.POINTER(Norm)
+    lib.flce_b200_norm_forward.argtypes = [NP, vp, vp, vp, vp]
+    lib.flce_b200_norm_forward.restype = C.c_int
+    lib.flce_b200_norm_workspace_bytes.argtypes = [NP]
+    lib.flce_b200_norm_workspace_bytes.restype = sz
+    lib.flce_b200_norm_backward.argtypes = [NP, vp, i64, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.flce_b200_norm_backward.restype = C.c_int
     lib.flce_b200_check_device_status.argtypes = [vp]
     lib.flce_b200_selftest_wait_expiry.argtypes = [i64, vp, vp]
     lib.flce_b200_selftest_wait_expiry.restype = C.c_int

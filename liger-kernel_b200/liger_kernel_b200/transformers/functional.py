@@ -1,6 +1,7 @@
 """Functional entry points, signature-compatible with ``liger_fused_linear_cross_entropy`` and
 ``liger_cross_entropy`` (reference: ``src/liger_kernel/transformers/functional.py:81-121`` and ``:42-78``) and
-their result type ``CrossEntropyOutput`` (``:34-39``), plus ``liger_fused_linear_jsd`` (``:124-146``)."""
+their result type ``CrossEntropyOutput`` (``:34-39``), plus ``liger_fused_linear_jsd`` (``:124-146``), ``liger_layer_norm`` and
+``liger_rms_norm``."""
 
 from dataclasses import dataclass
 from typing import Optional
@@ -10,6 +11,7 @@ import torch
 from ..ops.cross_entropy import LigerCrossEntropyFunction
 from ..ops.fused_linear_cross_entropy import LigerFusedLinearCrossEntropyFunction
 from ..ops.fused_linear_jsd import LigerFusedLinearJSDFunction
+from ..ops.norm import LigerLayerNormFunction, LigerRMSNormFunction
 
 
 @dataclass
@@ -86,3 +88,14 @@ def liger_fused_linear_jsd(
         student_input, student_weight, teacher_input, teacher_weight, shift_labels, jsd_beta, ignore_index, temperature,
         accum_dtype,
     )
+
+
+def liger_layer_norm(X, W=None, B=None, eps: float = 1e-6, offset: float = 0.0):
+    """Layer norm over the last dimension: ``(x - mean) * rstd * (offset + W) + B``; ``W`` and ``B`` may be None."""
+    return LigerLayerNormFunction.apply(X, W, B, eps, offset)
+
+
+def liger_rms_norm(X, W=None, eps: float = 1e-6, offset: float = 0.0, casting_mode: str = "llama", in_place: bool = True, row_mode=None):
+    """RMSNorm over the last dimension: ``x * rstd * (offset + W)``; ``W`` may be None.  ``in_place`` and ``row_mode`` are
+    accepted for the reference's call sites and mean nothing here."""
+    return LigerRMSNormFunction.apply(X, W, eps, offset, casting_mode, in_place, row_mode)

@@ -1,0 +1,50 @@
+// The C entry points of the norms, their host side and their kernels, compiled for the host and run on the host
+// through simt_emulation.hpp: the library's own launch shapes, index arithmetic and argument checks, with fibers in
+// the place of CUDA threads.  The "device" has three SMs, so that persistent grids walk over several rows.
+//
+// Test infrastructure only.
+#define FLCE_HOST_EMULATION 1
+#include <cuda_runtime.h>
+#include "simt_emulation.hpp"
+
+#include <cstdarg>
+#include <cstdio>
+#include <type_traits>
+
+inline emu::Dim3 emu_dim3(dim3 d) { return emu::Dim3(d.x, d.y, d.z); }
+
+#include "host_internal.hpp"
+
+namespace flce {
+static char g_message[512];
+static int g_launches = 0;
+int fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_message, sizeof(g_message), fmt, ap);
+  va_end(ap);
+  return code;
+}
+void count_launches(int n) { g_launches += n; }
+int current_sm_count(int* sm_count) {
+  *sm_count = 3;
+  return FLCE_OK;
+}
+}  // namespace flce
+
+// what the host sides call of the CUDA runtime (renamed: a process that holds the real one would get that)
+static cudaError_t emu_cuda_last_error() { return cudaSuccess; }
+static cudaError_t emu_cuda_memset_async(void* p, int v, size_t n, cudaStream_t) {
+  std::memset(p, v, n);
+  return cudaSuccess;
+}
+static const char* emu_cuda_error_string(cudaError_t) { return "emulated"; }
+#define cudaGetLastError emu_cuda_last_error
+#define cudaMemsetAsync emu_cuda_memset_async
+#define cudaGetErrorString emu_cuda_error_string
+extern "C" {
+const char* emu_last_error(void) { return flce::g_message; }
+int emu_launches(void) { return flce::g_launches; }
+}
+
+#include "norm_b200.cu"
