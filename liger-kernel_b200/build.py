@@ -1,4 +1,5 @@
-"""Build libflce_b200.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a.
+"""Build libflce_b200.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a, and libflce_b200_torch.so (the torch binding of
+the operators that run many times per step) with g++ against the headers of the installed torch.
 
     python liger-kernel_b200/build.py [--force] [--verbose]
 
@@ -6,6 +7,7 @@ nvcc cross-compiles, so no GPU is needed to build.
 """
 
 import argparse
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -16,6 +18,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "liger_kernel_b200", "libflce_b200.so")
 SOURCES = [os.path.join(CSRC, name) for name in ("flce_b200.cu", "norm_b200.cu")]
+BINDING = os.path.join(HERE, "liger_kernel_b200", "libflce_b200_torch.so")
+BINDING_SOURCE = os.path.join(CSRC, "torch_ops.cpp")
 
 
 def _deps():
@@ -26,9 +30,9 @@ def _deps():
 
 
 def needs_build():
-    if not os.path.exists(OUT):
+    if not (os.path.exists(OUT) and os.path.exists(BINDING)):
         return True
-    built = os.path.getmtime(OUT)
+    built = min(os.path.getmtime(OUT), os.path.getmtime(BINDING))
     return any(os.path.getmtime(d) > built for d in _deps())
 
 
@@ -51,8 +55,23 @@ def build(force=False, verbose=False, trace=False):
     if verbose:
         cmd.insert(1, "-Xptxas")
         cmd.insert(2, "-v")
-    subprocess.run(cmd, check=True)
+    binding = None if trace else subprocess.Popen(_binding_command(nvcc))
+    try:
+        subprocess.run(cmd, check=True)
+    finally:
+        status = 0 if binding is None else binding.wait()
+    if status != 0:
+        raise RuntimeError(f"building {BINDING} failed with exit code {status}")
     return out
+
+
+def _binding_command(nvcc):
+    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    cuda_dir = os.environ.get("CUDA_HOME") or os.path.dirname(os.path.dirname(os.path.realpath(nvcc)))
+    include = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+               os.path.join(cuda_dir, "include"), os.path.join(ROOT, "include")]
+    return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared"] + [f"-I{d}" for d in include] + ["-o", BINDING, BINDING_SOURCE]
+            + [f"-L{os.path.join(torch_dir, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ldl"])
 
 
 if __name__ == "__main__":

@@ -1,0 +1,40 @@
+"""Loads the compiled torch binding (``csrc/torch_ops.cpp``: allocation, checks and autograd nodes of the operators that run
+many times per step) and points it at the loaded ``libflce_b200.so``.
+
+There is no fallback: if the binding is missing, importing this module raises.
+"""
+
+import ctypes as C
+import os
+
+import torch
+
+from . import _lib
+
+_HERE = os.path.dirname(os.path.abspath(__file__))
+BINDING_PATH = os.path.join(_HERE, "libflce_b200_torch.so")
+
+
+def bind(path, host_memory=False):
+    """Route the binding to the library at ``path`` (``host_memory``: one that computes on host memory, for tests)."""
+    missing = _binding.liger_b200_bind(os.fsencode(path), int(host_memory))
+    if missing is not None:
+        raise ImportError(missing.decode())
+
+
+def _load():
+    if not os.path.exists(BINDING_PATH):
+        raise ImportError(
+            f"{BINDING_PATH} is missing: build it with `python liger-kernel_b200/build.py` "
+            "(g++, the headers of the installed torch). This package has no CPU or PyTorch fallback."
+        )
+    torch.ops.load_library(BINDING_PATH)
+    binding = C.CDLL(BINDING_PATH)
+    binding.liger_b200_bind.argtypes = [C.c_char_p, C.c_int]
+    binding.liger_b200_bind.restype = C.c_char_p
+    return binding
+
+
+_binding = _load()
+bind(_lib.LIB_PATH)
+norm = torch.ops.liger_b200.norm.default

@@ -43,7 +43,8 @@ static const char* emu_cuda_error_string(cudaError_t) { return "emulated"; }
 #define cudaMemsetAsync emu_cuda_memset_async
 #define cudaGetErrorString emu_cuda_error_string
 extern "C" {
-const char* emu_last_error(void) { return flce::g_message; }
+const char* flce_b200_last_error(void) { return flce::g_message; }
+const char* flce_b200_status_string(int) { return "emulated"; }
 int emu_launches(void) { return flce::g_launches; }
 }
 

@@ -18,8 +18,8 @@ BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
     (33, 31, FP16, FP16, 0), (21, 33, BF16, BF16, 2), (37, 128, BF16, BF16, 0), (19, 132, FP32, FP32, 4), (13, 250, FP16, FP16, 6),
     (14, 264, BF16, BF16, 16), (9, 1001, FP32, FP32, 0), (8, 1024, FP32, FP32, 0), (5, 4104, BF16, FP32, 0), (4, 5000, FP16, FP16, 1),
     (2, 9000, FP32, FP32, 0), (2, 16387, BF16, BF16, 0), (2, 16392, FP16, FP32, 0)])
-def test_matches_definition(monkeypatch, kind, n, hidden, dtype, wdtype, pitch):
-    with train_ops_emu.installed(monkeypatch):
+def test_matches_definition(kind, n, hidden, dtype, wdtype, pitch):
+    with train_ops_emu.installed():
         cases.case_matches_definition("cpu", kind, n, hidden, dtype, wdtype, True, True, 0.0, pitch)
 
 
@@ -27,30 +27,30 @@ def test_matches_definition(monkeypatch, kind, n, hidden, dtype, wdtype, pitch):
     ("layer", True, False, 1.0, "gemma"), ("layer", False, False, 0.0, "gemma"), ("layer", False, True, 0.0, "gemma"),
     ("rms", True, False, 1.0, "llama"), ("rms", False, False, 0.0, "llama"), ("rms", True, False, 1.0, "gemma")])
 @pytest.mark.parametrize("hidden", [27, 40, 336, 777])
-def test_parameters_and_casting(monkeypatch, kind, weight, bias, offset, mode, hidden):
-    with train_ops_emu.installed(monkeypatch):
+def test_parameters_and_casting(kind, weight, bias, offset, mode, hidden):
+    with train_ops_emu.installed():
         cases.case_matches_definition("cpu", kind, 11, hidden, BF16, None, weight, bias, offset, 0, mode)
 
 
 @pytest.mark.parametrize("kind", ["layer", "rms"])
-def test_gradient_against_differences(monkeypatch, kind):
-    with train_ops_emu.installed(monkeypatch):
+def test_gradient_against_differences(kind):
+    with train_ops_emu.installed():
         cases.case_gradient_against_differences("cpu", kind)
 
 
 @pytest.mark.parametrize("kind", ["layer", "rms"])
-def test_special_values_stay_in_their_row(monkeypatch, kind):
-    with train_ops_emu.installed(monkeypatch):
+def test_special_values_stay_in_their_row(kind):
+    with train_ops_emu.installed():
         cases.case_special_values("cpu", kind)
 
 
-def test_shapes_and_views(monkeypatch):
-    with train_ops_emu.installed(monkeypatch):
+def test_shapes_and_views():
+    with train_ops_emu.installed():
         cases.case_shapes_and_views("cpu")
 
 
-def test_refusals(monkeypatch):
-    with train_ops_emu.installed(monkeypatch):
+def test_refusals():
+    with train_ops_emu.installed():
         cases.case_refusals("cpu")
 
 
@@ -97,7 +97,7 @@ def test_entry_points_check_their_arguments():
     assert backward(norm(), dy=None) == INVALID and backward(norm(), rstd=None) == INVALID and backward(norm(), mean=None) == INVALID
     assert backward(norm(), dx=None) == INVALID and backward(norm(), ld=-1) == INVALID and backward(norm(), dy=base + 2) == INVALID
     assert backward(norm(), nbytes=15) == WORKSPACE and backward(norm(), ws=None) == WORKSPACE and backward(norm(), ws=base + 2) == WORKSPACE
-    assert b"workspace" in lib.emu_last_error()
+    assert b"workspace" in lib.flce_b200_last_error()
     assert backward(norm(), dw=None, ws=None, nbytes=0) == 0
     rms = norm(kind=_lib.FLCE_RMS_NORM, bias=None)
     assert backward(rms, mean=None) == 0 and backward(rms, db=base + 5120) == INVALID

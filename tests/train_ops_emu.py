@@ -35,20 +35,18 @@ def load():
         if hasattr(lib, name):
             fn, of = getattr(lib, name), getattr(real.lib, name)
             fn.argtypes, fn.restype = of.argtypes, of.restype
-    lib.emu_last_error.restype = C.c_char_p
     _lib = lib
     return lib
 
 
 @contextlib.contextmanager
-def installed(monkeypatch):
-    """The operators' modules call the emulation and accept CPU tensors."""
-    import liger_kernel_b200.ops.fused_linear_cross_entropy as fl
-    import liger_kernel_b200.ops.norm as norm
+def installed():
+    """The torch binding calls the emulation and accepts CPU tensors."""
+    from liger_kernel_b200 import _lib as real, _torch_ops
 
     lib = load()
-    monkeypatch.setattr(norm, "lib", lib)
-    monkeypatch.setattr(fl, "_stream", lambda device: None)
-    monkeypatch.setattr(fl, "_device_guard", lambda device: contextlib.nullcontext())
-    monkeypatch.setattr(fl, "_require_cuda", lambda t: None)
-    yield lib
+    _torch_ops.bind(_OUT, host_memory=True)
+    try:
+        yield lib
+    finally:
+        _torch_ops.bind(real.LIB_PATH)
