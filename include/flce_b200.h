@@ -446,6 +446,37 @@ int flce_b200_norm_backward(const flce_norm_t* p, const void* grad_y, int64_t ld
                             void* grad_x, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
                             void* stream);
 
+/* ---- Load-balancing loss of a mixture-of-experts router over the logits of all layers, with per-expert token counts.
+ *
+ *   C[l][e]  kept tokens of layer l with expert e among their top_k logits (equal logits: the lowest index first)
+ *   S_e      sum over the kept tokens of all layers of softmax(logits)_e;     N = kept tokens of all layers
+ *   loss   = n_experts / N^2 * sum_e (sum_l C[l][e]) * S_e + lse_square_scale / N * sum lse^2     (0 if no token is kept)
+ *
+ * The pooled form the mixture-of-experts models of the transformers library add to their loss.  logits: host array of
+ * n_layers device pointers, each [n_tokens, n_experts] with rows ld elements apart (rows of whole, aligned 16-byte vectors
+ * move fastest); n_experts <= 1024.  mask: n_tokens integers of mask_bytes (1, 4 or 8) that hold for every layer, 0 leaves the
+ * token out (its logits are not read, its gradient is zero); NULL keeps all.  A NaN in a kept row makes the loss NaN and
+ * leaves that row's share of the counts unspecified. */
+typedef struct flce_balance {
+  int64_t n_layers, n_tokens, n_experts, top_k, ld;
+  int32_t dtype;      /* of the logits and their gradients */
+  int32_t mask_bytes;
+  float lse_square_scale;
+  float reserved;
+  const void* mask;
+} flce_balance_t;
+
+size_t flce_b200_balance_workspace_bytes(const flce_balance_t* p);
+
+/* loss[0] = the loss, loss[1] = its lse^2 term; counts [n_layers, n_experts]; coef [n_experts + 1] fp32 is what the backward
+ * call needs of the forward one.  The workspace (8-byte aligned) is free again when the call's kernels have run. */
+int flce_b200_balance_forward(const flce_balance_t* p, const void* const* logits, float* loss, int64_t* counts, float* coef,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* grads: dense [n_layers, n_tokens, n_experts]; grad_loss: one fp32 value on the device. */
+int flce_b200_balance_backward(const flce_balance_t* p, const void* const* logits, const float* coef, const float* grad_loss,
+                               void* grads, void* stream);
+
 /* Synchronises `stream`, then reports whether any kernel of this library abandoned a bounded wait
  * since the last call (FLCE_ERR_DEVICE_TIMEOUT) and clears the record.  For tests and debugging. */
 int flce_b200_check_device_status(void* stream);

@@ -17,7 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "liger_kernel_b200", "libflce_b200.so")
-SOURCES = [os.path.join(CSRC, name) for name in ("flce_b200.cu", "norm_b200.cu")]
+SOURCES = [os.path.join(CSRC, name) for name in ("flce_b200.cu", "norm_b200.cu", "balance_b200.cu")]
 BINDING = os.path.join(HERE, "liger_kernel_b200", "libflce_b200_torch.so")
 BINDING_SOURCE = os.path.join(CSRC, "torch_ops.cpp")
 

@@ -1,0 +1,201 @@
+// Host side of the router's load-balancing loss (kernels: router_balance.cuh; documented in include/flce_b200.h).
+#include "host_internal.hpp"
+#include "router_balance.cuh"
+
+#include <cstdint>
+
+namespace flce {
+namespace {
+
+
+int check_balance(const flce_balance_t* p) {
+  if (p == nullptr) return fail(FLCE_ERR_INVALID_ARGUMENT, "balance is NULL");
+  if (p->n_layers <= 0 || p->n_tokens < 0 || p->n_tokens > 0x7fffffffll || p->n_experts <= 0 || p->n_layers > 0xffff)
+    return fail(FLCE_ERR_INVALID_ARGUMENT, "bad shape (n_layers=%lld n_tokens=%lld n_experts=%lld)", (long long)p->n_layers,
+                (long long)p->n_tokens, (long long)p->n_experts);
+  if (p->n_experts > 32 * kBalMaxEpt)
+    return fail(FLCE_ERR_UNSUPPORTED, "at most %d experts, got %lld", 32 * kBalMaxEpt, (long long)p->n_experts);
+  if (p->top_k <= 0 || p->top_k > p->n_experts)
+    return fail(FLCE_ERR_INVALID_ARGUMENT, "top_k must be in [1, %lld], got %lld", (long long)p->n_experts, (long long)p->top_k);
+  if (p->ld < 0) return fail(FLCE_ERR_INVALID_ARGUMENT, "negative pitch %lld", (long long)p->ld);
+  if (p->dtype < FLCE_BF16 || p->dtype > FLCE_FP32) return fail(FLCE_ERR_INVALID_ARGUMENT, "bad dtype %d", p->dtype);
+  if (p->mask != nullptr && p->mask_bytes != 1 && p->mask_bytes != 4 && p->mask_bytes != 8)
+    return fail(FLCE_ERR_INVALID_ARGUMENT, "mask elements have 1, 4 or 8 bytes, got %d", p->mask_bytes);
+  if (p->mask != nullptr && (reinterpret_cast<uintptr_t>(p->mask) % p->mask_bytes) != 0)
+    return fail(FLCE_ERR_INVALID_ARGUMENT, "the mask does not start on a multiple of its element size");
+  return FLCE_OK;
+}
+
+int check_layers(const flce_balance_t* p, const void* const* logits) {
+  if (logits == nullptr) return fail(FLCE_ERR_INVALID_ARGUMENT, "logits is NULL");
+  for (int64_t l = 0; l < p->n_layers; ++l) {
+    if (p->n_tokens > 0 && logits[l] == nullptr) return fail(FLCE_ERR_INVALID_ARGUMENT, "logits of layer %lld are NULL", (long long)l);
+    if ((reinterpret_cast<uintptr_t>(logits[l]) % element_size(p->dtype)) != 0)
+      return fail(FLCE_ERR_INVALID_ARGUMENT, "logits of layer %lld do not start on a multiple of their element size", (long long)l);
+  }
+  return FLCE_OK;
+}
+
+struct BalanceShape {
+  bool vectors;
+  int ept, log2_group;
+};
+
+// Lanes that share a row: as many as it takes with 8 logits each, and more logits per lane beyond 256 experts.
+BalanceShape balance_shape(const flce_balance_t* p, const void* const* logits, const void* out) {
+  BalanceShape s;
+  const int vec = 16 / element_size(p->dtype);
+  s.vectors = p->n_experts % vec == 0 && (p->n_tokens <= 1 || p->ld % vec == 0) && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  for (int64_t l = 0; l < p->n_layers; ++l) s.vectors = s.vectors && (reinterpret_cast<uintptr_t>(logits[l]) & 15) == 0;
+  s.ept = p->n_experts <= 256 ? 8 : (p->n_experts <= 512 ? 16 : 32);
+  for (s.log2_group = 0; (s.ept << s.log2_group) < p->n_experts;) ++s.log2_group;
+  return s;
+}
+
+// Blocks per layer: eight per SM over all layers, so that the last wave costs little, but a round of rows each.
+long long balance_blocks(const flce_balance_t* p, int sm_count) {
+  int log2_group = 0;
+  const int ept = p->n_experts <= 256 ? 8 : (p->n_experts <= 512 ? 16 : 32);
+  while ((ept << log2_group) < p->n_experts) ++log2_group;
+  const long long rounds = ceil_div(p->n_tokens, kBalThreads >> log2_group);
+  long long blocks = ceil_div(8ll * sm_count, p->n_layers);
+  if (blocks > rounds) blocks = rounds;
+  return blocks < 1 ? 1 : blocks;
+}
+
+BalanceArgs balance_args(const flce_balance_t* p, const void* const* logits, int64_t first_layer, int64_t layers, const BalanceShape& s) {
+  BalanceArgs a{};
+  for (int64_t l = 0; l < layers; ++l) a.logits[l] = logits[first_layer + l];
+  a.ld = p->ld;
+  a.n_tokens = p->n_tokens;
+  a.experts = static_cast<int>(p->n_experts);
+  a.top_k = static_cast<int>(p->top_k);
+  a.mask = p->mask;
+  a.mask_bytes = p->mask_bytes;
+  a.log2_group = s.log2_group;
+  a.want_lse = p->lse_square_scale != 0.f;
+  return a;
+}
+
+template <class Fn>
+void with_type(int dtype, Fn fn) {
+  if (dtype == FLCE_FP32) fn(float());
+  else if (dtype == FLCE_BF16) fn(__nv_bfloat16());
+  else fn(__half());
+}
+
+template <typename T, bool kVectors>
+void run_forward(const BalanceArgs& a, const BalanceShape& s, dim3 grid, float* partial, cudaStream_t stream) {
+  switch (s.ept) {
+    case 8: FLCE_LAUNCH((balance_forward_kernel<T, kVectors, 8>), grid, kBalThreads, stream, a, partial); break;
+    case 16: FLCE_LAUNCH((balance_forward_kernel<T, kVectors, 16>), grid, kBalThreads, stream, a, partial); break;
+    default: FLCE_LAUNCH((balance_forward_kernel<T, kVectors, 32>), grid, kBalThreads, stream, a, partial); break;
+  }
+}
+
+template <typename T, bool kVectors>
+void run_backward(const BalanceArgs& a, const BalanceShape& s, dim3 grid, const float* coef, const float* up, T* out,
+                  cudaStream_t stream) {
+  switch (s.ept) {
+    case 8: FLCE_LAUNCH((balance_backward_kernel<T, kVectors, 8>), grid, kBalThreads, stream, a, coef, up, out); break;
+    case 16: FLCE_LAUNCH((balance_backward_kernel<T, kVectors, 16>), grid, kBalThreads, stream, a, coef, up, out); break;
+    default: FLCE_LAUNCH((balance_backward_kernel<T, kVectors, 32>), grid, kBalThreads, stream, a, coef, up, out); break;
+  }
+}
+
+// workspace: sums [layers][experts + 1] fp64, kept [layers] int64, partial [layers][blocks][2 experts + 2] 32-bit
+size_t workspace_bytes(const flce_balance_t* p, long long blocks) {
+  const size_t layers = static_cast<size_t>(p->n_layers), experts = static_cast<size_t>(p->n_experts);
+  return layers * (experts + 1) * 8 + layers * 8 + layers * static_cast<size_t>(blocks) * (2 * experts + 2) * 4;
+}
+
+}  // namespace
+}  // namespace flce
+
+using namespace flce;
+
+extern "C" {
+
+size_t flce_b200_balance_workspace_bytes(const flce_balance_t* p) {
+  int sms = 0;
+  if (check_balance(p) != FLCE_OK || current_sm_count(&sms) != FLCE_OK) return 0;
+  return workspace_bytes(p, balance_blocks(p, sms));
+}
+
+int flce_b200_balance_forward(const flce_balance_t* p, const void* const* logits, float* loss, int64_t* counts, float* coef,
+                              void* workspace, size_t bytes, void* stream_) {
+  int rc = check_balance(p);
+  if (rc != FLCE_OK) return rc;
+  rc = check_layers(p, logits);
+  if (rc != FLCE_OK) return rc;
+  if (loss == nullptr || counts == nullptr || coef == nullptr) return fail(FLCE_ERR_INVALID_ARGUMENT, "NULL output");
+  int sms = 0;
+  rc = current_sm_count(&sms);
+  if (rc != FLCE_OK) return rc;
+  const long long blocks = balance_blocks(p, sms);
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 7) != 0 || bytes < workspace_bytes(p, blocks))
+    return fail(FLCE_ERR_WORKSPACE, "the balance loss needs %zu bytes of 8-byte aligned workspace, got %zu", workspace_bytes(p, blocks),
+                bytes);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  const int experts = static_cast<int>(p->n_experts);
+  double* sums = static_cast<double*>(workspace);
+  long long* kept = reinterpret_cast<long long*>(sums + p->n_layers * (p->n_experts + 1));
+  float* partial = reinterpret_cast<float*>(kept + p->n_layers);
+  const BalanceShape s = balance_shape(p, logits, nullptr);
+  int launches = 2;
+  for (int64_t l = 0; l < p->n_layers; l += kBalMaxLayers) {
+    const int64_t layers = p->n_layers - l < kBalMaxLayers ? p->n_layers - l : kBalMaxLayers;
+    const BalanceArgs a = balance_args(p, logits, l, layers, s);
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(layers));
+    float* mine = partial + l * blocks * balance_partial_words(experts);
+    with_type(p->dtype, [&](auto t) {
+      using T = decltype(t);
+      if (s.vectors) run_forward<T, true>(a, s, grid, mine, stream);
+      else run_forward<T, false>(a, s, grid, mine, stream);
+    });
+    ++launches;
+  }
+  FLCE_LAUNCH((balance_layer_kernel), static_cast<unsigned>(p->n_layers), kBalThreads, stream, partial, static_cast<int>(blocks), experts,
+              reinterpret_cast<long long*>(counts), sums, kept);
+  FLCE_LAUNCH((balance_total_kernel), 1u, kBalThreads, stream, reinterpret_cast<const long long*>(counts), sums, kept,
+              static_cast<int>(p->n_layers), experts, p->lse_square_scale, loss, coef);
+  FLCE_CUDA(cudaGetLastError());
+  count_launches(launches);
+  return FLCE_OK;
+}
+
+int flce_b200_balance_backward(const flce_balance_t* p, const void* const* logits, const float* coef, const float* grad_loss,
+                               void* grads, void* stream_) {
+  int rc = check_balance(p);
+  if (rc != FLCE_OK) return rc;
+  rc = check_layers(p, logits);
+  if (rc != FLCE_OK) return rc;
+  if (p->n_tokens == 0) return FLCE_OK;
+  if (coef == nullptr || grad_loss == nullptr || grads == nullptr) return fail(FLCE_ERR_INVALID_ARGUMENT, "NULL argument");
+  if ((reinterpret_cast<uintptr_t>(grads) % element_size(p->dtype)) != 0)
+    return fail(FLCE_ERR_INVALID_ARGUMENT, "the gradients do not start on a multiple of their element size");
+  int sms = 0;
+  rc = current_sm_count(&sms);
+  if (rc != FLCE_OK) return rc;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  const BalanceShape s = balance_shape(p, logits, grads);
+  const long long blocks = balance_blocks(p, sms);
+  int launches = 0;
+  for (int64_t l = 0; l < p->n_layers; l += kBalMaxLayers) {
+    const int64_t layers = p->n_layers - l < kBalMaxLayers ? p->n_layers - l : kBalMaxLayers;
+    const BalanceArgs a = balance_args(p, logits, l, layers, s);
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(layers));
+    with_type(p->dtype, [&](auto t) {
+      using T = decltype(t);
+      T* out = static_cast<T*>(grads) + l * p->n_tokens * p->n_experts;
+      if (s.vectors) run_backward<T, true>(a, s, grid, coef, grad_loss, out, stream);
+      else run_backward<T, false>(a, s, grid, coef, grad_loss, out, stream);
+    });
+    ++launches;
+  }
+  FLCE_CUDA(cudaGetLastError());
+  count_launches(launches);
+  return FLCE_OK;
+}
+
+}  // extern "C"

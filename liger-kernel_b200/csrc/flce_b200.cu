@@ -202,7 +202,6 @@ static int operand_map(CUtensorMap* map, const Operand& op, int dtype, int tile_
   return make_map(map, op.base, dtype, op.rows, op.depth, op.pitch, 64, kBlockK);
 }
 
-static long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 static size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 // n-tiles per raster group of an n-fastest GEMM, chosen by estimated DRAM traffic.  A group walks all m-tiles over g n-tiles, so

@@ -23,6 +23,9 @@ void count_launches(int n);
 // stream, so the first call on a device may come while a stream is being captured.
 int current_sm_count(int* sm_count);
 
+inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+inline int element_size(int dtype) { return dtype == FLCE_FP32 ? 4 : 2; }
+
 // A launch that the host emulation of the tests can stand in for.  `kernel` is parenthesised: it holds commas.
 #ifndef FLCE_HOST_EMULATION
 #define FLCE_LAUNCH(kernel, grid, block, stream, ...) kernel<<<grid, block, 0, stream>>>(__VA_ARGS__)

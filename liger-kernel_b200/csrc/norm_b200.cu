@@ -8,9 +8,7 @@
 namespace flce {
 namespace {
 
-long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-int element_size(int dtype) { return dtype == FLCE_FP32 ? 4 : 2; }
 
 int check_norm(const flce_norm_t* p) {
   if (p == nullptr) return fail(FLCE_ERR_INVALID_ARGUMENT, "norm is NULL");

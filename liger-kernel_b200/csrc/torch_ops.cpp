@@ -1,4 +1,4 @@
-// torch-side binding of the norms: argument checks, allocation, autograd nodes.  The kernels stay behind the C ABI of
+// torch-side binding of the norms and of the router's balance loss: argument checks, allocation, autograd nodes.  The kernels stay behind the C ABI of
 // libflce_b200.so, whose entry points are looked up at load time (liger_b200_bind); no torch type crosses it.
 //
 // Why not ctypes and a Python autograd.Function, as for the losses: those run once per step, a norm runs dozens of times and
@@ -32,6 +32,9 @@ struct Library {
   decltype(&flce_b200_norm_forward) norm_forward = nullptr;
   decltype(&flce_b200_norm_workspace_bytes) norm_workspace_bytes = nullptr;
   decltype(&flce_b200_norm_backward) norm_backward = nullptr;
+  decltype(&flce_b200_balance_workspace_bytes) balance_workspace_bytes = nullptr;
+  decltype(&flce_b200_balance_forward) balance_forward = nullptr;
+  decltype(&flce_b200_balance_backward) balance_backward = nullptr;
   decltype(&flce_b200_status_string) status_string = nullptr;
   decltype(&flce_b200_last_error) last_error = nullptr;
   bool host_memory = false;     // the tests' emulation of the library computes on host memory
@@ -211,7 +214,134 @@ Tensor norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tens
   return y;
 }
 
+// ------------------------------------------------------------------ the router's load-balancing loss
+struct BalanceOperands {
+  flce_balance_t p{};
+  std::vector<Tensor> logits;   // [tokens, experts] each, one pitch for all
+  std::vector<const void*> pointers;
+  Tensor mask;
+};
+
+BalanceOperands balance_operands(at::TensorList logits, int64_t num_experts, int64_t top_k, const Tensor& mask, double lse_square_scale) {
+  TORCH_CHECK_VALUE(!logits.empty(), "expected the router logits of at least one layer");
+  BalanceOperands o;
+  const Tensor& head = logits[0];
+  require_device(head);
+  o.p.dtype = dtype_of(head, "");
+  bool same_pitch = true;
+  for (const Tensor& t : logits) {
+    TORCH_CHECK_VALUE(t.dim() >= 1 && t.size(-1) == num_experts, "router logits must be [..., ", num_experts, "], got ", t.sizes());
+    TORCH_CHECK_VALUE(t.scalar_type() == head.scalar_type() && t.device() == head.device() && t.numel() == head.numel(),
+                      "the router logits of all layers must agree in type, device and number of tokens");
+    o.logits.push_back(as_rows(t, num_experts));
+    same_pitch = same_pitch && o.logits.back().stride(0) == o.logits[0].stride(0);
+  }
+  TORCH_CHECK_VALUE(num_experts >= 1, "num_experts must be at least 1, got ", num_experts);
+  TORCH_CHECK_VALUE(top_k >= 1 && top_k <= num_experts, "top_k must be in [1, ", num_experts, "], got ", top_k);
+  TORCH_CHECK_NOT_IMPLEMENTED(num_experts <= 1024, "at most 1024 experts, got ", num_experts);
+  o.p.n_layers = static_cast<int64_t>(o.logits.size());
+  o.p.n_tokens = o.logits[0].size(0);
+  o.p.n_experts = num_experts;
+  o.p.top_k = top_k;
+  for (Tensor& t : o.logits) {
+    if (!same_pitch) t = t.contiguous();
+    o.pointers.push_back(t.const_data_ptr());
+  }
+  o.p.ld = same_pitch ? o.logits[0].stride(0) : num_experts;
+  o.p.lse_square_scale = static_cast<float>(lse_square_scale);
+  if (mask.defined()) {
+    TORCH_CHECK_VALUE(mask.numel() == o.p.n_tokens, "the attention mask has ", mask.numel(), " elements, a layer's router logits ",
+                      o.p.n_tokens, " tokens");
+    const auto type = mask.scalar_type();
+    o.mask = type == at::kBool || type == at::kByte || type == at::kChar || type == at::kInt || type == at::kLong ? mask : mask.ne(0);
+    o.mask = o.mask.to(head.device()).contiguous();
+    o.p.mask_bytes = static_cast<int32_t>(o.mask.element_size());
+    o.p.mask = o.p.n_tokens > 0 ? o.mask.const_data_ptr() : nullptr;
+  }
+  return o;
+}
+
+struct BalanceBackward : public torch::autograd::Node {
+  std::vector<SavedVariable> logits;
+  SavedVariable mask;
+  Tensor coef;
+  int64_t num_experts = 0, top_k = 0;
+  double lse_square_scale = 0;
+
+  std::string name() const override { return "LigerLoadBalancingLossBackward"; }
+
+  void release_variables() override {
+    for (auto& t : logits) t.reset_data();
+    mask.reset_data();
+    coef.reset();
+  }
+
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(logits.size());
+    const Tensor& grad = grads[0];
+    if (!grad.defined()) return out;
+    std::vector<Tensor> x;
+    bool recording = grad.requires_grad();
+    for (auto& t : logits) {
+      x.push_back(t.unpack());
+      recording = recording || x.back().requires_grad();
+    }
+    const Tensor m = mask.unpack();
+    TORCH_CHECK(coef.defined(), torch::autograd::ERR_BACKWARD_TWICE);
+    recording = recording && at::GradMode::is_enabled();
+    at::AutoDispatchBelowAutograd below;
+    OnDevice on(x[0]);
+    const BalanceOperands o = balance_operands(x, num_experts, top_k, m, lse_square_scale);
+    const Tensor up = grad.to(at::kFloat).contiguous();
+    Tensor all = at::empty({o.p.n_layers, o.p.n_tokens, num_experts}, x[0].options().memory_format(at::MemoryFormat::Contiguous));
+    check(g_lib.balance_backward(&o.p, o.pointers.data(), coef.const_data_ptr<float>(), up.const_data_ptr<float>(), all.data_ptr(),
+                                 on.stream));
+    for (size_t l = 0; l < x.size(); ++l) {
+      if (task_should_compute_output(l)) out[l] = all.select(0, static_cast<int64_t>(l)).reshape(x[l].sizes());
+    }
+    return once_differentiable(std::move(out), recording);
+  }
+};
+
+// loss, its lse^2 term, counts [layers, experts]
+std::tuple<Tensor, Tensor, Tensor> load_balancing_loss(at::TensorList logits, int64_t num_experts, int64_t top_k,
+                                                       const optional<Tensor>& attention_mask, double lse_square_scale) {
+  const Tensor mask = attention_mask.value_or(Tensor());
+  const bool recording = torch::autograd::compute_requires_grad(logits);
+  Tensor loss, z_loss, counts, coef;
+  {
+    at::AutoDispatchBelowAutograd below;
+    const BalanceOperands o = balance_operands(logits, num_experts, top_k, mask, lse_square_scale);
+    OnDevice on(logits[0]);
+    const auto options = o.logits[0].options();
+    const Tensor out = at::empty({2}, options.dtype(at::kFloat));
+    counts = at::empty({o.p.n_layers, num_experts}, options.dtype(at::kLong));
+    coef = at::empty({num_experts + 1}, options.dtype(at::kFloat));
+    const size_t bytes = g_lib.balance_workspace_bytes(&o.p);
+    const Tensor workspace = at::empty({static_cast<int64_t>(bytes)}, options.dtype(at::kByte));
+    check(g_lib.balance_forward(&o.p, o.pointers.data(), out.data_ptr<float>(), counts.data_ptr<int64_t>(), coef.data_ptr<float>(),
+                                workspace.data_ptr(), bytes, on.stream));
+    loss = out.select(0, 0);
+    z_loss = out.select(0, 1);
+  }
+  if (recording) {
+    auto node = std::shared_ptr<BalanceBackward>(new BalanceBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(logits));
+    for (const Tensor& t : logits) node->logits.emplace_back(t, false);
+    node->mask = SavedVariable(mask, false);
+    node->coef = coef;
+    node->num_experts = num_experts;
+    node->top_k = top_k;
+    node->lse_square_scale = lse_square_scale;
+    torch::autograd::set_history(loss, node);
+  }
+  return {loss, z_loss, counts};
+}
+
 TORCH_LIBRARY(liger_b200, m) {
+  m.def("load_balancing_loss(Tensor[] logits, int num_experts, int top_k, Tensor? attention_mask, float lse_square_scale) -> "
+        "(Tensor, Tensor, Tensor)", load_balancing_loss);
   m.def("norm(Tensor x, Tensor? weight, Tensor? bias, int kind, float eps, float offset, bool round_xhat) -> Tensor", norm);
 }
 
@@ -236,6 +366,9 @@ extern "C" const char* liger_b200_bind(const char* path, int host_memory) {
   find(lib.norm_forward, "flce_b200_norm_forward");
   find(lib.norm_workspace_bytes, "flce_b200_norm_workspace_bytes");
   find(lib.norm_backward, "flce_b200_norm_backward");
+  find(lib.balance_workspace_bytes, "flce_b200_balance_workspace_bytes");
+  find(lib.balance_forward, "flce_b200_balance_forward");
+  find(lib.balance_backward, "flce_b200_balance_backward");
   find(lib.status_string, "flce_b200_status_string");
   find(lib.last_error, "flce_b200_last_error");
   if (missing != nullptr) {

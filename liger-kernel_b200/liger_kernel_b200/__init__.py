@@ -11,6 +11,8 @@ from .ops.fused_linear_jsd import LigerFusedLinearJSDFunction  # noqa: F401
 from .ops.fused_linear_scaled_cross_entropy import LigerFusedLinearScaledCrossEntropyFunction  # noqa: F401
 from .ops.fused_rmsnorm_linear_cross_entropy import LigerFusedRMSNormLinearCrossEntropyFunction  # noqa: F401
 from .ops.fused_rmsnorm_linear_cross_entropy import liger_fused_rmsnorm_linear_cross_entropy  # noqa: F401
+from .ops.load_balancing_loss import LigerLoadBalancingLossFunction  # noqa: F401
+from .ops.load_balancing_loss import LoadBalancingOutput  # noqa: F401
 from .ops.norm import LigerLayerNormFunction  # noqa: F401
 from .ops.norm import LigerRMSNormFunction  # noqa: F401
 from .transformers.cross_entropy import LigerCrossEntropyLoss  # noqa: F401
@@ -19,8 +21,10 @@ from .transformers.functional import CrossEntropyOutput  # noqa: F401
 from .transformers.functional import liger_fused_linear_cross_entropy  # noqa: F401
 from .transformers.functional import liger_fused_linear_jsd  # noqa: F401
 from .transformers.functional import liger_layer_norm  # noqa: F401
+from .transformers.functional import liger_load_balancing_loss  # noqa: F401
 from .transformers.functional import liger_rms_norm  # noqa: F401
 from .transformers.fused_linear_jsd import LigerFusedLinearJSD  # noqa: F401
+from .transformers.load_balancing_loss import LigerLoadBalancingLoss  # noqa: F401
 from .transformers.layer_norm import LigerLayerNorm  # noqa: F401
 from .transformers.rms_norm import LigerRMSNorm  # noqa: F401
 from .transformers.fused_linear_cross_entropy import LigerFusedLinearCrossEntropyLoss  # noqa: F401

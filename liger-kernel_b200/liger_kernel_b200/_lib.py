@@ -53,6 +53,9 @@ EXPORTS = (
     "flce_b200_norm_forward",
     "flce_b200_norm_workspace_bytes",
     "flce_b200_norm_backward",
+    "flce_b200_balance_workspace_bytes",
+    "flce_b200_balance_forward",
+    "flce_b200_balance_backward",
     "flce_b200_check_device_status",
     "flce_b200_profile_enable",
     "flce_b200_profile_read",
@@ -122,6 +125,14 @@ class Norm(C.Structure):
         ("kind", C.c_int32), ("dtype", C.c_int32), ("weight_dtype", C.c_int32), ("round_xhat", C.c_int32),
         ("eps", C.c_float), ("offset", C.c_float),
         ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p),
+    ]
+
+
+class Balance(C.Structure):
+    _fields_ = [
+        ("n_layers", C.c_int64), ("n_tokens", C.c_int64), ("n_experts", C.c_int64), ("top_k", C.c_int64), ("ld", C.c_int64),
+        ("dtype", C.c_int32), ("mask_bytes", C.c_int32), ("lse_square_scale", C.c_float), ("reserved", C.c_float),
+        ("mask", C.c_void_p),
     ]
 
 
@@ -217,6 +228,13 @@ def _load():
     lib.flce_b200_norm_workspace_bytes.restype = sz
     lib.flce_b200_norm_backward.argtypes = [NP, vp, i64, vp, vp, vp, vp, vp, vp, sz, vp]
     lib.flce_b200_norm_backward.restype = C.c_int
+    BP, VPP = C.POINTER(Balance), C.POINTER(C.c_void_p)
+    lib.flce_b200_balance_workspace_bytes.argtypes = [BP]
+    lib.flce_b200_balance_workspace_bytes.restype = sz
+    lib.flce_b200_balance_forward.argtypes = [BP, VPP, vp, vp, vp, vp, sz, vp]
+    lib.flce_b200_balance_forward.restype = C.c_int
+    lib.flce_b200_balance_backward.argtypes = [BP, VPP, vp, vp, vp, vp]
+    lib.flce_b200_balance_backward.restype = C.c_int
     lib.flce_b200_check_device_status.argtypes = [vp]
     lib.flce_b200_selftest_wait_expiry.argtypes = [i64, vp, vp]
     lib.flce_b200_selftest_wait_expiry.restype = C.c_int

@@ -38,3 +38,4 @@ def _load():
 _binding = _load()
 bind(_lib.LIB_PATH)
 norm = torch.ops.liger_b200.norm.default
+load_balancing_loss = torch.ops.liger_b200.load_balancing_loss.default

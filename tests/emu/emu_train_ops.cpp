@@ -1,4 +1,4 @@
-// The C entry points of the norms, their host side and their kernels, compiled for the host and run on the host
+// The C entry points of the norms and of the router's balance loss, their host side and their kernels, compiled for the host and run on the host
 // through simt_emulation.hpp: the library's own launch shapes, index arithmetic and argument checks, with fibers in
 // the place of CUDA threads.  The "device" has three SMs, so that persistent grids walk over several rows.
 //
@@ -10,6 +10,19 @@
 #include <cstdarg>
 #include <cstdio>
 #include <type_traits>
+
+// warp votes, through the same slots as the shuffles
+inline unsigned __ballot_sync(unsigned, bool v) {
+  unsigned bits = 0;
+  for (unsigned o = 0; o < 32; ++o) {
+    const unsigned from = (emu::linear_tid() & 31u) ^ o;
+    if (emu::shuffle_from(static_cast<unsigned>(v), from)) bits |= 1u << from;
+  }
+  return bits;
+}
+inline bool __any_sync(unsigned m, bool v) { return __ballot_sync(m, v) != 0; }
+inline int __popc(unsigned v) { return __builtin_popcount(v); }
+inline int __clz(unsigned v) { return v ? __builtin_clz(v) : 32; }
 
 inline emu::Dim3 emu_dim3(dim3 d) { return emu::Dim3(d.x, d.y, d.z); }
 
@@ -49,3 +62,4 @@ int emu_launches(void) { return flce::g_launches; }
 }
 
 #include "norm_b200.cu"
+#include "balance_b200.cu"
