@@ -438,7 +438,7 @@ typedef struct flce_norm {
 /* mean, rstd: [n_rows] fp32, needed by the backward call; either may be NULL (RMSNorm has no mean). */
 int flce_b200_norm_forward(const flce_norm_t* p, void* y, float* mean, float* rstd, void* stream);
 
-/* grad_weight / grad_bias [hidden] in weight_dtype, NULL where not wanted.  The workspace (4-byte aligned, of
+/* grad_weight / grad_bias [hidden] in weight_dtype, NULL where not wanted.  The workspace (16-byte aligned, of
  * flce_b200_norm_workspace_bytes; only read by the call that wrote it) may be NULL when neither is.  Sums run in a fixed
  * order: the same bits in every run. */
 size_t flce_b200_norm_workspace_bytes(const flce_norm_t* p);

@@ -3,6 +3,8 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "flce_b200.h"
 
 namespace flce {
@@ -33,5 +35,25 @@ inline int element_size(int dtype) { return dtype == FLCE_FP32 ? 4 : 2; }
 #define FLCE_LAUNCH(kernel, grid, block, stream, ...) \
   emu::launch(emu_dim3(grid), emu_dim3(block), [&]() { (void)(stream), (kernel)(__VA_ARGS__); })
 #endif
+
+// The same for a kernel with `bytes` of dynamic shared memory; the permission for more than 48 KB is asked for once per kernel
+// and device (kKernel names the instantiation).
+template <auto kKernel, class Args>
+int launch_with_shared(dim3 grid, unsigned block, size_t bytes, cudaStream_t stream, const Args& args) {
+#ifndef FLCE_HOST_EMULATION
+  static std::atomic<bool> allowed[64];
+  int device = 0;
+  FLCE_CUDA(cudaGetDevice(&device));
+  if (!allowed[device & 63].load(std::memory_order_acquire)) {
+    FLCE_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+    allowed[device & 63].store(true, std::memory_order_release);
+  }
+  kKernel<<<grid, block, bytes, stream>>>(args);
+#else
+  (void)bytes;
+  FLCE_LAUNCH((kKernel), grid, block, stream, args);
+#endif
+  return FLCE_OK;
+}
 
 }  // namespace flce

@@ -50,6 +50,46 @@ NormShape norm_shape(const flce_norm_t* p, bool whole_vectors, int preferred_thr
   }
 }
 
+// Rows of whole vectors go to the streaming kernels, or to the narrow ones if a warp's lanes hold one with a vector each.
+enum NormPath { kNormGeneric, kNormStream, kNormNarrow };
+constexpr int kNarrowForwardRows = 4, kNarrowBackwardRows = 2;
+
+struct NormPlan {
+  NormPath path;
+  NormShape shape;      // ept holds the vectors per lane, except on the generic path
+};
+
+int log2_ceil(long long v) {
+  int l = 0;
+  while ((1ll << l) < v) ++l;
+  return l;
+}
+
+// The streaming kernels give every thread of a 512-thread block its columns: one vector if that reaches, up to four.
+NormPlan norm_plan(const flce_norm_t* p, bool vectors, int preferred_threads) {
+  NormPlan plan{kNormGeneric, {}};
+  const long long n = p->hidden * element_size(p->dtype) / 16;
+  if (vectors && n <= 32) {
+    plan.path = kNormNarrow;
+    plan.shape = {1, 1, log2_ceil(n), true};
+  } else if (vectors && n <= 4 * kStreamThreads) {
+    int units = 1;
+    while (units * kStreamThreads < n) units *= 2;
+    int log2_group = 5;
+    while ((units << log2_group) < n) ++log2_group;
+    plan.path = kNormStream;
+    plan.shape = {1, units, log2_group, true};
+  } else {
+    plan.shape = norm_shape(p, vectors, preferred_threads);
+  }
+  return plan;
+}
+
+template <bool kGrad>
+int stream_rows(int units) {
+  return units == 1 ? Stream<1, kGrad>::kRows : (units == 2 ? Stream<2, kGrad>::kRows : Stream<4, kGrad>::kRows);
+}
+
 bool whole_vectors(const flce_norm_t* p, const void* other, long long ld_other) {
   const int vec = 16 / element_size(p->dtype);
   const bool pitches = p->n_rows <= 1 || (p->ld_x % vec == 0 && ld_other % vec == 0);     // one row has no pitch
@@ -88,12 +128,43 @@ void with_types(const flce_norm_t* p, Fn fn) {
 }
 
 // Blocks of the backward kernel: they are resident together and walk over the rows.  Each leaves hidden partial sums per
-// parameter, so no more than two per SM.
-long long backward_blocks(const flce_norm_t* p, const NormShape& s, int sm_count) {
-  const long long groups = s.fits ? kNormMaxThreads >> s.log2_group : 1;
-  const long long most = ceil_div(p->n_rows, groups);
-  const long long resident = 2ll * sm_count;
+// parameter, so no more of them than it takes to fill the device.
+long long backward_blocks(const flce_norm_t* p, const NormPlan& plan, int sm_count) {
+  long long rows = 1, per_sm = 2;
+  if (plan.path == kNormNarrow) {
+    rows = (kNarrowThreads >> plan.shape.log2_group) * kNarrowBackwardRows;
+    per_sm = 4;
+  } else if (plan.path == kNormStream) {
+    rows = (kStreamThreads >> plan.shape.log2_group) * stream_rows<true>(plan.shape.ept);
+    per_sm = plan.shape.ept == 1 ? 2 : 1;
+  } else if (plan.shape.fits) {
+    rows = kNormMaxThreads >> plan.shape.log2_group;
+  }
+  const long long most = ceil_div(p->n_rows, rows);
+  const long long resident = per_sm * sm_count;
   return most < resident ? most : resident;
+}
+
+template <typename T, typename W, bool kCentered>
+int run_forward_stream(const NormForwardArgs& a, const NormShape& s, int sm_count, cudaStream_t stream) {
+  const long long most = ceil_div(a.n_rows, (kStreamThreads >> s.log2_group) * stream_rows<false>(s.ept));
+  const long long resident = (s.ept == 1 ? 2ll : 1ll) * sm_count;
+  const dim3 grid(static_cast<unsigned>(most < resident ? most : resident));
+  switch (s.ept) {
+    case 1: return launch_with_shared<norm_forward_stream_kernel<T, W, kCentered, 1>>(grid, kStreamThreads, Stream<1, false>::kRingBytes, stream, a);
+    case 2: return launch_with_shared<norm_forward_stream_kernel<T, W, kCentered, 2>>(grid, kStreamThreads, Stream<2, false>::kRingBytes, stream, a);
+    default: return launch_with_shared<norm_forward_stream_kernel<T, W, kCentered, 4>>(grid, kStreamThreads, Stream<4, false>::kRingBytes, stream, a);
+  }
+}
+
+template <typename T, typename W, bool kCentered>
+int run_backward_stream(const NormBackwardArgs& a, const NormShape& s, unsigned blocks, cudaStream_t stream) {
+  const dim3 grid(blocks);
+  switch (s.ept) {
+    case 1: return launch_with_shared<norm_backward_stream_kernel<T, W, kCentered, 1>>(grid, kStreamThreads, Stream<1, true>::kRingBytes, stream, a);
+    case 2: return launch_with_shared<norm_backward_stream_kernel<T, W, kCentered, 2>>(grid, kStreamThreads, Stream<2, true>::kRingBytes, stream, a);
+    default: return launch_with_shared<norm_backward_stream_kernel<T, W, kCentered, 4>>(grid, kStreamThreads, Stream<4, true>::kRingBytes, stream, a);
+  }
 }
 
 }  // namespace
@@ -125,7 +196,8 @@ int flce_b200_norm_forward(const flce_norm_t* p, void* y, float* mean, float* rs
   a.eps = p->eps;
   a.offset = p->offset;
   a.round_xhat = p->round_xhat;
-  const NormShape s = norm_shape(p, whole_vectors(p, y, p->hidden), kNormForwardThreads);
+  const NormPlan plan = norm_plan(p, whole_vectors(p, y, p->hidden), kNormForwardThreads);
+  const NormShape& s = plan.shape;
   a.log2_group = s.log2_group;
   const int threads = (1 << s.log2_group) > kNormForwardThreads ? (1 << s.log2_group) : kNormForwardThreads;
   const bool centered = p->kind == FLCE_LAYER_NORM;
@@ -133,6 +205,16 @@ int flce_b200_norm_forward(const flce_norm_t* p, void* y, float* mean, float* rs
     using T = decltype(t);
     using W = decltype(w);
     constexpr int kVec = CeElem<T>::kVec;
+    if (plan.path == kNormStream) {
+      rc = centered ? run_forward_stream<T, W, true>(a, s, sms, stream) : run_forward_stream<T, W, false>(a, s, sms, stream);
+      return;
+    }
+    if (plan.path == kNormNarrow) {
+      const unsigned grid = static_cast<unsigned>(ceil_div(p->n_rows, (kNarrowThreads >> s.log2_group) * kNarrowForwardRows));
+      if (centered) FLCE_LAUNCH((norm_forward_narrow_kernel<T, W, true, kNarrowForwardRows>), grid, kNarrowThreads, stream, a);
+      else FLCE_LAUNCH((norm_forward_narrow_kernel<T, W, false, kNarrowForwardRows>), grid, kNarrowThreads, stream, a);
+      return;
+    }
     if (!s.fits) {
       const unsigned grid = static_cast<unsigned>(p->n_rows);
       if (centered) FLCE_LAUNCH((norm_forward_long_kernel<T, W, true>), grid, kNormMaxThreads, stream, a);
@@ -148,6 +230,7 @@ int flce_b200_norm_forward(const flce_norm_t* p, void* y, float* mean, float* rs
       else run_forward<T, W, false, kVec>(a, s, grid, threads, stream);
     }
   });
+  if (rc != FLCE_OK) return rc;
   FLCE_CUDA(cudaGetLastError());
   count_launches(1);
   return FLCE_OK;
@@ -158,8 +241,8 @@ size_t flce_b200_norm_workspace_bytes(const flce_norm_t* p) {
   int sms = 0;
   if (current_sm_count(&sms) != FLCE_OK) return 0;
   // the row's spread may turn out either way (the gradient's alignment is not known yet): room for the larger grid
-  const long long blocks_vec = backward_blocks(p, norm_shape(p, true, kNormMaxThreads), sms);
-  const long long blocks_one = backward_blocks(p, norm_shape(p, false, kNormMaxThreads), sms);
+  const long long blocks_vec = backward_blocks(p, norm_plan(p, true, kNormMaxThreads), sms);
+  const long long blocks_one = backward_blocks(p, norm_plan(p, false, kNormMaxThreads), sms);
   const long long blocks = blocks_vec > blocks_one ? blocks_vec : blocks_one;
   return static_cast<size_t>(blocks) * static_cast<size_t>(p->hidden) * sizeof(float) * (p->kind == FLCE_LAYER_NORM ? 2 : 1);
 }
@@ -185,14 +268,15 @@ int flce_b200_norm_backward(const flce_norm_t* p, const void* grad_y, int64_t ld
   int sms = 0;
   rc = current_sm_count(&sms);
   if (rc != FLCE_OK) return rc;
-  const NormShape s = norm_shape(p, whole_vectors(p, grad_y, ld_grad) && aligned16(grad_x), kNormMaxThreads);
-  const long long blocks = backward_blocks(p, s, sms);
+  const NormPlan plan = norm_plan(p, whole_vectors(p, grad_y, ld_grad) && aligned16(grad_x), kNormMaxThreads);
+  const NormShape& s = plan.shape;
+  const long long blocks = backward_blocks(p, plan, sms);
   const bool parameters = grad_weight != nullptr || grad_bias != nullptr;
   const size_t plane = static_cast<size_t>(blocks) * static_cast<size_t>(p->hidden);
   const size_t planes = (grad_weight != nullptr ? 1 : 0) + (grad_bias != nullptr ? 1 : 0);
-  if (parameters && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 3) != 0 ||
+  if (parameters && (workspace == nullptr || !aligned16(workspace) ||
                      workspace_bytes < plane * planes * sizeof(float)))
-    return fail(FLCE_ERR_WORKSPACE, "the norm's backward needs %zu bytes of workspace, got %zu", plane * planes * sizeof(float),
+    return fail(FLCE_ERR_WORKSPACE, "the norm's backward needs %zu bytes of 16-byte aligned workspace, got %zu", plane * planes * sizeof(float),
                 workspace_bytes);
   NormBackwardArgs a;
   a.dy = grad_y;
@@ -215,7 +299,13 @@ int flce_b200_norm_backward(const flce_norm_t* p, const void* grad_y, int64_t ld
     using T = decltype(t);
     using W = decltype(w);
     constexpr int kVec = CeElem<T>::kVec;
-    if (!s.fits) {
+    if (plan.path == kNormStream) {
+      rc = centered ? run_backward_stream<T, W, true>(a, s, grid, stream) : run_backward_stream<T, W, false>(a, s, grid, stream);
+      if (rc != FLCE_OK) return;
+    } else if (plan.path == kNormNarrow) {
+      if (centered) FLCE_LAUNCH((norm_backward_narrow_kernel<T, W, true, kNarrowBackwardRows>), grid, kNarrowThreads, stream, a);
+      else FLCE_LAUNCH((norm_backward_narrow_kernel<T, W, false, kNarrowBackwardRows>), grid, kNarrowThreads, stream, a);
+    } else if (!s.fits) {
       const unsigned rows = static_cast<unsigned>(p->n_rows);
       const dim3 columns(static_cast<unsigned>(ceil_div(p->hidden, kNormForwardThreads)), grid < 65535u ? grid : 65535u);
       if (centered) FLCE_LAUNCH((norm_backward_long_kernel<T, W, true>), rows, kNormMaxThreads, stream, a);
@@ -237,6 +327,7 @@ int flce_b200_norm_backward(const flce_norm_t* p, const void* grad_y, int64_t ld
           a.dw_partial, a.db_partial, static_cast<int>(grid), a.hidden, static_cast<W*>(grad_weight), static_cast<W*>(grad_bias));
     }
   });
+  if (rc != FLCE_OK) return rc;
   FLCE_CUDA(cudaGetLastError());
   count_launches(1 + (parameters ? (s.fits ? 1 : 2) : 0));
   return FLCE_OK;

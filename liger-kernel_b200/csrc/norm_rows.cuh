@@ -20,6 +20,7 @@
 #include <type_traits>
 
 #include "ce_kernels.cuh"
+#include "packed_math.cuh"
 #include "simt_common.cuh"
 
 namespace flce {
@@ -319,6 +320,580 @@ norm_backward_kernel(NormBackwardArgs a) {
       for (int e = 0; e < kEpt; ++e) {
         const int col = norm_column<kUnit>(first, e);
         if (col < a.hidden) mine[col] = acc[e];
+      }
+    }
+  };
+  if (a.dw_partial != nullptr) leave(dw, a.dw_partial);
+  if constexpr (kCentered) {
+    if (a.db_partial != nullptr) leave(db, a.db_partial);
+  }
+}
+
+// ---- rows of whole, aligned 16-byte vectors, more than a warp's worth: streamed through shared memory
+//
+// What the kernels above lose is not bandwidth but issue slots and waiting: at 32768 x 4096 bf16 they ran at 46 % (forward) and
+// 41 % (backward) of the copy rate with rows of one warp reaching 55 % and fp32 rows, with half the elements per byte, 87 %.
+// Here the arithmetic goes two elements to an instruction, and the next rows are always on their way: every thread copies
+// the vectors that it will read itself, with cp.async, so the ring needs no barrier and no wait on another thread.
+
+constexpr int kStreamThreads = 512;
+
+// Four sums over a group of `warps` warps.  In a warp by six exchanges: lanes that differ in bit 4 trade two sums for the other
+// two, those that differ in bit 3 one for the other; bits 4 and 3 of the lane then name its sum.  Across warps through one of
+// two buffers, taken in turn (see norm_group_sum).  Returns sum number lane >> 3, the same in the eight lanes that share it.
+__device__ __forceinline__ float stream_four_sums(const float (&v)[4], int warps, int group_id, float (*scratch)[kNormMaxWarps * 4],
+                                                  int& phase) {
+  const int lane = static_cast<int>(threadIdx.x) & 31;
+  const bool up = (lane & 16) != 0, right = (lane & 8) != 0;
+  const float a0 = __shfl_xor_sync(0xffffffffu, up ? v[0] : v[2], 16) + (up ? v[2] : v[0]);
+  const float a1 = __shfl_xor_sync(0xffffffffu, up ? v[1] : v[3], 16) + (up ? v[3] : v[1]);
+  float sum = __shfl_xor_sync(0xffffffffu, right ? a0 : a1, 8) + (right ? a1 : a0);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (warps == 1) return sum;
+  float* buf = scratch[phase];
+  phase ^= 1;
+  if ((lane & 7) == 0) buf[(threadIdx.x >> 5) * 4 + (lane >> 3)] = sum;
+  named_barrier(1 + group_id, warps * 32);
+  const float* of = buf + group_id * warps * 4 + (lane >> 3);
+  sum = 0.f;
+  for (int w = lane & 7; w < warps; w += 8) sum += of[w * 4];
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+
+// kUnits vectors of a parameter, zeros where there is none
+template <typename W, int kUnits, int kWVecs>
+__device__ __forceinline__ void stream_load_parameter(const void* src, int first, int vectors, uint4 (&raw)[kUnits * kWVecs]) {
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+#pragma unroll
+    for (int i = 0; i < kWVecs; ++i) {
+      raw[u * kWVecs + i] = make_uint4(0u, 0u, 0u, 0u);
+      if (src != nullptr && first + u * 32 < vectors)
+        raw[u * kWVecs + i] = __ldg(reinterpret_cast<const uint4*>(src) + (first + u * 32) * kWVecs + i);
+    }
+  }
+}
+
+// Shape of the streaming kernels by the vectors per thread: rows that a group takes per round, rounds in the ring, blocks per SM.
+// Two rows of backward are four sums, as four rows of forward are.
+template <int kUnits, bool kGrad>
+struct Stream {
+  static constexpr int kRows = kUnits == 4 ? 1 : (kUnits == 2 || kGrad ? 2 : 4);
+  static constexpr int kSlots = 3;
+  static constexpr int kBlocksPerSm = kUnits == 1 ? 2 : 1;
+  static constexpr int kRingBytes = kSlots * kRows * (kGrad ? 2 : 1) * kUnits * kStreamThreads * 16;
+};
+
+// y and the row statistics.  Each thread of a group owns kUnits vectors of columns, their gain and bias in registers; a group takes
+// kRows rows per round, which meet in one reduction (one barrier, if the group is wider than a warp) for the means and one for
+// the variances.  A fixed grid walks over the rows.
+template <typename T, typename W, bool kCentered, int kUnits>
+__global__ void __launch_bounds__(kStreamThreads, (Stream<kUnits, false>::kBlocksPerSm))
+norm_forward_stream_kernel(NormForwardArgs a) {
+  constexpr int kRows = Stream<kUnits, false>::kRows, kSlots = Stream<kUnits, false>::kSlots;
+  constexpr int kVec = CeElem<T>::kVec;
+  constexpr int kPairs = kVec / 2;
+  constexpr int kWVecs = kVec * static_cast<int>(sizeof(W)) / 16;
+  FLCE_DYNAMIC_SHARED(uint4, stream_ring);                    // [slot][row][unit][thread]
+  __shared__ float scratch[2][kNormMaxWarps * 4];
+  const int group = 1 << a.log2_group;
+  const int warps = group >> 5;
+  const int groups = kStreamThreads >> a.log2_group;
+  const int g = static_cast<int>(threadIdx.x) >> a.log2_group;
+  const int t = static_cast<int>(threadIdx.x) & (group - 1);
+  const int first = (t >> 5) * 32 * kUnits + (t & 31);        // this lane's first vector; the others follow in strides of 32
+  const int vectors = a.hidden / kVec;
+  const long long step = static_cast<long long>(gridDim.x) * groups * kRows;
+  const bool rounded = !kCentered && a.round_xhat != 0;
+
+  uint4 raw_w[kUnits * kWVecs], raw_b[kCentered ? kUnits * kWVecs : 1];
+  stream_load_parameter<W, kUnits, kWVecs>(a.w, first, vectors, raw_w);
+  if constexpr (kCentered) stream_load_parameter<W, kUnits, kWVecs>(a.b, first, vectors, raw_b);
+  const F2 offset = both(a.w != nullptr ? a.offset : 1.f);     // without a weight the gain is one
+
+  auto cell = [&](int slot, int r, int u) -> uint4& { return stream_ring[((slot * kRows + r) * kUnits + u) * kStreamThreads + threadIdx.x]; };
+  // rows behind the last one come in as zeros and are not stored
+  auto fetch = [&](long long base, int slot) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const bool live = base + r < a.n_rows;
+      const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (live ? base + r : 0) * a.ld_x) + first;
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) async_copy16(&cell(slot, r, u), x + u * 32, live && first + u * 32 < vectors);
+    }
+    async_commit();
+  };
+  long long row = (static_cast<long long>(blockIdx.x) * groups + g) * kRows;
+#pragma unroll
+  for (int s = 0; s < kSlots - 1; ++s) fetch(row + s * step, s);
+  int slot = 0, phase = 0;
+  const float inv = 1.f / static_cast<float>(a.hidden);
+  for (; row < a.n_rows; row += step) {
+    // into the slot of the round before this one, which this thread, its only reader, has read for the last time
+    fetch(row + (kSlots - 1) * step, slot == 0 ? kSlots - 1 : slot - 1);
+    async_wait<kSlots - 1>();
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    F2 minus_mean[kRows];
+    float mean = 0.f;                       // of row lane >> 3
+    if constexpr (kCentered) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        F2 acc = both(0.f);
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+          const uint4 raw = cell(slot, r, u);
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) acc = add2(acc, Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw) + i * Pairs<T>::kWords));
+        }
+        v[r] = f2_lo(acc) + f2_hi(acc);
+      }
+      mean = stream_four_sums(v, warps, g, scratch, phase) * inv;
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      minus_mean[r] = both(kCentered ? -__shfl_sync(0xffffffffu, mean, r * 8) : 0.f);
+      F2 acc = both(0.f);
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const uint4 raw = cell(slot, r, u);
+        if (!kCentered || first + u * 32 < vectors) {
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) {
+            F2 e = Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw) + i * Pairs<T>::kWords);
+            if (kCentered) e = add2(e, minus_mean[r]);
+            acc = fma2(e, e, acc);
+          }
+        }
+      }
+      v[r] = f2_lo(acc) + f2_hi(acc);
+    }
+    const float rstd = 1.f / sqrtf(fmaf(stream_four_sums(v, warps, g, scratch, phase), inv, a.eps));
+    {
+      const int r = static_cast<int>(threadIdx.x & 31) >> 3;
+      if ((t & ~24) == 0 && r < kRows && row + r < a.n_rows) {      // lanes 0, 8, 16, 24 of the group's first warp
+        if (kCentered && a.mean != nullptr) a.mean[row + r] = mean;
+        if (a.rstd != nullptr) a.rstd[row + r] = rstd;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const F2 scale = both(__shfl_sync(0xffffffffu, rstd, r * 8));
+      if (row + r >= a.n_rows) continue;
+      uint4* y = reinterpret_cast<uint4*>(static_cast<T*>(a.y) + (row + r) * a.hidden) + first;
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        if (first + u * 32 >= vectors) continue;
+        const uint4 raw = cell(slot, r, u);
+        uint4 out;
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          F2 e = Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw) + i * Pairs<T>::kWords);
+          if (kCentered) e = add2(e, minus_mean[r]);
+          e = mul2(e, scale);
+          if (rounded) e = f2(norm_round<T>(f2_lo(e)), norm_round<T>(f2_hi(e)));
+          const F2 gain = add2(offset, Pairs<W>::get(reinterpret_cast<const uint32_t*>(&raw_w[u * kWVecs]) + i * Pairs<W>::kWords));
+          if constexpr (kCentered)
+            e = fma2(e, gain, Pairs<W>::get(reinterpret_cast<const uint32_t*>(&raw_b[u * kWVecs]) + i * Pairs<W>::kWords));
+          else
+            e = mul2(e, gain);
+          Pairs<T>::set(reinterpret_cast<uint32_t*>(&out) + i * Pairs<T>::kWords, e);
+        }
+        y[u * 32] = out;
+      }
+    }
+    slot = slot + 1 == kSlots ? 0 : slot + 1;
+  }
+  async_wait<0>();
+}
+
+// dx, and this block's share of the parameters' gradients.  Each thread of a group owns kUnits vectors of columns; a round
+// takes kRows rows per group, their sums meet in one reduction (and one barrier, if the group is wider than a warp).
+template <typename T, typename W, bool kCentered, int kUnits>
+__global__ void __launch_bounds__(kStreamThreads, (Stream<kUnits, true>::kBlocksPerSm))
+norm_backward_stream_kernel(NormBackwardArgs a) {
+  constexpr int kRows = Stream<kUnits, true>::kRows, kSlots = Stream<kUnits, true>::kSlots;
+  constexpr int kVec = CeElem<T>::kVec;
+  constexpr int kPairs = kVec / 2;
+  constexpr int kWVecs = kVec * static_cast<int>(sizeof(W)) / 16;
+  FLCE_DYNAMIC_SHARED(uint4, stream_ring);                // [slot][row][x, dy][unit][thread]; at the end: the blocks' folds
+  __shared__ float scratch[2][kNormMaxWarps * 4];
+  const int group = 1 << a.log2_group;
+  const int warps = group >> 5;
+  const int groups = kStreamThreads >> a.log2_group;
+  const int g = static_cast<int>(threadIdx.x) >> a.log2_group;
+  const int t = static_cast<int>(threadIdx.x) & (group - 1);
+  const int first = (t >> 5) * 32 * kUnits + (t & 31);
+  const int vectors = a.hidden / kVec;
+  const long long step = static_cast<long long>(gridDim.x) * groups * kRows;
+  const bool rounded = !kCentered && a.round_xhat != 0;
+
+  uint4 raw_w[kUnits * kWVecs];
+  stream_load_parameter<W, kUnits, kWVecs>(a.w, first, vectors, raw_w);
+  // without a weight the gain is one: zeros plus an offset of one
+  const F2 offset = both(a.w != nullptr ? a.offset : 1.f);
+  auto gain = [&](int u, int i) {
+    return add2(offset, Pairs<W>::get(reinterpret_cast<const uint32_t*>(&raw_w[u * kWVecs]) + i * Pairs<W>::kWords));
+  };
+
+  F2 dw[kUnits * kPairs], db[kCentered ? kUnits * kPairs : 1];
+#pragma unroll
+  for (int i = 0; i < kUnits * kPairs; ++i) {
+    dw[i] = both(0.f);
+    if (kCentered) db[i] = both(0.f);
+  }
+
+  // rows of this group in a round: consecutive ones.  A row behind the last one comes in as zeros and is not stored.
+  auto cell = [&](int slot, int r, int which, int u) -> uint4& {
+    return stream_ring[(((slot * kRows + r) * 2 + which) * kUnits + u) * kStreamThreads + threadIdx.x];
+  };
+  auto fetch = [&](long long base, int slot) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const long long row = base + r;
+      const bool live = row < a.n_rows;
+      const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (live ? row : 0) * a.ld_x) + first;
+      const uint4* dy = reinterpret_cast<const uint4*>(static_cast<const T*>(a.dy) + (live ? row : 0) * a.ld_dy) + first;
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        async_copy16(&cell(slot, r, 0, u), x + u * 32, live && first + u * 32 < vectors);
+        async_copy16(&cell(slot, r, 1, u), dy + u * 32, live && first + u * 32 < vectors);
+      }
+    }
+    async_commit();
+  };
+  float next_mean[kRows], next_rstd[kRows];
+  auto fetch_statistics = [&](long long base) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const bool live = base + r < a.n_rows;
+      next_mean[r] = kCentered && live ? __ldg(a.mean + base + r) : 0.f;
+      next_rstd[r] = live ? __ldg(a.rstd + base + r) : 0.f;
+    }
+  };
+
+  long long round = static_cast<long long>(blockIdx.x) * groups * kRows;     // the block's first row: the same in every thread
+  const int mine = g * kRows;
+#pragma unroll
+  for (int s = 0; s < kSlots - 1; ++s) fetch(round + s * step + mine, s);
+  fetch_statistics(round + mine);
+  int slot = 0, phase = 0;
+  for (; round < a.n_rows; round += step) {
+    // the slot of the round before this one: its second reading is done, in this thread, which is the only one to read it
+    fetch(round + (kSlots - 1) * step + mine, slot == 0 ? kSlots - 1 : slot - 1);
+    async_wait<kSlots - 1>();
+    float rstd[kRows];
+    F2 minus_mean[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      minus_mean[r] = both(-next_mean[r]);
+      rstd[r] = next_rstd[r];
+    }
+    fetch_statistics(round + step + mine);
+    float v[4] = {0.f, 0.f, 0.f, 0.f};        // (sum m xhat, sum m) of each row
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      F2 s_mx = both(0.f), s_m = both(0.f);
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const uint4 raw_x = cell(slot, r, 0, u), raw_dy = cell(slot, r, 1, u);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          // behind the row's end dy is zero, which keeps xhat out of every sum
+          F2 xhat = Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw_x) + i * Pairs<T>::kWords);
+          if (kCentered) xhat = add2(xhat, minus_mean[r]);
+          xhat = mul2(xhat, both(rstd[r]));
+          const F2 d = Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw_dy) + i * Pairs<T>::kWords);
+          F2 xw = xhat;
+          if (rounded) xw = f2(norm_round<T>(f2_lo(xhat)), norm_round<T>(f2_hi(xhat)));
+          dw[u * kPairs + i] = fma2(d, xw, dw[u * kPairs + i]);
+          if (kCentered) db[u * kPairs + i] = add2(db[u * kPairs + i], d);
+          const F2 m = mul2(d, gain(u, i));
+          s_mx = fma2(m, xhat, s_mx);
+          if (kCentered) s_m = add2(s_m, m);
+        }
+      }
+      v[2 * r] = f2_lo(s_mx) + f2_hi(s_mx);
+      if (kCentered) v[2 * r + 1] = f2_lo(s_m) + f2_hi(s_m);
+    }
+    const float sum = stream_four_sums(v, warps, g, scratch, phase);
+    const float inv = 1.f / static_cast<float>(a.hidden);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const float c = __shfl_sync(0xffffffffu, sum, r * 16) * inv;
+      const float m_mean = kCentered ? __shfl_sync(0xffffffffu, sum, r * 16 + 8) * inv : 0.f;
+      const long long row = round + mine + r;
+      if (row >= a.n_rows) continue;
+      uint4* dx = reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + row * a.hidden) + first;
+      // rstd (m - mean(m) - xhat c), xhat = (x - mean) rstd
+      const F2 minus_c = both(-c), minus_m = both(-m_mean);
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        if (first + u * 32 >= vectors) continue;
+        const uint4 raw_x = cell(slot, r, 0, u), raw_dy = cell(slot, r, 1, u);
+        uint4 out;
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          F2 xhat = Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw_x) + i * Pairs<T>::kWords);
+          if (kCentered) xhat = add2(xhat, minus_mean[r]);
+          xhat = mul2(xhat, both(rstd[r]));
+          F2 m = mul2(Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw_dy) + i * Pairs<T>::kWords), gain(u, i));
+          if (kCentered) m = add2(m, minus_m);
+          Pairs<T>::set(reinterpret_cast<uint32_t*>(&out) + i * Pairs<T>::kWords, mul2(fma2(xhat, minus_c, m), both(rstd[r])));
+        }
+        dx[u * 32] = out;
+      }
+    }
+    slot = slot + 1 == kSlots ? 0 : slot + 1;
+  }
+  // the groups of the block, folded in halves in a fixed order; the ring is free once all copies (of zeros, behind the last
+  // row) have landed
+  async_wait<0>();
+  float* fold = reinterpret_cast<float*>(stream_ring);
+  auto leave = [&](F2* acc, float* partial) {
+    for (int half = groups >> 1; half > 0; half >>= 1) {
+      __syncthreads();
+      if (g >= half && g < 2 * half) {
+#pragma unroll
+        for (int i = 0; i < kUnits * kPairs; ++i) {
+          fold[((g - half) * 2 * kUnits * kPairs + 2 * i) * group + t] = f2_lo(acc[i]);
+          fold[((g - half) * 2 * kUnits * kPairs + 2 * i + 1) * group + t] = f2_hi(acc[i]);
+        }
+      }
+      __syncthreads();
+      if (g < half) {
+#pragma unroll
+        for (int i = 0; i < kUnits * kPairs; ++i)
+          acc[i] = add2(acc[i], f2(fold[(g * 2 * kUnits * kPairs + 2 * i) * group + t], fold[(g * 2 * kUnits * kPairs + 2 * i + 1) * group + t]));
+      }
+    }
+    if (g == 0) {
+      float* out = partial + static_cast<size_t>(blockIdx.x) * a.hidden;
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        if (first + u * 32 >= vectors) continue;
+        float e[kVec];
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          e[2 * i] = f2_lo(acc[u * kPairs + i]);
+          e[2 * i + 1] = f2_hi(acc[u * kPairs + i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kVec; i += 4) *reinterpret_cast<float4*>(out + (first + u * 32) * kVec + i) = make_float4(e[i], e[i + 1], e[i + 2], e[i + 3]);
+      }
+    }
+  };
+  if (a.dw_partial != nullptr) leave(dw, a.dw_partial);
+  if constexpr (kCentered) {
+    if (a.db_partial != nullptr) leave(db, a.db_partial);
+  }
+}
+
+// ---- rows of at most 32 aligned 16-byte vectors: one vector per lane, several rows to a warp, kRows of them per thread at a
+// time, so that the loads and the shuffles of one row hide those of another
+
+constexpr int kNarrowThreads = 256;
+
+template <typename T, typename W, bool kCentered, int kRows>
+__global__ void __launch_bounds__(kNarrowThreads)
+norm_forward_narrow_kernel(NormForwardArgs a) {
+  constexpr int kVec = CeElem<T>::kVec;
+  constexpr int kPairs = kVec / 2;
+  constexpr int kWVecs = kVec * static_cast<int>(sizeof(W)) / 16;
+  const int group = 1 << a.log2_group;
+  const int groups = kNarrowThreads >> a.log2_group;
+  const int t = static_cast<int>(threadIdx.x) & (group - 1);
+  const bool column = t * kVec < a.hidden;
+  const bool rounded = !kCentered && a.round_xhat != 0;
+  const long long base = static_cast<long long>(blockIdx.x) * groups * kRows + (threadIdx.x >> a.log2_group);
+  uint4 raw[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const long long row = base + r * groups;
+    raw[r] = make_uint4(0u, 0u, 0u, 0u);
+    if (column && row < a.n_rows) raw[r] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.ld_x) + t);
+  }
+  F2 gain[kPairs], bias[kPairs];
+  {
+    uint4 w[kWVecs], b[kWVecs];
+#pragma unroll
+    for (int i = 0; i < kWVecs; ++i) {
+      w[i] = b[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (column && a.w != nullptr) w[i] = __ldg(reinterpret_cast<const uint4*>(a.w) + t * kWVecs + i);
+      if (column && a.b != nullptr) b[i] = __ldg(reinterpret_cast<const uint4*>(a.b) + t * kWVecs + i);
+    }
+    const F2 offset = both(a.w != nullptr ? a.offset : 1.f);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      gain[i] = add2(offset, Pairs<W>::get(reinterpret_cast<const uint32_t*>(w) + i * Pairs<W>::kWords));
+      bias[i] = Pairs<W>::get(reinterpret_cast<const uint32_t*>(b) + i * Pairs<W>::kWords);
+    }
+  }
+  float mean[kRows], square[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    mean[r] = 0.f;
+    if (kCentered) {
+      F2 acc = both(0.f);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) acc = add2(acc, Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw[r]) + i * Pairs<T>::kWords));
+      mean[r] = f2_lo(acc) + f2_hi(acc);
+    }
+  }
+  if (kCentered) {
+    for (int o = group >> 1; o > 0; o >>= 1) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) mean[r] += __shfl_xor_sync(0xffffffffu, mean[r], o);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    mean[r] /= static_cast<float>(a.hidden);
+    F2 acc = both(0.f);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const F2 v = add2(Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw[r]) + i * Pairs<T>::kWords), both(-mean[r]));
+      acc = fma2(v, v, acc);
+    }
+    square[r] = column ? f2_lo(acc) + f2_hi(acc) : 0.f;
+  }
+  for (int o = group >> 1; o > 0; o >>= 1) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) square[r] += __shfl_xor_sync(0xffffffffu, square[r], o);
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const long long row = base + r * groups;
+    if (row >= a.n_rows) continue;
+    const float rstd = 1.f / sqrtf(square[r] / static_cast<float>(a.hidden) + a.eps);
+    if (t == 0) {
+      if (kCentered && a.mean != nullptr) a.mean[row] = mean[r];
+      if (a.rstd != nullptr) a.rstd[row] = rstd;
+    }
+    uint4 out;
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      F2 v = Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw[r]) + i * Pairs<T>::kWords);
+      if (kCentered) v = add2(v, both(-mean[r]));
+      v = mul2(v, both(rstd));
+      if (rounded) v = f2(norm_round<T>(f2_lo(v)), norm_round<T>(f2_hi(v)));
+      Pairs<T>::set(reinterpret_cast<uint32_t*>(&out) + i * Pairs<T>::kWords, kCentered ? fma2(v, gain[i], bias[i]) : mul2(v, gain[i]));
+    }
+    if (column) reinterpret_cast<uint4*>(static_cast<T*>(a.y) + row * a.hidden)[t] = out;
+  }
+}
+
+template <typename T, typename W, bool kCentered, int kRows>
+__global__ void __launch_bounds__(kNarrowThreads)
+norm_backward_narrow_kernel(NormBackwardArgs a) {
+  constexpr int kVec = CeElem<T>::kVec;
+  constexpr int kPairs = kVec / 2;
+  constexpr int kWVecs = kVec * static_cast<int>(sizeof(W)) / 16;
+  __shared__ float fold[kNarrowThreads / 2 * kVec];
+  const int group = 1 << a.log2_group;
+  const int groups = kNarrowThreads >> a.log2_group;
+  const int t = static_cast<int>(threadIdx.x) & (group - 1);
+  const int g = static_cast<int>(threadIdx.x) >> a.log2_group;
+  const bool column = t * kVec < a.hidden;
+  const bool rounded = !kCentered && a.round_xhat != 0;
+  const long long step = static_cast<long long>(gridDim.x) * groups * kRows;
+  F2 gain[kPairs], dw[kPairs], db[kPairs];
+  {
+    uint4 w[kWVecs];
+#pragma unroll
+    for (int i = 0; i < kWVecs; ++i) {
+      w[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (column && a.w != nullptr) w[i] = __ldg(reinterpret_cast<const uint4*>(a.w) + t * kWVecs + i);
+    }
+    const F2 offset = both(a.w != nullptr ? a.offset : 1.f);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      gain[i] = add2(offset, Pairs<W>::get(reinterpret_cast<const uint32_t*>(w) + i * Pairs<W>::kWords));
+      dw[i] = db[i] = both(0.f);
+    }
+  }
+  const float inv = 1.f / static_cast<float>(a.hidden);
+  for (long long base = static_cast<long long>(blockIdx.x) * groups * kRows; base < a.n_rows; base += step) {
+    uint4 raw_x[kRows], raw_dy[kRows];
+    float mean[kRows], rstd[kRows], s_mx[kRows], s_m[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {       // rows behind the last one come in as zeros
+      const long long row = base + g + r * groups;
+      const bool live = row < a.n_rows;
+      raw_x[r] = raw_dy[r] = make_uint4(0u, 0u, 0u, 0u);
+      if (column && live) {
+        raw_x[r] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.ld_x) + t);
+        raw_dy[r] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.dy) + row * a.ld_dy) + t);
+      }
+      mean[r] = kCentered && live ? __ldg(a.mean + row) : 0.f;
+      rstd[r] = live ? __ldg(a.rstd + row) : 0.f;
+    }
+    auto xhat_of = [&](int r, int i) {
+      F2 v = Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw_x[r]) + i * Pairs<T>::kWords);
+      if (kCentered) v = add2(v, both(-mean[r]));
+      return mul2(v, both(rstd[r]));
+    };
+    auto dy_of = [&](int r, int i) { return Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw_dy[r]) + i * Pairs<T>::kWords); };
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      F2 mx = both(0.f), m = both(0.f);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        const F2 xhat = xhat_of(r, i), d = dy_of(r, i), md = mul2(d, gain[i]);
+        dw[i] = fma2(d, rounded ? f2(norm_round<T>(f2_lo(xhat)), norm_round<T>(f2_hi(xhat))) : xhat, dw[i]);
+        if (kCentered) db[i] = add2(db[i], d);
+        mx = fma2(md, xhat, mx);
+        if (kCentered) m = add2(m, md);
+      }
+      s_mx[r] = f2_lo(mx) + f2_hi(mx);
+      s_m[r] = f2_lo(m) + f2_hi(m);
+    }
+    for (int o = group >> 1; o > 0; o >>= 1) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        s_mx[r] += __shfl_xor_sync(0xffffffffu, s_mx[r], o);
+        if (kCentered) s_m[r] += __shfl_xor_sync(0xffffffffu, s_m[r], o);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const long long row = base + g + r * groups;
+      uint4 out;
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        F2 m = mul2(dy_of(r, i), gain[i]);
+        if (kCentered) m = add2(m, both(-s_m[r] * inv));
+        Pairs<T>::set(reinterpret_cast<uint32_t*>(&out) + i * Pairs<T>::kWords,
+                      mul2(fma2(xhat_of(r, i), both(-s_mx[r] * inv), m), both(rstd[r])));
+      }
+      if (column && row < a.n_rows) reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + row * a.hidden)[t] = out;
+    }
+  }
+  // the groups of the block, folded in halves in a fixed order
+  auto leave = [&](F2 (&acc)[kPairs], float* partial) {
+    for (int half = groups >> 1; half > 0; half >>= 1) {
+      __syncthreads();
+      if (g >= half && g < 2 * half) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          fold[((g - half) * kVec + 2 * i) * group + t] = f2_lo(acc[i]);
+          fold[((g - half) * kVec + 2 * i + 1) * group + t] = f2_hi(acc[i]);
+        }
+      }
+      __syncthreads();
+      if (g < half) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) acc[i] = add2(acc[i], f2(fold[(g * kVec + 2 * i) * group + t], fold[(g * kVec + 2 * i + 1) * group + t]));
+      }
+    }
+    if (g == 0 && column) {
+      float* out = partial + static_cast<size_t>(blockIdx.x) * a.hidden + t * kVec;
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        out[2 * i] = f2_lo(acc[i]);
+        out[2 * i + 1] = f2_hi(acc[i]);
       }
     }
   };

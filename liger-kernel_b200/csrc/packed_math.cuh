@@ -1,0 +1,129 @@
+// Arithmetic on pairs of floats in one 64-bit register (add / mul / fma .f32x2: one instruction for two elements on sm_100) and
+// asynchronous 16-byte copies into shared memory, for kernels that are short of issue slots rather than of bandwidth.
+//
+// With FLCE_HOST_EMULATION the pairs are two floats and a copy is done when it is issued.
+#pragma once
+
+#include <cstdint>
+#include <cstring>
+
+#include "ce_kernels.cuh"
+#include "simt_common.cuh"
+
+namespace flce {
+
+#ifdef FLCE_HOST_EMULATION
+struct F2 {
+  float lo, hi;
+};
+inline F2 f2(float lo, float hi) { return {lo, hi}; }
+inline float f2_lo(F2 a) { return a.lo; }
+inline float f2_hi(F2 a) { return a.hi; }
+inline F2 add2(F2 a, F2 b) { return {a.lo + b.lo, a.hi + b.hi}; }
+inline F2 mul2(F2 a, F2 b) { return {a.lo * b.lo, a.hi * b.hi}; }
+inline F2 fma2(F2 a, F2 b, F2 c) { return {std::fma(a.lo, b.lo, c.lo), std::fma(a.hi, b.hi, c.hi)}; }
+#else
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float f2_lo(F2 a) {
+  float lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a));
+  return lo;
+}
+__device__ __forceinline__ float f2_hi(F2 a) {
+  float lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a));
+  return hi;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+#endif
+__device__ __forceinline__ F2 both(float v) { return f2(v, v); }
+
+// Elements 2 i and 2 i + 1 of a run of elements held in 32-bit words (two 16-bit elements or one fp32 element per word).
+template <typename T>
+struct Pairs;
+template <>
+struct Pairs<float> {
+  static constexpr int kWords = 2;             // words per pair
+  __device__ static F2 get(const uint32_t* w) { return f2(__uint_as_float(w[0]), __uint_as_float(w[1])); }
+  __device__ static void set(uint32_t* w, F2 v) {
+    w[0] = __float_as_uint(f2_lo(v));
+    w[1] = __float_as_uint(f2_hi(v));
+  }
+};
+template <>
+struct Pairs<__nv_bfloat16> {
+  static constexpr int kWords = 1;
+  __device__ static F2 get(const uint32_t* w) { return f2(__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u)); }
+  __device__ static void set(uint32_t* w, F2 v) { w[0] = pack2(f2_lo(v), f2_hi(v), kOutBf16); }
+};
+template <>
+struct Pairs<__half> {
+  static constexpr int kWords = 1;
+  __device__ static F2 get(const uint32_t* w) {
+    __half h[2];
+    memcpy(h, w, 4);
+    return f2(__half2float(h[0]), __half2float(h[1]));
+  }
+  __device__ static void set(uint32_t* w, F2 v) { w[0] = pack2(f2_lo(v), f2_hi(v), kOutFp16); }
+};
+
+// the block's dynamic shared memory
+#ifdef FLCE_HOST_EMULATION
+#define FLCE_DYNAMIC_SHARED(type, name) type* name = static_cast<type*>(emu_dynamic_shared())
+#else
+#define FLCE_DYNAMIC_SHARED(type, name) extern __shared__ type name[]
+#endif
+
+// 16 bytes from global to this CTA's shared memory (past L1), or 16 zero bytes if !read; both addresses 16-byte aligned.  A
+// thread sees its own copies after async_wait; groups are waited for in the order they were committed.
+__device__ __forceinline__ void async_copy16(void* dst, const void* src, bool read) {
+#ifdef FLCE_HOST_EMULATION
+  if (read) std::memcpy(dst, src, 16);
+  else std::memset(dst, 0, 16);
+#else
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src),
+               "r"(read ? 16 : 0)
+               : "memory");
+#endif
+}
+__device__ __forceinline__ void async_commit() {
+#ifndef FLCE_HOST_EMULATION
+  asm volatile("cp.async.commit_group;" ::: "memory");
+#endif
+}
+template <int kPending>
+__device__ __forceinline__ void async_wait() {
+#ifndef FLCE_HOST_EMULATION
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+#endif
+}
+
+// Barrier of the `threads` threads (whole warps) that name it; ids 1..15, 0 is __syncthreads.
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+#ifdef FLCE_HOST_EMULATION
+  emu_named_barrier(id, threads);
+#else
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+#endif
+}
+
+}  // namespace flce

@@ -24,6 +24,21 @@ inline bool __any_sync(unsigned m, bool v) { return __ballot_sync(m, v) != 0; }
 inline int __popc(unsigned v) { return __builtin_popcount(v); }
 inline int __clz(unsigned v) { return v ? __builtin_clz(v) : 32; }
 
+template <typename T>
+T __shfl_sync(unsigned, T v, int src_lane) {
+  return emu::shuffle_from(v, static_cast<unsigned>(src_lane));
+}
+// bar.sync id, n: its own barrier per id; every id is left empty by the kernels that use it
+inline void emu_named_barrier(int id, int threads) {
+  static emu::Barrier named[16];
+  named[id].expected = static_cast<unsigned>(threads);
+  emu::barrier_wait(named[id]);
+}
+inline void* emu_dynamic_shared() {
+  alignas(128) static char bytes[227 * 1024];
+  return bytes;
+}
+
 inline emu::Dim3 emu_dim3(dim3 d) { return emu::Dim3(d.x, d.y, d.z); }
 
 #include "host_internal.hpp"
