@@ -27,67 +27,63 @@ int check_norm(const flce_norm_t* p) {
   return FLCE_OK;
 }
 
-// How a row is spread: `unit` consecutive elements per access, `ept` elements per thread, 1 << log2_group threads.
-struct NormShape {
-  int unit, ept, log2_group;
-  bool fits;
-};
-
-NormShape norm_shape(const flce_norm_t* p, bool whole_vectors, int preferred_threads) {
-  NormShape s;
-  s.unit = whole_vectors ? 16 / element_size(p->dtype) : 1;
-  const long long units = ceil_div(p->hidden, s.unit);
-  if (units <= 32) {        // one unit per thread, several rows to a warp
-    s.ept = s.unit;
-    for (s.log2_group = 0; (1ll << s.log2_group) < units;) ++s.log2_group;
-    s.fits = true;
-    return s;
-  }
-  for (s.ept = 8;; s.ept *= 2) {
-    for (s.log2_group = 5; (1ll << s.log2_group) * s.ept < units * s.unit;) ++s.log2_group;
-    s.fits = (1ll << s.log2_group) <= kNormMaxThreads;
-    if ((1ll << s.log2_group) <= preferred_threads || s.ept == kNormMaxEpt) return s;
-  }
-}
-
-// Rows of whole vectors go to the streaming kernels, or to the narrow ones if a warp's lanes hold one with a vector each.
-enum NormPath { kNormGeneric, kNormStream, kNormNarrow };
-constexpr int kNarrowForwardRows = 4, kNarrowBackwardRows = 2;
-
+// How the rows are spread over threads: `share` elements (scalar) or 16-byte vectors (otherwise) per thread, 1 << log2_group
+// threads to a row.
+enum NormPath { kNormStream, kNormNarrow, kNormScalar, kNormLong };
 struct NormPlan {
   NormPath path;
-  NormShape shape;      // ept holds the vectors per lane, except on the generic path
+  int share, log2_group;
 };
 
-int log2_ceil(long long v) {
-  int l = 0;
-  while ((1ll << l) < v) ++l;
+int log2_group_for(long long pieces, int smallest) {
+  int l = smallest;
+  while ((1ll << l) < pieces) ++l;
   return l;
 }
 
-// The streaming kernels give every thread of a 512-thread block its columns: one vector if that reaches, up to four.
-NormPlan norm_plan(const flce_norm_t* p, bool vectors, int preferred_threads) {
-  NormPlan plan{kNormGeneric, {}};
+// Narrow: a lane per vector, rows of up to 32 of them.  Stream: two vectors per thread if a block's 512 threads reach so, else four.
+// Scalar: one element per thread up to 32, then 4 or 16 strides of a warp.  Long: what is left, above 8192 elements.
+NormPlan norm_plan(const flce_norm_t* p, bool vectors) {
   const long long n = p->hidden * element_size(p->dtype) / 16;
-  if (vectors && n <= 32) {
-    plan.path = kNormNarrow;
-    plan.shape = {1, 1, log2_ceil(n), true};
-  } else if (vectors && n <= 4 * kStreamThreads) {
-    int units = 1;
-    while (units * kStreamThreads < n) units *= 2;
-    int log2_group = 5;
-    while ((units << log2_group) < n) ++log2_group;
-    plan.path = kNormStream;
-    plan.shape = {1, units, log2_group, true};
-  } else {
-    plan.shape = norm_shape(p, vectors, preferred_threads);
+  if (vectors && n <= 32) return {kNormNarrow, 1, log2_group_for(n, 2)};
+  if (vectors && n <= 4 * kStreamThreads) {
+    const int share = n <= 2 * kStreamThreads ? 2 : 4;
+    return {kNormStream, share, log2_group_for(ceil_div(n, share), 5)};
   }
-  return plan;
+  if (p->hidden <= 32) return {kNormScalar, 1, log2_group_for(p->hidden, 2)};
+  if (p->hidden <= 16 * kScalarThreads) {
+    const int share = p->hidden <= 4 * kScalarThreads ? 4 : 16;
+    return {kNormScalar, share, log2_group_for(ceil_div(p->hidden, share), 5)};
+  }
+  return {kNormLong, 0, 9};
 }
 
+// rows that a block takes per round, and blocks that are resident on an SM
 template <bool kGrad>
-int stream_rows(int units) {
-  return units == 1 ? Stream<1, kGrad>::kRows : (units == 2 ? Stream<2, kGrad>::kRows : Stream<4, kGrad>::kRows);
+int rows_per_round(const NormPlan& plan) {
+  switch (plan.path) {
+    case kNormNarrow: return (kNarrowThreads >> plan.log2_group) * (kGrad ? kNarrowBackwardRows : kNarrowForwardRows);
+    case kNormStream: return (kStreamThreads >> plan.log2_group) * (plan.share == 2 ? Stream<2, kGrad>::kRows : Stream<4, kGrad>::kRows);
+    case kNormScalar: return (kScalarThreads >> plan.log2_group) * (plan.share < 16 ? Scalar<4, kGrad>::kRows : Scalar<16, kGrad>::kRows);
+    default: return 1;
+  }
+}
+int blocks_per_sm(const NormPlan& plan) {
+  switch (plan.path) {
+    case kNormNarrow: return 4;
+    case kNormStream: return 1;
+    case kNormScalar: return plan.share < 16 ? Scalar<4, true>::kBlocksPerSm : Scalar<16, true>::kBlocksPerSm;
+    default: return 2;
+  }
+}
+
+// Blocks that walk over the rows: as many as are resident together.  Those of the backward kernel leave `hidden` partial sums
+// per parameter each.
+template <bool kGrad>
+long long walking_blocks(const flce_norm_t* p, const NormPlan& plan, int sm_count) {
+  const long long most = ceil_div(p->n_rows, rows_per_round<kGrad>(plan));
+  const long long resident = static_cast<long long>(blocks_per_sm(plan)) * sm_count;
+  return most < resident ? most : resident;
 }
 
 bool whole_vectors(const flce_norm_t* p, const void* other, long long ld_other) {
@@ -95,26 +91,6 @@ bool whole_vectors(const flce_norm_t* p, const void* other, long long ld_other) 
   const bool pitches = p->n_rows <= 1 || (p->ld_x % vec == 0 && ld_other % vec == 0);     // one row has no pitch
   return p->hidden % vec == 0 && pitches && aligned16(p->x) && aligned16(other) &&
          aligned16(p->weight) && aligned16(p->bias);
-}
-
-template <typename T, typename W, bool kCentered, int kUnit>
-void run_forward(const NormForwardArgs& a, const NormShape& s, unsigned grid, int threads, cudaStream_t stream) {
-  switch (s.ept) {
-    case kUnit < 8 ? kUnit : -1: FLCE_LAUNCH((norm_forward_kernel<T, W, kCentered, kUnit, kUnit>), grid, threads, stream, a); break;
-    case 8: FLCE_LAUNCH((norm_forward_kernel<T, W, kCentered, kUnit, 8>), grid, threads, stream, a); break;
-    case 16: FLCE_LAUNCH((norm_forward_kernel<T, W, kCentered, kUnit, 16>), grid, threads, stream, a); break;
-    default: FLCE_LAUNCH((norm_forward_kernel<T, W, kCentered, kUnit, 32>), grid, threads, stream, a); break;
-  }
-}
-
-template <typename T, typename W, bool kCentered, int kUnit>
-void run_backward(const NormBackwardArgs& a, const NormShape& s, unsigned grid, cudaStream_t stream) {
-  switch (s.ept) {
-    case kUnit < 8 ? kUnit : -1: FLCE_LAUNCH((norm_backward_kernel<T, W, kCentered, kUnit, kUnit>), grid, kNormMaxThreads, stream, a); break;
-    case 8: FLCE_LAUNCH((norm_backward_kernel<T, W, kCentered, kUnit, 8>), grid, kNormMaxThreads, stream, a); break;
-    case 16: FLCE_LAUNCH((norm_backward_kernel<T, W, kCentered, kUnit, 16>), grid, kNormMaxThreads, stream, a); break;
-    default: FLCE_LAUNCH((norm_backward_kernel<T, W, kCentered, kUnit, 32>), grid, kNormMaxThreads, stream, a); break;
-  }
 }
 
 // fn(T{}, W{}) for the problem's types
@@ -127,43 +103,53 @@ void with_types(const flce_norm_t* p, Fn fn) {
   else fn(__half(), float());
 }
 
-// Blocks of the backward kernel: they are resident together and walk over the rows.  Each leaves hidden partial sums per
-// parameter, so no more of them than it takes to fill the device.
-long long backward_blocks(const flce_norm_t* p, const NormPlan& plan, int sm_count) {
-  long long rows = 1, per_sm = 2;
-  if (plan.path == kNormNarrow) {
-    rows = (kNarrowThreads >> plan.shape.log2_group) * kNarrowBackwardRows;
-    per_sm = 4;
-  } else if (plan.path == kNormStream) {
-    rows = (kStreamThreads >> plan.shape.log2_group) * stream_rows<true>(plan.shape.ept);
-    per_sm = plan.shape.ept == 1 ? 2 : 1;
-  } else if (plan.shape.fits) {
-    rows = kNormMaxThreads >> plan.shape.log2_group;
-  }
-  const long long most = ceil_div(p->n_rows, rows);
-  const long long resident = per_sm * sm_count;
-  return most < resident ? most : resident;
-}
-
 template <typename T, typename W, bool kCentered>
-int run_forward_stream(const NormForwardArgs& a, const NormShape& s, int sm_count, cudaStream_t stream) {
-  const long long most = ceil_div(a.n_rows, (kStreamThreads >> s.log2_group) * stream_rows<false>(s.ept));
-  const long long resident = (s.ept == 1 ? 2ll : 1ll) * sm_count;
-  const dim3 grid(static_cast<unsigned>(most < resident ? most : resident));
-  switch (s.ept) {
-    case 1: return launch_with_shared<norm_forward_stream_kernel<T, W, kCentered, 1>>(grid, kStreamThreads, Stream<1, false>::kRingBytes, stream, a);
-    case 2: return launch_with_shared<norm_forward_stream_kernel<T, W, kCentered, 2>>(grid, kStreamThreads, Stream<2, false>::kRingBytes, stream, a);
-    default: return launch_with_shared<norm_forward_stream_kernel<T, W, kCentered, 4>>(grid, kStreamThreads, Stream<4, false>::kRingBytes, stream, a);
+int run_forward(const NormForwardArgs& a, const NormPlan& plan, unsigned walking, cudaStream_t stream) {
+  const dim3 grid(walking);
+  switch (plan.path) {
+    case kNormStream:
+      if (plan.share == 2)
+        return launch_with_shared<norm_forward_stream_kernel<T, W, kCentered, 2>>(grid, kStreamThreads, Stream<2, false>::kRingBytes, stream, a);
+      return launch_with_shared<norm_forward_stream_kernel<T, W, kCentered, 4>>(grid, kStreamThreads, Stream<4, false>::kRingBytes, stream, a);
+    case kNormNarrow: {
+      const unsigned all = static_cast<unsigned>(ceil_div(a.n_rows, rows_per_round<false>(plan)));
+      FLCE_LAUNCH((norm_forward_narrow_kernel<T, W, kCentered>), all, kNarrowThreads, stream, a);
+      return FLCE_OK;
+    }
+    case kNormScalar:
+      if (plan.share == 1) FLCE_LAUNCH((norm_forward_scalar_kernel<T, W, kCentered, 1>), grid, kScalarThreads, stream, a);
+      else if (plan.share == 4) FLCE_LAUNCH((norm_forward_scalar_kernel<T, W, kCentered, 4>), grid, kScalarThreads, stream, a);
+      else FLCE_LAUNCH((norm_forward_scalar_kernel<T, W, kCentered, 16>), grid, kScalarThreads, stream, a);
+      return FLCE_OK;
+    default:
+      FLCE_LAUNCH((norm_forward_long_kernel<T, W, kCentered>), static_cast<unsigned>(a.n_rows), kNormMaxThreads, stream, a);
+      return FLCE_OK;
   }
 }
 
 template <typename T, typename W, bool kCentered>
-int run_backward_stream(const NormBackwardArgs& a, const NormShape& s, unsigned blocks, cudaStream_t stream) {
-  const dim3 grid(blocks);
-  switch (s.ept) {
-    case 1: return launch_with_shared<norm_backward_stream_kernel<T, W, kCentered, 1>>(grid, kStreamThreads, Stream<1, true>::kRingBytes, stream, a);
-    case 2: return launch_with_shared<norm_backward_stream_kernel<T, W, kCentered, 2>>(grid, kStreamThreads, Stream<2, true>::kRingBytes, stream, a);
-    default: return launch_with_shared<norm_backward_stream_kernel<T, W, kCentered, 4>>(grid, kStreamThreads, Stream<4, true>::kRingBytes, stream, a);
+int run_backward(const NormBackwardArgs& a, const NormPlan& plan, unsigned walking, cudaStream_t stream) {
+  const dim3 grid(walking);
+  switch (plan.path) {
+    case kNormStream:
+      if (plan.share == 2)
+        return launch_with_shared<norm_backward_stream_kernel<T, W, kCentered, 2>>(grid, kStreamThreads, Stream<2, true>::kRingBytes, stream, a);
+      return launch_with_shared<norm_backward_stream_kernel<T, W, kCentered, 4>>(grid, kStreamThreads, Stream<4, true>::kRingBytes, stream, a);
+    case kNormNarrow:
+      FLCE_LAUNCH((norm_backward_narrow_kernel<T, W, kCentered>), grid, kNarrowThreads, stream, a);
+      return FLCE_OK;
+    case kNormScalar:
+      if (plan.share == 1) FLCE_LAUNCH((norm_backward_scalar_kernel<T, W, kCentered, 1>), grid, kScalarThreads, stream, a);
+      else if (plan.share == 4) FLCE_LAUNCH((norm_backward_scalar_kernel<T, W, kCentered, 4>), grid, kScalarThreads, stream, a);
+      else FLCE_LAUNCH((norm_backward_scalar_kernel<T, W, kCentered, 16>), grid, kScalarThreads, stream, a);
+      return FLCE_OK;
+    default:
+      FLCE_LAUNCH((norm_backward_long_kernel<T, W, kCentered>), static_cast<unsigned>(a.n_rows), kNormMaxThreads, stream, a);
+      if (a.dw_partial != nullptr || a.db_partial != nullptr) {
+        const dim3 columns(static_cast<unsigned>(ceil_div(a.hidden, kNormColumnThreads)), walking);
+        FLCE_LAUNCH((norm_parameter_partial_long_kernel<T, kCentered>), columns, kNormColumnThreads, stream, a);
+      }
+      return FLCE_OK;
   }
 }
 
@@ -196,39 +182,13 @@ int flce_b200_norm_forward(const flce_norm_t* p, void* y, float* mean, float* rs
   a.eps = p->eps;
   a.offset = p->offset;
   a.round_xhat = p->round_xhat;
-  const NormPlan plan = norm_plan(p, whole_vectors(p, y, p->hidden), kNormForwardThreads);
-  const NormShape& s = plan.shape;
-  a.log2_group = s.log2_group;
-  const int threads = (1 << s.log2_group) > kNormForwardThreads ? (1 << s.log2_group) : kNormForwardThreads;
-  const bool centered = p->kind == FLCE_LAYER_NORM;
+  const NormPlan plan = norm_plan(p, whole_vectors(p, y, p->hidden));
+  a.log2_group = plan.log2_group;
+  const unsigned walking = static_cast<unsigned>(walking_blocks<false>(p, plan, sms));
   with_types(p, [&](auto t, auto w) {
     using T = decltype(t);
     using W = decltype(w);
-    constexpr int kVec = CeElem<T>::kVec;
-    if (plan.path == kNormStream) {
-      rc = centered ? run_forward_stream<T, W, true>(a, s, sms, stream) : run_forward_stream<T, W, false>(a, s, sms, stream);
-      return;
-    }
-    if (plan.path == kNormNarrow) {
-      const unsigned grid = static_cast<unsigned>(ceil_div(p->n_rows, (kNarrowThreads >> s.log2_group) * kNarrowForwardRows));
-      if (centered) FLCE_LAUNCH((norm_forward_narrow_kernel<T, W, true, kNarrowForwardRows>), grid, kNarrowThreads, stream, a);
-      else FLCE_LAUNCH((norm_forward_narrow_kernel<T, W, false, kNarrowForwardRows>), grid, kNarrowThreads, stream, a);
-      return;
-    }
-    if (!s.fits) {
-      const unsigned grid = static_cast<unsigned>(p->n_rows);
-      if (centered) FLCE_LAUNCH((norm_forward_long_kernel<T, W, true>), grid, kNormMaxThreads, stream, a);
-      else FLCE_LAUNCH((norm_forward_long_kernel<T, W, false>), grid, kNormMaxThreads, stream, a);
-      return;
-    }
-    const unsigned grid = static_cast<unsigned>(ceil_div(p->n_rows, threads >> s.log2_group));
-    if (s.unit == 1) {
-      if (centered) run_forward<T, W, true, 1>(a, s, grid, threads, stream);
-      else run_forward<T, W, false, 1>(a, s, grid, threads, stream);
-    } else {
-      if (centered) run_forward<T, W, true, kVec>(a, s, grid, threads, stream);
-      else run_forward<T, W, false, kVec>(a, s, grid, threads, stream);
-    }
+    rc = p->kind == FLCE_LAYER_NORM ? run_forward<T, W, true>(a, plan, walking, stream) : run_forward<T, W, false>(a, plan, walking, stream);
   });
   if (rc != FLCE_OK) return rc;
   FLCE_CUDA(cudaGetLastError());
@@ -241,8 +201,8 @@ size_t flce_b200_norm_workspace_bytes(const flce_norm_t* p) {
   int sms = 0;
   if (current_sm_count(&sms) != FLCE_OK) return 0;
   // the row's spread may turn out either way (the gradient's alignment is not known yet): room for the larger grid
-  const long long blocks_vec = backward_blocks(p, norm_plan(p, true, kNormMaxThreads), sms);
-  const long long blocks_one = backward_blocks(p, norm_plan(p, false, kNormMaxThreads), sms);
+  const long long blocks_vec = walking_blocks<true>(p, norm_plan(p, true), sms);
+  const long long blocks_one = walking_blocks<true>(p, norm_plan(p, false), sms);
   const long long blocks = blocks_vec > blocks_one ? blocks_vec : blocks_one;
   return static_cast<size_t>(blocks) * static_cast<size_t>(p->hidden) * sizeof(float) * (p->kind == FLCE_LAYER_NORM ? 2 : 1);
 }
@@ -268,9 +228,8 @@ int flce_b200_norm_backward(const flce_norm_t* p, const void* grad_y, int64_t ld
   int sms = 0;
   rc = current_sm_count(&sms);
   if (rc != FLCE_OK) return rc;
-  const NormPlan plan = norm_plan(p, whole_vectors(p, grad_y, ld_grad) && aligned16(grad_x), kNormMaxThreads);
-  const NormShape& s = plan.shape;
-  const long long blocks = backward_blocks(p, plan, sms);
+  const NormPlan plan = norm_plan(p, whole_vectors(p, grad_y, ld_grad) && aligned16(grad_x));
+  const long long blocks = walking_blocks<true>(p, plan, sms);
   const bool parameters = grad_weight != nullptr || grad_bias != nullptr;
   const size_t plane = static_cast<size_t>(blocks) * static_cast<size_t>(p->hidden);
   const size_t planes = (grad_weight != nullptr ? 1 : 0) + (grad_bias != nullptr ? 1 : 0);
@@ -293,43 +252,22 @@ int flce_b200_norm_backward(const flce_norm_t* p, const void* grad_y, int64_t ld
   a.hidden = static_cast<int>(p->hidden);
   a.offset = p->offset;
   a.round_xhat = p->round_xhat;
-  a.log2_group = s.log2_group;
-  const unsigned grid = static_cast<unsigned>(blocks);
+  a.log2_group = plan.log2_group;
+  const unsigned walking = static_cast<unsigned>(blocks);
   with_types(p, [&](auto t, auto w) {
     using T = decltype(t);
     using W = decltype(w);
-    constexpr int kVec = CeElem<T>::kVec;
-    if (plan.path == kNormStream) {
-      rc = centered ? run_backward_stream<T, W, true>(a, s, grid, stream) : run_backward_stream<T, W, false>(a, s, grid, stream);
-      if (rc != FLCE_OK) return;
-    } else if (plan.path == kNormNarrow) {
-      if (centered) FLCE_LAUNCH((norm_backward_narrow_kernel<T, W, true, kNarrowBackwardRows>), grid, kNarrowThreads, stream, a);
-      else FLCE_LAUNCH((norm_backward_narrow_kernel<T, W, false, kNarrowBackwardRows>), grid, kNarrowThreads, stream, a);
-    } else if (!s.fits) {
-      const unsigned rows = static_cast<unsigned>(p->n_rows);
-      const dim3 columns(static_cast<unsigned>(ceil_div(p->hidden, kNormForwardThreads)), grid < 65535u ? grid : 65535u);
-      if (centered) FLCE_LAUNCH((norm_backward_long_kernel<T, W, true>), rows, kNormMaxThreads, stream, a);
-      else FLCE_LAUNCH((norm_backward_long_kernel<T, W, false>), rows, kNormMaxThreads, stream, a);
-      if (parameters) {
-        if (centered) FLCE_LAUNCH((norm_parameter_partial_long_kernel<T, true>), columns, kNormForwardThreads, stream, a);
-        else FLCE_LAUNCH((norm_parameter_partial_long_kernel<T, false>), columns, kNormForwardThreads, stream, a);
-      }
-    } else if (s.unit == 1) {
-      if (centered) run_backward<T, W, true, 1>(a, s, grid, stream);
-      else run_backward<T, W, false, 1>(a, s, grid, stream);
-    } else {
-      if (centered) run_backward<T, W, true, kVec>(a, s, grid, stream);
-      else run_backward<T, W, false, kVec>(a, s, grid, stream);
-    }
+    rc = centered ? run_backward<T, W, true>(a, plan, walking, stream) : run_backward<T, W, false>(a, plan, walking, stream);
+    if (rc != FLCE_OK) return;
     if (parameters) {
       const dim3 columns(static_cast<unsigned>(ceil_div(p->hidden, 32)), centered ? 2 : 1);
       FLCE_LAUNCH((norm_parameter_gradient_kernel<W>), columns, dim3(32, kNormReduceLanes), stream, 
-          a.dw_partial, a.db_partial, static_cast<int>(grid), a.hidden, static_cast<W*>(grad_weight), static_cast<W*>(grad_bias));
+          a.dw_partial, a.db_partial, static_cast<int>(walking), a.hidden, static_cast<W*>(grad_weight), static_cast<W*>(grad_bias));
     }
   });
   if (rc != FLCE_OK) return rc;
   FLCE_CUDA(cudaGetLastError());
-  count_launches(1 + (parameters ? (s.fits ? 1 : 2) : 0));
+  count_launches(1 + (parameters ? (plan.path == kNormLong ? 2 : 1) : 0));
   return FLCE_OK;
 }
 

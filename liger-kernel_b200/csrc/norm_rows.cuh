@@ -7,14 +7,17 @@
 //                dw = sum over rows of dy * xhat,  db = sum over rows of dy
 //
 // Both directions are bound by HBM: forward moves a row in and out, backward two rows in and one out.  A row is read once and
-// stays in the registers of the threads that share it, so the variance is taken around the mean that is already known (no
-// sum of squares minus square of sum) at no further traffic.  A *group* of 2..512 threads shares a row; a block holds as many
-// groups as fit, so narrow rows need no barrier and wide rows have one per reduction.  Everything between load and store is
-// fp32; the only roundings to fewer bits are those of the results, and of xhat in the "llama" casting mode, which asks for it.
+// stays on the SM, so the variance is taken around the mean that is already known (no sum of squares minus square of sum)
+// at no further traffic.  A *group* of 4..512 threads shares a row; a block holds as many groups as fit, so narrow rows need no
+// barrier.  Everything between load and store is fp32; the only roundings to fewer bits are those of the results, and of
+// xhat in the "llama" casting mode, which asks for it.
 //
-// In backward a thread keeps the same columns for all rows of its block, so the weight's and the bias's gradient are sums in
-// its registers; blocks leave one partial sum per column, added up in block order by a second kernel: no atomics, the same
-// bits in every run.  The next row is on its way while the current one is reduced.
+// A thread keeps the same columns for all its rows.  In backward the weight's and the bias's gradient are therefore sums in its
+// registers; blocks leave one partial sum per column, added up in block order by a second kernel: no atomics, the same
+// bits in every run.
+//
+// Four forms: rows of aligned 16-byte vectors, streamed (wide) or in registers (narrow), rows without that alignment (scalar), and
+// rows longer than a block's threads hold (long).
 #pragma once
 
 #include <type_traits>
@@ -25,10 +28,9 @@
 
 namespace flce {
 
-constexpr int kNormMaxThreads = 512;     // largest group, and the block of the backward kernel
-constexpr int kNormForwardThreads = 256; // block of the forward kernel unless a row needs a larger group
+constexpr int kNormMaxThreads = 512;     // largest group of threads that shares a row
 constexpr int kNormMaxWarps = kNormMaxThreads / 32;
-constexpr int kNormMaxEpt = 32;          // elements of a row per thread: rows of up to 16384 elements stay in registers
+constexpr int kNormColumnThreads = 256;
 
 struct NormForwardArgs {
   const void* x;
@@ -63,83 +65,6 @@ struct NormBackwardArgs {
   int log2_group;
 };
 
-// One thread's share of a row: kEpt elements as kEpt / kUnit units of kUnit consecutive ones.  The units of a warp lie side by
-// side in strides of 32, so that neighbouring threads touch neighbouring memory and a thread's accesses differ by constants;
-// groups of fewer than 32 threads have one unit per thread.  kUnit is 1, or as many elements of the row's type as fill
-// 16 bytes; then rows start on 16-byte boundaries and hold whole units.
-template <int kUnit, int kEpt>
-__device__ __forceinline__ int norm_first_column(int t) {
-  constexpr int kUnits = kEpt / kUnit;
-  return (kUnits == 1 ? t : (t >> 5) * 32 * kUnits + (t & 31)) * kUnit;
-}
-template <int kUnit>
-__device__ __forceinline__ int norm_column(int first, int e) {
-  return first + (e / kUnit) * 32 * kUnit + e % kUnit;
-}
-
-template <typename E, int kUnit, int kEpt>
-struct NormChunk {
-  static constexpr int kUnits = kEpt / kUnit;
-  static constexpr int kPer = kUnit == 1 ? 1 : kUnit * static_cast<int>(sizeof(E)) / 16;   // words per unit
-  typedef typename std::conditional<kUnit == 1, E, uint4>::type Word;
-  Word q[kUnits * kPer];
-
-  // zeros behind the row's end
-  __device__ __forceinline__ void load(const E* row, int first, int hidden) {
-    const Word* p = reinterpret_cast<const Word*>(row + first);
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        q[u * kPer + i] = Word();
-        if (first + u * 32 * kUnit < hidden) q[u * kPer + i] = p[u * 32 * kPer + i];
-      }
-    }
-  }
-  __device__ __forceinline__ float get(int e) const { return CeElem<E>::load(reinterpret_cast<const E*>(q) + e); }
-  __device__ __forceinline__ void set(int e, float v) { CeElem<E>::store(reinterpret_cast<E*>(q) + e, v); }
-
-  __device__ __forceinline__ void store(E* row, int first, int hidden) const {
-    Word* p = reinterpret_cast<Word*>(row + first);
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        if (first + u * 32 * kUnit < hidden) p[u * 32 * kPer + i] = q[u * kPer + i];
-      }
-    }
-  }
-};
-
-// Sums of kN values over each group, returned to all its threads; every thread of the block calls it.  Groups of more than a
-// warp meet in shared memory, in one of two buffers taken in turn: a thread writes a buffer again only behind the barrier
-// of the call in between, which the readers of the older sums reach after reading them, so one barrier per call is enough.
-template <int kN>
-__device__ __forceinline__ void norm_group_sum(float (&v)[kN], int log2_group, float (*scratch)[kNormMaxWarps * kN], int& phase) {
-  const int lanes = log2_group < 5 ? (1 << log2_group) : 32;
-  for (int o = lanes >> 1; o > 0; o >>= 1) {
-#pragma unroll
-    for (int i = 0; i < kN; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-  }
-  if (log2_group <= 5) return;
-  float* buf = scratch[phase];
-  phase ^= 1;
-  const int tid = static_cast<int>(threadIdx.x);
-  if ((tid & 31) == 0) {
-#pragma unroll
-    for (int i = 0; i < kN; ++i) buf[(tid >> 5) * kN + i] = v[i];
-  }
-  __syncthreads();
-  const int warps = 1 << (log2_group - 5);
-  const float* mine = buf + (tid >> log2_group) * warps * kN;
-#pragma unroll
-  for (int i = 0; i < kN; ++i) v[i] = 0.f;
-  for (int w = 0; w < warps; ++w) {
-#pragma unroll
-    for (int i = 0; i < kN; ++i) v[i] += mine[w * kN + i];
-  }
-}
-
 template <typename T>
 __device__ __forceinline__ float norm_round(float v) {
   T r;
@@ -147,221 +72,61 @@ __device__ __forceinline__ float norm_round(float v) {
   return CeElem<T>::load(&r);
 }
 
-// y and the row statistics.  One row per group; blocks of 256 threads, or of the group if that is larger.
-template <typename T, typename W, bool kCentered, int kUnit, int kEpt>
-__global__ void __launch_bounds__(kNormMaxThreads)
-norm_forward_kernel(NormForwardArgs a) {
-  __shared__ float scratch[2][kNormMaxWarps];
-  const int group = 1 << a.log2_group;
-  const int t = static_cast<int>(threadIdx.x) & (group - 1);
-  const int first = norm_first_column<kUnit, kEpt>(t);
-  const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x >> a.log2_group) + (threadIdx.x >> a.log2_group);
-  const bool live = row < a.n_rows;
-  const int hidden = live ? a.hidden : 0;     // a group behind the last row takes part in the barriers only
-  const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.ld_x;
-  NormChunk<T, kUnit, kEpt> c;
-  c.load(x, first, hidden);
-  float v[kEpt];
-  float s[1] = {0.f};
-#pragma unroll
-  for (int e = 0; e < kEpt; ++e) v[e] = c.get(e);
-  int phase = 0;
-  float mean = 0.f;
-  if constexpr (kCentered) {
-#pragma unroll
-    for (int e = 0; e < kEpt; ++e) s[0] += v[e];
-    norm_group_sum<1>(s, a.log2_group, scratch, phase);
-    mean = s[0] / static_cast<float>(a.hidden);
-    s[0] = 0.f;
-#pragma unroll
-    for (int e = 0; e < kEpt; ++e) {
-      v[e] = norm_column<kUnit>(first, e) < hidden ? v[e] - mean : 0.f;
-      s[0] = fmaf(v[e], v[e], s[0]);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < kEpt; ++e) s[0] = fmaf(v[e], v[e], s[0]);
-  }
-  norm_group_sum<1>(s, a.log2_group, scratch, phase);
-  if (!live) return;
-  const float rstd = 1.f / sqrtf(s[0] / static_cast<float>(a.hidden) + a.eps);
-  if (t == 0) {
-    if (kCentered && a.mean != nullptr) a.mean[row] = mean;
-    if (a.rstd != nullptr) a.rstd[row] = rstd;
-  }
-  NormChunk<T, kUnit, kEpt> y;
-  const bool rounded = !kCentered && a.round_xhat != 0;
-#pragma unroll
-  for (int e = 0; e < kEpt; ++e) {
-    v[e] *= rstd;
-    if (rounded) v[e] = norm_round<T>(v[e]);
-  }
-  if (a.w != nullptr) {
-    NormChunk<W, kUnit, kEpt> w;
-    w.load(static_cast<const W*>(a.w), first, hidden);
-    if (a.b != nullptr) {
-      NormChunk<W, kUnit, kEpt> b;
-      b.load(static_cast<const W*>(a.b), first, hidden);
-#pragma unroll
-      for (int e = 0; e < kEpt; ++e) v[e] = fmaf(v[e], a.offset + w.get(e), b.get(e));
-    } else {
-#pragma unroll
-      for (int e = 0; e < kEpt; ++e) v[e] *= a.offset + w.get(e);
-    }
-  } else if (a.b != nullptr) {
-    NormChunk<W, kUnit, kEpt> b;
-    b.load(static_cast<const W*>(a.b), first, hidden);
-#pragma unroll
-    for (int e = 0; e < kEpt; ++e) v[e] += b.get(e);
-  }
-#pragma unroll
-  for (int e = 0; e < kEpt; ++e) y.set(e, v[e]);
-  y.store(static_cast<T*>(a.y) + row * a.hidden, first, hidden);
+// 1 / sqrt(v) to the last bit or two: the hardware's estimate and one Newton step (v > 0; NaN and infinity pass through)
+__device__ __forceinline__ float norm_rsqrt(float v) {
+  const float r = rsqrtf(v);
+  return v < INFINITY ? r * fmaf(-0.5f * v * r, r, 1.5f) : r;
 }
 
-// dx, and this block's share of the parameters' gradients.  A fixed grid of blocks of 512 threads walks over the rows.  The
-// rows are kept as they were loaded and converted again after the reduction: the registers go to the sums and to the next row.
-template <typename T, typename W, bool kCentered, int kUnit, int kEpt>
-__global__ void __launch_bounds__(kNormMaxThreads)
-norm_backward_kernel(NormBackwardArgs a) {
-  constexpr int kSums = kCentered ? 2 : 1;
-  constexpr bool kAhead = kEpt * sizeof(T) <= 32;      // room for the next row beside the current one
-  __shared__ float scratch[2][kNormMaxWarps * kSums];
-  __shared__ float fold[kNormMaxThreads / 2 * kEpt];
-  const int group = 1 << a.log2_group;
-  const int t = static_cast<int>(threadIdx.x) & (group - 1);
-  const int first = norm_first_column<kUnit, kEpt>(t);
-  const int g = static_cast<int>(threadIdx.x) >> a.log2_group;
-  const int groups = static_cast<int>(blockDim.x) >> a.log2_group;
-  const long long step = static_cast<long long>(gridDim.x) * groups;
-  const bool rounded = !kCentered && a.round_xhat != 0;
-  const bool gain = a.w != nullptr;
-  typedef NormChunk<T, kUnit, kEpt> Row;
-  typedef NormChunk<W, kUnit, kEpt> Parameters;
+// ---- four sums at a time
+//
+// Lanes that differ in the group's highest bit trade two sums for the other two, those that differ in the next bit one for the
+// other: 5 or 6 exchanges for four sums instead of 16 or 20.  The lane's two highest bits within its group (of its warp, if
+// the group is wider) then name its sum.
+__device__ __forceinline__ float norm_low_lane_sum(float v, int lanes) {      // over `lanes` neighbouring lanes
+  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float norm_lane_four_sums(const float (&v)[4], int lanes) {      // lanes: 4, 8, 16 or 32
+  const int lane = static_cast<int>(threadIdx.x) & 31;
+  const int half = lanes >> 1, quarter = lanes >> 2;
+  const bool up = (lane & half) != 0, right = (lane & quarter) != 0;
+  const float a0 = __shfl_xor_sync(0xffffffffu, up ? v[0] : v[2], half) + (up ? v[2] : v[0]);
+  const float a1 = __shfl_xor_sync(0xffffffffu, up ? v[1] : v[3], half) + (up ? v[3] : v[1]);
+  return norm_low_lane_sum(__shfl_xor_sync(0xffffffffu, right ? a0 : a1, quarter) + (right ? a1 : a0), quarter);
+}
 
-  Parameters w;
-  w.load(static_cast<const W*>(a.w), first, gain ? a.hidden : 0);
-  float dw[kEpt], db[kCentered ? kEpt : 1];
-#pragma unroll
-  for (int e = 0; e < kEpt; ++e) {
-    dw[e] = 0.f;
-    if (kCentered) db[e] = 0.f;
-  }
-  struct Fetched {
-    Row x, dy;
-    float mean, rstd;
-  };
-  // a row behind the last one is loaded as zeros: it adds nothing and is not stored
-  auto fetch = [&](Fetched& f, long long row) {
-    const bool live = row < a.n_rows;
-    const int hidden = live ? a.hidden : 0;
-    const long long r = live ? row : 0;
-    f.x.load(static_cast<const T*>(a.x) + r * a.ld_x, first, hidden);
-    f.dy.load(static_cast<const T*>(a.dy) + r * a.ld_dy, first, hidden);
-    f.mean = kCentered && live ? a.mean[r] : 0.f;
-    f.rstd = live ? a.rstd[r] : 0.f;
-  };
-  Fetched cur;
-  long long row = static_cast<long long>(blockIdx.x) * groups;
-  if (kAhead) fetch(cur, row + g);
-  int phase = 0;
-  for (; row < a.n_rows; row += step) {       // the same number of rounds in every thread of the block
-    Fetched next;
-    if (kAhead) {
-      if (row + step < a.n_rows) fetch(next, row + step + g);
-    } else {
-      fetch(cur, row + g);
-    }
-    float s[kSums] = {};
-#pragma unroll
-    for (int e = 0; e < kEpt; ++e) {
-      // the columns behind the row's end hold dy = 0, which keeps their xhat out of every sum
-      const float xhat = (cur.x.get(e) - cur.mean) * cur.rstd;
-      float d = cur.dy.get(e);
-      dw[e] = fmaf(d, rounded ? norm_round<T>(xhat) : xhat, dw[e]);
-      if (kCentered) db[e] += d;
-      if (gain) d *= a.offset + w.get(e);
-      s[0] = fmaf(d, xhat, s[0]);
-      if (kCentered) s[kSums - 1] += d;
-    }
-    norm_group_sum<kSums>(s, a.log2_group, scratch, phase);
-    const float c = s[0] / static_cast<float>(a.hidden);
-    const float m = kCentered ? s[kSums - 1] / static_cast<float>(a.hidden) : 0.f;
-    if (row + g < a.n_rows) {
-      Row out;
-#pragma unroll
-      for (int e = 0; e < kEpt; ++e) {
-        const float xhat = (cur.x.get(e) - cur.mean) * cur.rstd;
-        float d = cur.dy.get(e);
-        if (gain) d *= a.offset + w.get(e);
-        out.set(e, cur.rstd * (fmaf(-xhat, c, d) - m));
-      }
-      out.store(static_cast<T*>(a.dx) + (row + g) * a.hidden, first, a.hidden);
-    }
-    if (kAhead) cur = next;
-  }
-  // the groups of the block, folded in halves in a fixed order
-  auto leave = [&](float (&acc)[kEpt], float* partial) {
-    for (int half = groups >> 1; half > 0; half >>= 1) {
-      __syncthreads();
-      if (g >= half && g < 2 * half) {
-#pragma unroll
-        for (int e = 0; e < kEpt; ++e) fold[((g - half) * kEpt + e) * group + t] = acc[e];
-      }
-      __syncthreads();
-      if (g < half) {
-#pragma unroll
-        for (int e = 0; e < kEpt; ++e) acc[e] += fold[(g * kEpt + e) * group + t];
-      }
-    }
-    if (g == 0) {
-      float* mine = partial + static_cast<size_t>(blockIdx.x) * a.hidden;
-#pragma unroll
-      for (int e = 0; e < kEpt; ++e) {
-        const int col = norm_column<kUnit>(first, e);
-        if (col < a.hidden) mine[col] = acc[e];
-      }
-    }
-  };
-  if (a.dw_partial != nullptr) leave(dw, a.dw_partial);
-  if constexpr (kCentered) {
-    if (a.db_partial != nullptr) leave(db, a.db_partial);
-  }
+// Over a group of 1 << log2_group threads, 4 or more.  Warps meet in one of two buffers taken in turn: a thread writes a buffer
+// again only behind the barrier of the call in between, which the readers of the older sums reach after reading them, so
+// one barrier per call is enough.
+__device__ __forceinline__ float norm_group_four_sums(const float (&v)[4], int log2_group, float (*scratch)[kNormMaxWarps * 4], int& phase) {
+  float sum = norm_lane_four_sums(v, log2_group < 5 ? 1 << log2_group : 32);
+  if (log2_group <= 5) return sum;
+  const int lane = static_cast<int>(threadIdx.x) & 31, warps = 1 << (log2_group - 5), g = static_cast<int>(threadIdx.x) >> log2_group;
+  float* buf = scratch[phase];
+  phase ^= 1;
+  if ((lane & 7) == 0) buf[(threadIdx.x >> 5) * 4 + (lane >> 3)] = sum;
+  named_barrier(1 + g, 1 << log2_group);
+  const float* of = buf + g * warps * 4 + (lane >> 3);
+  sum = 0.f;
+  for (int w = lane & 7; w < warps; w += 8) sum += of[w * 4];
+  return norm_low_lane_sum(sum, 8);
+}
+// sum number i of those, from a lane that holds it
+__device__ __forceinline__ float norm_of_four(float sums, int i, int log2_group) {
+  const int lanes = log2_group < 5 ? 1 << log2_group : 32;
+  return __shfl_sync(0xffffffffu, sums, (static_cast<int>(threadIdx.x) & 31 & ~(lanes - 1)) | i * (lanes >> 2));
 }
 
 // ---- rows of whole, aligned 16-byte vectors, more than a warp's worth: streamed through shared memory
 //
-// What the kernels above lose is not bandwidth but issue slots and waiting: at 32768 x 4096 bf16 they ran at 46 % (forward) and
-// 41 % (backward) of the copy rate with rows of one warp reaching 55 % and fp32 rows, with half the elements per byte, 87 %.
-// Here the arithmetic goes two elements to an instruction, and the next rows are always on their way: every thread copies
-// the vectors that it will read itself, with cp.async, so the ring needs no barrier and no wait on another thread.
+// One row at a time per block, in registers, loses not bandwidth but issue slots and waiting: at 32768 x 4096 bf16 such kernels
+// ran at 46 % (forward) and 41 % (backward) of the copy rate, with fp32 rows, half the elements per byte, forward at 87 %.
+// Here the arithmetic goes two elements to an instruction, several rows share a barrier, and the next rows are always on
+// their way: every thread copies the vectors that it will read itself, with cp.async, so the ring needs no barrier and no
+// wait on another thread.
 
 constexpr int kStreamThreads = 512;
-
-// Four sums over a group of `warps` warps.  In a warp by six exchanges: lanes that differ in bit 4 trade two sums for the other
-// two, those that differ in bit 3 one for the other; bits 4 and 3 of the lane then name its sum.  Across warps through one of
-// two buffers, taken in turn (see norm_group_sum).  Returns sum number lane >> 3, the same in the eight lanes that share it.
-__device__ __forceinline__ float stream_four_sums(const float (&v)[4], int warps, int group_id, float (*scratch)[kNormMaxWarps * 4],
-                                                  int& phase) {
-  const int lane = static_cast<int>(threadIdx.x) & 31;
-  const bool up = (lane & 16) != 0, right = (lane & 8) != 0;
-  const float a0 = __shfl_xor_sync(0xffffffffu, up ? v[0] : v[2], 16) + (up ? v[2] : v[0]);
-  const float a1 = __shfl_xor_sync(0xffffffffu, up ? v[1] : v[3], 16) + (up ? v[3] : v[1]);
-  float sum = __shfl_xor_sync(0xffffffffu, right ? a0 : a1, 8) + (right ? a1 : a0);
-#pragma unroll
-  for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (warps == 1) return sum;
-  float* buf = scratch[phase];
-  phase ^= 1;
-  if ((lane & 7) == 0) buf[(threadIdx.x >> 5) * 4 + (lane >> 3)] = sum;
-  named_barrier(1 + group_id, warps * 32);
-  const float* of = buf + group_id * warps * 4 + (lane >> 3);
-  sum = 0.f;
-  for (int w = lane & 7; w < warps; w += 8) sum += of[w * 4];
-#pragma unroll
-  for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum;
-}
 
 // kUnits vectors of a parameter, zeros where there is none
 template <typename W, int kUnits, int kWVecs>
@@ -377,21 +142,23 @@ __device__ __forceinline__ void stream_load_parameter(const void* src, int first
   }
 }
 
-// Shape of the streaming kernels by the vectors per thread: rows that a group takes per round, rounds in the ring, blocks per SM.
-// Two rows of backward are four sums, as four rows of forward are.
+// Shape of the streaming kernels by the vectors per thread, 2 or 4: rows that a group takes per round (two rows of backward are
+// four sums, as four rows of forward are), rounds in the ring, which takes 128 or 192 KB: one block per SM.
+// With one vector per thread the groups are twice as wide and wait longer for each other: 32768 x 4096 bf16 backward 158 us
+// against 127, forward 124 against 88; with four in rows that two would hold, registers run out (138 and 138 us).
 template <int kUnits, bool kGrad>
 struct Stream {
-  static constexpr int kRows = kUnits == 4 ? 1 : (kUnits == 2 || kGrad ? 2 : 4);
-  static constexpr int kSlots = 3;
-  static constexpr int kBlocksPerSm = kUnits == 1 ? 2 : 1;
+  static constexpr int kRows = kUnits == 4 ? 1 : (kGrad ? 2 : 4);
+  static constexpr int kSlots = kUnits == 2 && !kGrad ? 2 : 3;
   static constexpr int kRingBytes = kSlots * kRows * (kGrad ? 2 : 1) * kUnits * kStreamThreads * 16;
 };
 
 // y and the row statistics.  Each thread of a group owns kUnits vectors of columns, their gain and bias in registers; a group takes
-// kRows rows per round, which meet in one reduction (one barrier, if the group is wider than a warp) for the means and one for
-// the variances.  A fixed grid walks over the rows.
+// kRows rows per round.  Each warp centres its part of a row on that part's own mean; across warps the parts' sums and squares
+// meet behind one barrier, sum (x - mean)^2 = sum over parts of (squares + elements * (part's mean - mean)^2): nothing is
+// subtracted that has to cancel.  A fixed grid walks over the rows.
 template <typename T, typename W, bool kCentered, int kUnits>
-__global__ void __launch_bounds__(kStreamThreads, (Stream<kUnits, false>::kBlocksPerSm))
+__global__ void __launch_bounds__(kStreamThreads, 1)
 norm_forward_stream_kernel(NormForwardArgs a) {
   constexpr int kRows = Stream<kUnits, false>::kRows, kSlots = Stream<kUnits, false>::kSlots;
   constexpr int kVec = CeElem<T>::kVec;
@@ -399,11 +166,13 @@ norm_forward_stream_kernel(NormForwardArgs a) {
   constexpr int kWVecs = kVec * static_cast<int>(sizeof(W)) / 16;
   FLCE_DYNAMIC_SHARED(uint4, stream_ring);                    // [slot][row][unit][thread]
   __shared__ float scratch[2][kNormMaxWarps * 4];
+  __shared__ float scratch_sums[2][kCentered ? kNormMaxWarps * 4 : 1];
   const int group = 1 << a.log2_group;
   const int warps = group >> 5;
   const int groups = kStreamThreads >> a.log2_group;
   const int g = static_cast<int>(threadIdx.x) >> a.log2_group;
   const int t = static_cast<int>(threadIdx.x) & (group - 1);
+  const int lane = static_cast<int>(threadIdx.x) & 31;
   const int first = (t >> 5) * 32 * kUnits + (t & 31);        // this lane's first vector; the others follow in strides of 32
   const int vectors = a.hidden / kVec;
   const long long step = static_cast<long long>(gridDim.x) * groups * kRows;
@@ -431,13 +200,19 @@ norm_forward_stream_kernel(NormForwardArgs a) {
   for (int s = 0; s < kSlots - 1; ++s) fetch(row + s * step, s);
   int slot = 0, phase = 0;
   const float inv = 1.f / static_cast<float>(a.hidden);
+  // elements of the row that warp w of a group holds
+  auto part_elements = [&](int w) {
+    const int left = vectors - w * 32 * kUnits;
+    return static_cast<float>((left < 0 ? 0 : (left < 32 * kUnits ? left : 32 * kUnits)) * kVec);
+  };
+  const float part_inv = part_elements(t >> 5) > 0.f ? 1.f / part_elements(t >> 5) : 0.f;
   for (; row < a.n_rows; row += step) {
     // into the slot of the round before this one, which this thread, its only reader, has read for the last time
     fetch(row + (kSlots - 1) * step, slot == 0 ? kSlots - 1 : slot - 1);
     async_wait<kSlots - 1>();
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     F2 minus_mean[kRows];
-    float mean = 0.f;                       // of row lane >> 3
+    float part_sum = 0.f;                   // this warp's, of row lane >> 3
     if constexpr (kCentered) {
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
@@ -450,11 +225,11 @@ norm_forward_stream_kernel(NormForwardArgs a) {
         }
         v[r] = f2_lo(acc) + f2_hi(acc);
       }
-      mean = stream_four_sums(v, warps, g, scratch, phase) * inv;
+      part_sum = norm_lane_four_sums(v, 32);
     }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      minus_mean[r] = both(kCentered ? -__shfl_sync(0xffffffffu, mean, r * 8) : 0.f);
+      const F2 centre = both(kCentered ? -__shfl_sync(0xffffffffu, part_sum, r * 8) * part_inv : 0.f);
       F2 acc = both(0.f);
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
@@ -463,16 +238,45 @@ norm_forward_stream_kernel(NormForwardArgs a) {
 #pragma unroll
           for (int i = 0; i < kPairs; ++i) {
             F2 e = Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw) + i * Pairs<T>::kWords);
-            if (kCentered) e = add2(e, minus_mean[r]);
+            if (kCentered) e = add2(e, centre);
             acc = fma2(e, e, acc);
           }
         }
       }
       v[r] = f2_lo(acc) + f2_hi(acc);
     }
-    const float rstd = 1.f / sqrtf(fmaf(stream_four_sums(v, warps, g, scratch, phase), inv, a.eps));
+    float square = norm_lane_four_sums(v, 32);
+    float mean = part_sum * part_inv;       // of row lane >> 3, once the parts have met
+    if (warps > 1) {
+      float *buf = scratch[phase], *buf_sums = scratch_sums[kCentered ? phase : 0];
+      phase ^= 1;                           // taken in turn: see norm_group_four_sums
+      if ((lane & 7) == 0) {
+        buf[(threadIdx.x >> 5) * 4 + (lane >> 3)] = square;
+        if (kCentered) buf_sums[(threadIdx.x >> 5) * 4 + (lane >> 3)] = part_sum;
+      }
+      named_barrier(1 + g, group);
+      // eight lanes add up a row's parts
+      const int of = g * warps * 4 + (lane >> 3);
+      square = 0.f;
+      if constexpr (kCentered) {
+        float sum = 0.f;
+        for (int w = lane & 7; w < warps; w += 8) sum += buf_sums[of + w * 4];
+        mean = norm_low_lane_sum(sum, 8) * inv;
+        for (int w = lane & 7; w < warps; w += 8) {
+          const float n = part_elements(w);
+          const float off = n > 0.f ? buf_sums[of + w * 4] / n - mean : 0.f;
+          square += fmaf(n * off, off, buf[of + w * 4]);
+        }
+      } else {
+        for (int w = lane & 7; w < warps; w += 8) square += buf[of + w * 4];
+      }
+      square = norm_low_lane_sum(square, 8);
+    }
+    const float rstd = norm_rsqrt(fmaf(square, inv, a.eps));
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) minus_mean[r] = both(kCentered ? -__shfl_sync(0xffffffffu, mean, r * 8) : 0.f);
     {
-      const int r = static_cast<int>(threadIdx.x & 31) >> 3;
+      const int r = lane >> 3;
       if ((t & ~24) == 0 && r < kRows && row + r < a.n_rows) {      // lanes 0, 8, 16, 24 of the group's first warp
         if (kCentered && a.mean != nullptr) a.mean[row + r] = mean;
         if (a.rstd != nullptr) a.rstd[row + r] = rstd;
@@ -512,7 +316,7 @@ norm_forward_stream_kernel(NormForwardArgs a) {
 // dx, and this block's share of the parameters' gradients.  Each thread of a group owns kUnits vectors of columns; a round
 // takes kRows rows per group, their sums meet in one reduction (and one barrier, if the group is wider than a warp).
 template <typename T, typename W, bool kCentered, int kUnits>
-__global__ void __launch_bounds__(kStreamThreads, (Stream<kUnits, true>::kBlocksPerSm))
+__global__ void __launch_bounds__(kStreamThreads, 1)
 norm_backward_stream_kernel(NormBackwardArgs a) {
   constexpr int kRows = Stream<kUnits, true>::kRows, kSlots = Stream<kUnits, true>::kSlots;
   constexpr int kVec = CeElem<T>::kVec;
@@ -618,7 +422,7 @@ norm_backward_stream_kernel(NormBackwardArgs a) {
       v[2 * r] = f2_lo(s_mx) + f2_hi(s_mx);
       if (kCentered) v[2 * r + 1] = f2_lo(s_m) + f2_hi(s_m);
     }
-    const float sum = stream_four_sums(v, warps, g, scratch, phase);
+    const float sum = norm_group_four_sums(v, a.log2_group, scratch, phase);
     const float inv = 1.f / static_cast<float>(a.hidden);
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
@@ -692,13 +496,15 @@ norm_backward_stream_kernel(NormBackwardArgs a) {
 }
 
 // ---- rows of at most 32 aligned 16-byte vectors: one vector per lane, several rows to a warp, kRows of them per thread at a
-// time, so that the loads and the shuffles of one row hide those of another
+// time, so that the loads of one row hide those of another.  Groups of 4 to 32 lanes.
 
 constexpr int kNarrowThreads = 256;
+constexpr int kNarrowForwardRows = 4, kNarrowBackwardRows = 2;      // four sums either way
 
-template <typename T, typename W, bool kCentered, int kRows>
+template <typename T, typename W, bool kCentered>
 __global__ void __launch_bounds__(kNarrowThreads)
 norm_forward_narrow_kernel(NormForwardArgs a) {
+  constexpr int kRows = kNarrowForwardRows;
   constexpr int kVec = CeElem<T>::kVec;
   constexpr int kPairs = kVec / 2;
   constexpr int kWVecs = kVec * static_cast<int>(sizeof(W)) / 16;
@@ -731,63 +537,62 @@ norm_forward_narrow_kernel(NormForwardArgs a) {
       bias[i] = Pairs<W>::get(reinterpret_cast<const uint32_t*>(b) + i * Pairs<W>::kWords);
     }
   }
-  float mean[kRows], square[kRows];
+  const float inv = 1.f / static_cast<float>(a.hidden);
+  float v[4];
+  float mean = 0.f;                         // of the row that this lane's sum belongs to
+  if constexpr (kCentered) {
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    mean[r] = 0.f;
-    if (kCentered) {
+    for (int r = 0; r < kRows; ++r) {
       F2 acc = both(0.f);
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) acc = add2(acc, Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw[r]) + i * Pairs<T>::kWords));
-      mean[r] = f2_lo(acc) + f2_hi(acc);
+      v[r] = f2_lo(acc) + f2_hi(acc);
     }
+    mean = norm_lane_four_sums(v, group) * inv;
   }
-  if (kCentered) {
-    for (int o = group >> 1; o > 0; o >>= 1) {
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) mean[r] += __shfl_xor_sync(0xffffffffu, mean[r], o);
-    }
-  }
+  F2 minus_mean[kRows];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    mean[r] /= static_cast<float>(a.hidden);
+    minus_mean[r] = both(kCentered ? -norm_of_four(mean, r, a.log2_group) : 0.f);
     F2 acc = both(0.f);
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
-      const F2 v = add2(Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw[r]) + i * Pairs<T>::kWords), both(-mean[r]));
-      acc = fma2(v, v, acc);
+      F2 e = Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw[r]) + i * Pairs<T>::kWords);
+      if (kCentered) e = add2(e, minus_mean[r]);
+      acc = fma2(e, e, acc);
     }
-    square[r] = column ? f2_lo(acc) + f2_hi(acc) : 0.f;
+    v[r] = column ? f2_lo(acc) + f2_hi(acc) : 0.f;
   }
-  for (int o = group >> 1; o > 0; o >>= 1) {
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) square[r] += __shfl_xor_sync(0xffffffffu, square[r], o);
+  const float rstd = norm_rsqrt(fmaf(norm_lane_four_sums(v, group), inv, a.eps));
+  {
+    const int r = t / (group >> 2);
+    const long long row = base + r * groups;
+    if (t % (group >> 2) == 0 && row < a.n_rows) {
+      if (kCentered && a.mean != nullptr) a.mean[row] = mean;
+      if (a.rstd != nullptr) a.rstd[row] = rstd;
+    }
   }
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const long long row = base + r * groups;
-    if (row >= a.n_rows) continue;
-    const float rstd = 1.f / sqrtf(square[r] / static_cast<float>(a.hidden) + a.eps);
-    if (t == 0) {
-      if (kCentered && a.mean != nullptr) a.mean[row] = mean[r];
-      if (a.rstd != nullptr) a.rstd[row] = rstd;
-    }
+    const F2 scale = both(norm_of_four(rstd, r, a.log2_group));
     uint4 out;
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
-      F2 v = Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw[r]) + i * Pairs<T>::kWords);
-      if (kCentered) v = add2(v, both(-mean[r]));
-      v = mul2(v, both(rstd));
-      if (rounded) v = f2(norm_round<T>(f2_lo(v)), norm_round<T>(f2_hi(v)));
-      Pairs<T>::set(reinterpret_cast<uint32_t*>(&out) + i * Pairs<T>::kWords, kCentered ? fma2(v, gain[i], bias[i]) : mul2(v, gain[i]));
+      F2 e = Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw[r]) + i * Pairs<T>::kWords);
+      if (kCentered) e = add2(e, minus_mean[r]);
+      e = mul2(e, scale);
+      if (rounded) e = f2(norm_round<T>(f2_lo(e)), norm_round<T>(f2_hi(e)));
+      Pairs<T>::set(reinterpret_cast<uint32_t*>(&out) + i * Pairs<T>::kWords, kCentered ? fma2(e, gain[i], bias[i]) : mul2(e, gain[i]));
     }
-    if (column) reinterpret_cast<uint4*>(static_cast<T*>(a.y) + row * a.hidden)[t] = out;
+    if (column && row < a.n_rows) reinterpret_cast<uint4*>(static_cast<T*>(a.y) + row * a.hidden)[t] = out;
   }
 }
 
-template <typename T, typename W, bool kCentered, int kRows>
+template <typename T, typename W, bool kCentered>
 __global__ void __launch_bounds__(kNarrowThreads)
 norm_backward_narrow_kernel(NormBackwardArgs a) {
+  constexpr int kRows = kNarrowBackwardRows;
   constexpr int kVec = CeElem<T>::kVec;
   constexpr int kPairs = kVec / 2;
   constexpr int kWVecs = kVec * static_cast<int>(sizeof(W)) / 16;
@@ -817,7 +622,7 @@ norm_backward_narrow_kernel(NormBackwardArgs a) {
   const float inv = 1.f / static_cast<float>(a.hidden);
   for (long long base = static_cast<long long>(blockIdx.x) * groups * kRows; base < a.n_rows; base += step) {
     uint4 raw_x[kRows], raw_dy[kRows];
-    float mean[kRows], rstd[kRows], s_mx[kRows], s_m[kRows];
+    float mean[kRows], rstd[kRows], v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {       // rows behind the last one come in as zeros
       const long long row = base + g + r * groups;
@@ -847,26 +652,21 @@ norm_backward_narrow_kernel(NormBackwardArgs a) {
         mx = fma2(md, xhat, mx);
         if (kCentered) m = add2(m, md);
       }
-      s_mx[r] = f2_lo(mx) + f2_hi(mx);
-      s_m[r] = f2_lo(m) + f2_hi(m);
+      v[2 * r] = f2_lo(mx) + f2_hi(mx);
+      v[2 * r + 1] = f2_lo(m) + f2_hi(m);
     }
-    for (int o = group >> 1; o > 0; o >>= 1) {
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        s_mx[r] += __shfl_xor_sync(0xffffffffu, s_mx[r], o);
-        if (kCentered) s_m[r] += __shfl_xor_sync(0xffffffffu, s_m[r], o);
-      }
-    }
+    const float sums = norm_lane_four_sums(v, group) * -inv;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       const long long row = base + g + r * groups;
+      const F2 minus_c = both(norm_of_four(sums, 2 * r, a.log2_group));
+      const F2 minus_m = both(kCentered ? norm_of_four(sums, 2 * r + 1, a.log2_group) : 0.f);
       uint4 out;
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
         F2 m = mul2(dy_of(r, i), gain[i]);
-        if (kCentered) m = add2(m, both(-s_m[r] * inv));
-        Pairs<T>::set(reinterpret_cast<uint32_t*>(&out) + i * Pairs<T>::kWords,
-                      mul2(fma2(xhat_of(r, i), both(-s_mx[r] * inv), m), both(rstd[r])));
+        if (kCentered) m = add2(m, minus_m);
+        Pairs<T>::set(reinterpret_cast<uint32_t*>(&out) + i * Pairs<T>::kWords, mul2(fma2(xhat_of(r, i), minus_c, m), both(rstd[r])));
       }
       if (column && row < a.n_rows) reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + row * a.hidden)[t] = out;
     }
@@ -894,6 +694,221 @@ norm_backward_narrow_kernel(NormBackwardArgs a) {
       for (int i = 0; i < kPairs; ++i) {
         out[2 * i] = f2_lo(acc[i]);
         out[2 * i + 1] = f2_hi(acc[i]);
+      }
+    }
+  };
+  if (a.dw_partial != nullptr) leave(dw, a.dw_partial);
+  if constexpr (kCentered) {
+    if (a.db_partial != nullptr) leave(db, a.db_partial);
+  }
+}
+
+// ---- rows that do not start on 16-byte boundaries or do not hold whole vectors: element by element
+//
+// Neighbouring lanes take neighbouring elements, so a warp still moves whole sectors; what counts is that enough of the narrow
+// loads are under way.  Columns are fixed per thread here too, several rows share a barrier, and the next rows are
+// loaded into registers while the current ones are reduced.  Groups of 4 to 512 threads.
+constexpr int kScalarThreads = 512;
+template <int kEpt, bool kGrad>
+struct Scalar {
+  static constexpr int kRows = kEpt >= 16 ? 1 : (kGrad ? 2 : 4);
+  static constexpr int kBlocksPerSm = kEpt >= 16 ? 1 : 2;
+};
+
+template <typename T, typename W, bool kCentered, int kEpt>
+__global__ void __launch_bounds__(kScalarThreads, (Scalar<kEpt, false>::kBlocksPerSm))
+norm_forward_scalar_kernel(NormForwardArgs a) {
+  constexpr int kRows = Scalar<kEpt, false>::kRows;
+  __shared__ float scratch[2][kNormMaxWarps * 4];
+  const int group = 1 << a.log2_group;
+  const int groups = kScalarThreads >> a.log2_group;
+  const int g = static_cast<int>(threadIdx.x) >> a.log2_group;
+  const int t = static_cast<int>(threadIdx.x) & (group - 1);
+  const int first = kEpt == 1 ? t : (t >> 5) * 32 * kEpt + (t & 31);
+  const long long step = static_cast<long long>(gridDim.x) * groups * kRows;
+  const bool rounded = !kCentered && a.round_xhat != 0;
+  const float inv = 1.f / static_cast<float>(a.hidden);
+  float gain[kEpt], bias[kCentered ? kEpt : 1];
+#pragma unroll
+  for (int e = 0; e < kEpt; ++e) {
+    const bool in = first + 32 * e < a.hidden;
+    gain[e] = in && a.w != nullptr ? a.offset + CeElem<W>::load(static_cast<const W*>(a.w) + first + 32 * e) : 1.f;
+    if (kCentered) bias[e] = in && a.b != nullptr ? CeElem<W>::load(static_cast<const W*>(a.b) + first + 32 * e) : 0.f;
+  }
+  T next[kRows][kEpt];
+  auto fetch = [&](long long base) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const bool live = base + r < a.n_rows;
+      const T* x = static_cast<const T*>(a.x) + (live ? base + r : 0) * a.ld_x + first;
+#pragma unroll
+      for (int e = 0; e < kEpt; ++e) {
+        CeElem<T>::store(&next[r][e], 0.f);
+        if (live && first + 32 * e < a.hidden) next[r][e] = x[32 * e];
+      }
+    }
+  };
+  // the same number of rounds in every thread of the block: groups of less than a warp share its shuffles
+  long long round = static_cast<long long>(blockIdx.x) * groups * kRows;
+  const int mine = g * kRows;
+  fetch(round + mine);
+  int phase = 0;
+  for (; round < a.n_rows; round += step) {
+    const long long row = round + mine;
+    float x[kRows][kEpt], v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+      for (int e = 0; e < kEpt; ++e) x[r][e] = CeElem<T>::load(&next[r][e]);
+    }
+    fetch(row + step);
+    float mean = 0.f;                       // of the row that this lane's sum belongs to
+    if constexpr (kCentered) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+        for (int e = 0; e < kEpt; ++e) v[r] += x[r][e];
+      }
+      mean = norm_group_four_sums(v, a.log2_group, scratch, phase) * inv;
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const float m = kCentered ? norm_of_four(mean, r, a.log2_group) : 0.f;
+      v[r] = 0.f;
+#pragma unroll
+      for (int e = 0; e < kEpt; ++e) {
+        if (kCentered) x[r][e] = first + 32 * e < a.hidden ? x[r][e] - m : 0.f;
+        v[r] = fmaf(x[r][e], x[r][e], v[r]);
+      }
+    }
+    const float rstd = norm_rsqrt(fmaf(norm_group_four_sums(v, a.log2_group, scratch, phase), inv, a.eps));
+    {
+      const int quarter = a.log2_group < 5 ? group >> 2 : 8;
+      const int r = t / quarter;
+      if (t % quarter == 0 && r < kRows && row + r < a.n_rows) {
+        if (kCentered && a.mean != nullptr) a.mean[row + r] = mean;
+        if (a.rstd != nullptr) a.rstd[row + r] = rstd;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const float scale = norm_of_four(rstd, r, a.log2_group);
+      if (row + r >= a.n_rows) continue;
+      T* y = static_cast<T*>(a.y) + (row + r) * a.hidden + first;
+#pragma unroll
+      for (int e = 0; e < kEpt; ++e) {
+        float o = x[r][e] * scale;
+        if (rounded) o = norm_round<T>(o);
+        o = kCentered ? fmaf(o, gain[e], bias[e]) : o * gain[e];
+        if (first + 32 * e < a.hidden) CeElem<T>::store(y + 32 * e, o);
+      }
+    }
+  }
+}
+
+template <typename T, typename W, bool kCentered, int kEpt>
+__global__ void __launch_bounds__(kScalarThreads, (Scalar<kEpt, true>::kBlocksPerSm))
+norm_backward_scalar_kernel(NormBackwardArgs a) {
+  constexpr int kRows = Scalar<kEpt, true>::kRows;
+  __shared__ float scratch[2][kNormMaxWarps * 4];
+  __shared__ float fold[kScalarThreads / 2 * kEpt];
+  const int group = 1 << a.log2_group;
+  const int groups = kScalarThreads >> a.log2_group;
+  const int g = static_cast<int>(threadIdx.x) >> a.log2_group;
+  const int t = static_cast<int>(threadIdx.x) & (group - 1);
+  const int first = kEpt == 1 ? t : (t >> 5) * 32 * kEpt + (t & 31);
+  const long long step = static_cast<long long>(gridDim.x) * groups * kRows;
+  const bool rounded = !kCentered && a.round_xhat != 0;
+  const float inv = 1.f / static_cast<float>(a.hidden);
+  float gain[kEpt], dw[kEpt], db[kCentered ? kEpt : 1];
+#pragma unroll
+  for (int e = 0; e < kEpt; ++e) {
+    gain[e] = first + 32 * e < a.hidden && a.w != nullptr ? a.offset + CeElem<W>::load(static_cast<const W*>(a.w) + first + 32 * e) : 1.f;
+    dw[e] = 0.f;
+    if (kCentered) db[e] = 0.f;
+  }
+  T next_x[kRows][kEpt], next_dy[kRows][kEpt];
+  float next_mean[kRows], next_rstd[kRows];
+  auto fetch = [&](long long base) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const bool live = base + r < a.n_rows;
+      const T* x = static_cast<const T*>(a.x) + (live ? base + r : 0) * a.ld_x + first;
+      const T* dy = static_cast<const T*>(a.dy) + (live ? base + r : 0) * a.ld_dy + first;
+#pragma unroll
+      for (int e = 0; e < kEpt; ++e) {
+        CeElem<T>::store(&next_x[r][e], 0.f);
+        CeElem<T>::store(&next_dy[r][e], 0.f);
+        if (live && first + 32 * e < a.hidden) {
+          next_x[r][e] = x[32 * e];
+          next_dy[r][e] = dy[32 * e];
+        }
+      }
+      next_mean[r] = kCentered && live ? __ldg(a.mean + base + r) : 0.f;
+      next_rstd[r] = live ? __ldg(a.rstd + base + r) : 0.f;
+    }
+  };
+  long long round = static_cast<long long>(blockIdx.x) * groups * kRows;
+  const int mine = g * kRows;
+  fetch(round + mine);
+  int phase = 0;
+  for (; round < a.n_rows; round += step) {
+    const long long row = round + mine;
+    float xhat[kRows][kEpt], m[kRows][kEpt], rstd[kRows], v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      rstd[r] = next_rstd[r];
+#pragma unroll
+      for (int e = 0; e < kEpt; ++e) {
+        xhat[r][e] = (CeElem<T>::load(&next_x[r][e]) - next_mean[r]) * rstd[r];
+        m[r][e] = CeElem<T>::load(&next_dy[r][e]);
+      }
+    }
+    fetch(row + step);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+      for (int e = 0; e < kEpt; ++e) {
+        // behind the row's end dy is zero, which keeps xhat out of every sum
+        dw[e] = fmaf(m[r][e], rounded ? norm_round<T>(xhat[r][e]) : xhat[r][e], dw[e]);
+        if (kCentered) db[e] += m[r][e];
+        m[r][e] *= gain[e];
+        v[2 * r] = fmaf(m[r][e], xhat[r][e], v[2 * r]);
+        if (kCentered) v[2 * r + 1] += m[r][e];
+      }
+    }
+    const float sums = norm_group_four_sums(v, a.log2_group, scratch, phase) * inv;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const float c = norm_of_four(sums, 2 * r, a.log2_group);
+      const float mm = kCentered ? norm_of_four(sums, 2 * r + 1, a.log2_group) : 0.f;
+      if (row + r >= a.n_rows) continue;
+      T* dx = static_cast<T*>(a.dx) + (row + r) * a.hidden + first;
+#pragma unroll
+      for (int e = 0; e < kEpt; ++e) {
+        if (first + 32 * e < a.hidden) CeElem<T>::store(dx + 32 * e, rstd[r] * (fmaf(-xhat[r][e], c, m[r][e]) - mm));
+      }
+    }
+  }
+  // the groups of the block, folded in halves in a fixed order
+  auto leave = [&](float (&acc)[kEpt], float* partial) {
+    for (int half = groups >> 1; half > 0; half >>= 1) {
+      __syncthreads();
+      if (g >= half && g < 2 * half) {
+#pragma unroll
+        for (int e = 0; e < kEpt; ++e) fold[((g - half) * kEpt + e) * group + t] = acc[e];
+      }
+      __syncthreads();
+      if (g < half) {
+#pragma unroll
+        for (int e = 0; e < kEpt; ++e) acc[e] += fold[(g * kEpt + e) * group + t];
+      }
+    }
+    if (g == 0) {
+      float* out = partial + static_cast<size_t>(blockIdx.x) * a.hidden + first;
+#pragma unroll
+      for (int e = 0; e < kEpt; ++e) {
+        if (first + 32 * e < a.hidden) out[32 * e] = acc[e];
       }
     }
   };
@@ -931,15 +946,18 @@ norm_parameter_gradient_kernel(const float* dw_partial, const float* db_partial,
 
 // ---- rows longer than the registers of a block hold: one block per row, read again for every pass (from L2)
 
-template <int kN>
-__device__ __forceinline__ void norm_block_sum(float (&v)[kN], float (*scratch)[kNormMaxWarps * kN], int& phase) {
-  norm_group_sum<kN>(v, 9, scratch, phase);
+// two sums over the block, to all its threads
+__device__ __forceinline__ void norm_block_sum(float& s0, float& s1, float (*scratch)[kNormMaxWarps * 4], int& phase) {
+  const float v[4] = {s0, s1, 0.f, 0.f};
+  const float sums = norm_group_four_sums(v, 9, scratch, phase);
+  s0 = norm_of_four(sums, 0, 9);
+  s1 = norm_of_four(sums, 1, 9);
 }
 
 template <typename T, typename W, bool kCentered>
 __global__ void __launch_bounds__(kNormMaxThreads)
 norm_forward_long_kernel(NormForwardArgs a) {
-  __shared__ float scratch[2][kNormMaxWarps];
+  __shared__ float scratch[2][kNormMaxWarps * 4];
   const long long row = blockIdx.x;
   const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
   const W* w = static_cast<const W*>(a.w);
@@ -947,10 +965,10 @@ norm_forward_long_kernel(NormForwardArgs a) {
   const int tid = static_cast<int>(threadIdx.x);
   int phase = 0;
   float mean = 0.f;
-  float s[1] = {0.f};
+  float s[2] = {0.f, 0.f};
   if constexpr (kCentered) {
     for (int c = tid; c < a.hidden; c += kNormMaxThreads) s[0] += CeElem<T>::load(x + c);
-    norm_block_sum<1>(s, scratch, phase);
+    norm_block_sum(s[0], s[1], scratch, phase);
     mean = s[0] / static_cast<float>(a.hidden);
     s[0] = 0.f;
   }
@@ -958,8 +976,8 @@ norm_forward_long_kernel(NormForwardArgs a) {
     const float v = CeElem<T>::load(x + c) - mean;
     s[0] = fmaf(v, v, s[0]);
   }
-  norm_block_sum<1>(s, scratch, phase);
-  const float rstd = 1.f / sqrtf(s[0] / static_cast<float>(a.hidden) + a.eps);
+  norm_block_sum(s[0], s[1], scratch, phase);
+  const float rstd = norm_rsqrt(s[0] / static_cast<float>(a.hidden) + a.eps);
   if (tid == 0) {
     if (kCentered && a.mean != nullptr) a.mean[row] = mean;
     if (a.rstd != nullptr) a.rstd[row] = rstd;
@@ -978,7 +996,7 @@ norm_forward_long_kernel(NormForwardArgs a) {
 template <typename T, typename W, bool kCentered>
 __global__ void __launch_bounds__(kNormMaxThreads)
 norm_backward_long_kernel(NormBackwardArgs a) {
-  __shared__ float scratch[2][kNormMaxWarps * 2];
+  __shared__ float scratch[2][kNormMaxWarps * 4];
   const long long row = blockIdx.x;
   const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
   const T* dy = static_cast<const T*>(a.dy) + row * a.ld_dy;
@@ -991,7 +1009,7 @@ norm_backward_long_kernel(NormBackwardArgs a) {
     s[0] = fmaf(m, (CeElem<T>::load(x + c) - mean) * rstd, s[0]);
     s[1] += m;
   }
-  norm_block_sum<2>(s, scratch, phase);
+  norm_block_sum(s[0], s[1], scratch, phase);
   const float c2 = s[0] / static_cast<float>(a.hidden);
   const float c1 = kCentered ? s[1] / static_cast<float>(a.hidden) : 0.f;
   T* dx = static_cast<T*>(a.dx) + row * a.hidden;
@@ -1003,7 +1021,7 @@ norm_backward_long_kernel(NormBackwardArgs a) {
 
 // partial sums of the parameters' gradients for such rows: one thread per column, blockIdx.y = a share of the rows
 template <typename T, bool kCentered>
-__global__ void __launch_bounds__(kNormForwardThreads)
+__global__ void __launch_bounds__(kNormColumnThreads)
 norm_parameter_partial_long_kernel(NormBackwardArgs a) {
   const int c = static_cast<int>(blockIdx.x * blockDim.x + threadIdx.x);
   if (c >= a.hidden) return;

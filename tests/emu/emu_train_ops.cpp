@@ -21,6 +21,7 @@ inline unsigned __ballot_sync(unsigned, bool v) {
   return bits;
 }
 inline bool __any_sync(unsigned m, bool v) { return __ballot_sync(m, v) != 0; }
+inline float rsqrtf(float v) { return 1.f / std::sqrt(v); }
 inline int __popc(unsigned v) { return __builtin_popcount(v); }
 inline int __clz(unsigned v) { return v ? __builtin_clz(v) : 32; }
 
