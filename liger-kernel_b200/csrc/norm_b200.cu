@@ -27,12 +27,12 @@ int check_norm(const flce_norm_t* p) {
   return FLCE_OK;
 }
 
-// How the rows are spread over threads: `share` elements (scalar) or 16-byte vectors (otherwise) per thread, 1 << log2_group
-// threads to a row.
-enum NormPath { kNormStream, kNormNarrow, kNormScalar, kNormLong };
+// How the rows are spread over threads: `share` elements (window) or 16-byte vectors (stream) per thread; the threads of a row
+// as a power of two (narrow, stream, tiny) or as whole warps (stream, window).
+enum NormPath { kNormStream, kNormNarrow, kNormWindow, kNormTiny, kNormLong };
 struct NormPlan {
   NormPath path;
-  int share, log2_group;
+  int share, log2_group, warps;
 };
 
 int log2_group_for(long long pieces, int smallest) {
@@ -42,39 +42,56 @@ int log2_group_for(long long pieces, int smallest) {
 }
 
 // Narrow: a lane per vector, rows of up to 32 of them.  Stream: two vectors per thread if a block's 512 threads reach so, else four.
-// Scalar: one element per thread up to 32, then 4 or 16 strides of a warp.  Long: what is left, above 8192 elements.
+// Window: of 2, 4, 8 and 16 elements per lane the choice that leaves the fewest of the block's lanes without a column, the most
+// elements among equals (fewer warps to a row wait for each other).  Long: what is left, above 8192 elements.
 NormPlan norm_plan(const flce_norm_t* p, bool vectors) {
   const long long n = p->hidden * element_size(p->dtype) / 16;
-  if (vectors && n <= 32) return {kNormNarrow, 1, log2_group_for(n, 2)};
+  if (vectors && n <= 32) return {kNormNarrow, 1, log2_group_for(n, 2), 0};
   if (vectors && n <= 4 * kStreamThreads) {
     const int share = n <= 2 * kStreamThreads ? 2 : 4;
-    return {kNormStream, share, log2_group_for(ceil_div(n, share), 5)};
+    const int log2_group = log2_group_for(ceil_div(n, share), 5);
+    return {kNormStream, share, log2_group, 1 << (log2_group - 5)};
   }
-  if (p->hidden <= 32) return {kNormScalar, 1, log2_group_for(p->hidden, 2)};
-  if (p->hidden <= 16 * kScalarThreads) {
-    const int share = p->hidden <= 4 * kScalarThreads ? 4 : 16;
-    return {kNormScalar, share, log2_group_for(ceil_div(p->hidden, share), 5)};
+  if (p->hidden <= 32) return {kNormTiny, 1, log2_group_for(p->hidden, 2), 0};
+  NormPlan best{kNormLong, 0, 9, kNormMaxWarps};
+  double used = 0.0;
+  for (int share = 2; share <= 16; share *= 2) {
+    const long long warps = ceil_div(p->hidden, 32 * share);
+    if (warps > kWindowWarps) continue;
+    const double lanes = static_cast<double>(kWindowWarps / warps) * p->hidden / (32.0 * share * kWindowWarps);
+    if (lanes >= used) {
+      used = lanes;
+      best = {kNormWindow, share, 0, static_cast<int>(warps)};
+    }
   }
-  return {kNormLong, 0, 9};
+  return best;
+}
+
+// fn(std::integral_constant<int, elements per lane>) for a window plan
+template <class Fn>
+int with_share(int share, Fn fn) {
+  switch (share) {
+    case 2: return fn(std::integral_constant<int, 2>());
+    case 4: return fn(std::integral_constant<int, 4>());
+    case 8: return fn(std::integral_constant<int, 8>());
+    default: return fn(std::integral_constant<int, 16>());
+  }
 }
 
 // rows that a block takes per round, and blocks that are resident on an SM
 template <bool kGrad>
 int rows_per_round(const NormPlan& plan) {
   switch (plan.path) {
-    case kNormNarrow: return (kNarrowThreads >> plan.log2_group) * (kGrad ? kNarrowBackwardRows : kNarrowForwardRows);
+    case kNormNarrow:
+    case kNormTiny: return (kNarrowThreads >> plan.log2_group) * (kGrad ? kNarrowBackwardRows : kNarrowForwardRows);
     case kNormStream: return (kStreamThreads >> plan.log2_group) * (plan.share == 2 ? Stream<2, kGrad>::kRows : Stream<4, kGrad>::kRows);
-    case kNormScalar: return (kScalarThreads >> plan.log2_group) * (plan.share < 16 ? Scalar<4, kGrad>::kRows : Scalar<16, kGrad>::kRows);
+    case kNormWindow:
+      return kWindowWarps / plan.warps * with_share(plan.share, [](auto e) { return Window<float, decltype(e)::value, kGrad>::kRows; });
     default: return 1;
   }
 }
 int blocks_per_sm(const NormPlan& plan) {
-  switch (plan.path) {
-    case kNormNarrow: return 4;
-    case kNormStream: return 1;
-    case kNormScalar: return plan.share < 16 ? Scalar<4, true>::kBlocksPerSm : Scalar<16, true>::kBlocksPerSm;
-    default: return 2;
-  }
+  return plan.path == kNormStream || plan.path == kNormWindow ? 1 : (plan.path == kNormLong ? 2 : 4);
 }
 
 // Blocks that walk over the rows: as many as are resident together.  Those of the backward kernel leave `hidden` partial sums
@@ -116,11 +133,17 @@ int run_forward(const NormForwardArgs& a, const NormPlan& plan, unsigned walking
       FLCE_LAUNCH((norm_forward_narrow_kernel<T, W, kCentered>), all, kNarrowThreads, stream, a);
       return FLCE_OK;
     }
-    case kNormScalar:
-      if (plan.share == 1) FLCE_LAUNCH((norm_forward_scalar_kernel<T, W, kCentered, 1>), grid, kScalarThreads, stream, a);
-      else if (plan.share == 4) FLCE_LAUNCH((norm_forward_scalar_kernel<T, W, kCentered, 4>), grid, kScalarThreads, stream, a);
-      else FLCE_LAUNCH((norm_forward_scalar_kernel<T, W, kCentered, 16>), grid, kScalarThreads, stream, a);
+    case kNormTiny: {
+      const unsigned all = static_cast<unsigned>(ceil_div(a.n_rows, rows_per_round<false>(plan)));
+      FLCE_LAUNCH((norm_forward_tiny_kernel<T, W, kCentered>), all, kNarrowThreads, stream, a);
       return FLCE_OK;
+    }
+    case kNormWindow:
+      return with_share(plan.share, [&](auto e) {
+        constexpr int kEpt = decltype(e)::value;
+        return launch_with_shared<norm_forward_window_kernel<T, W, kCentered, kEpt>>(grid, kWindowThreads, Window<T, kEpt, false>::kRingBytes,
+                                                                                    stream, a);
+      });
     default:
       FLCE_LAUNCH((norm_forward_long_kernel<T, W, kCentered>), static_cast<unsigned>(a.n_rows), kNormMaxThreads, stream, a);
       return FLCE_OK;
@@ -138,11 +161,15 @@ int run_backward(const NormBackwardArgs& a, const NormPlan& plan, unsigned walki
     case kNormNarrow:
       FLCE_LAUNCH((norm_backward_narrow_kernel<T, W, kCentered>), grid, kNarrowThreads, stream, a);
       return FLCE_OK;
-    case kNormScalar:
-      if (plan.share == 1) FLCE_LAUNCH((norm_backward_scalar_kernel<T, W, kCentered, 1>), grid, kScalarThreads, stream, a);
-      else if (plan.share == 4) FLCE_LAUNCH((norm_backward_scalar_kernel<T, W, kCentered, 4>), grid, kScalarThreads, stream, a);
-      else FLCE_LAUNCH((norm_backward_scalar_kernel<T, W, kCentered, 16>), grid, kScalarThreads, stream, a);
+    case kNormTiny:
+      FLCE_LAUNCH((norm_backward_tiny_kernel<T, W, kCentered>), grid, kNarrowThreads, stream, a);
       return FLCE_OK;
+    case kNormWindow:
+      return with_share(plan.share, [&](auto e) {
+        constexpr int kEpt = decltype(e)::value;
+        return launch_with_shared<norm_backward_window_kernel<T, W, kCentered, kEpt>>(grid, kWindowThreads, Window<T, kEpt, true>::kRingBytes,
+                                                                                     stream, a);
+      });
     default:
       FLCE_LAUNCH((norm_backward_long_kernel<T, W, kCentered>), static_cast<unsigned>(a.n_rows), kNormMaxThreads, stream, a);
       if (a.dw_partial != nullptr || a.db_partial != nullptr) {
@@ -184,6 +211,7 @@ int flce_b200_norm_forward(const flce_norm_t* p, void* y, float* mean, float* rs
   a.round_xhat = p->round_xhat;
   const NormPlan plan = norm_plan(p, whole_vectors(p, y, p->hidden));
   a.log2_group = plan.log2_group;
+  a.group_warps = plan.warps;
   const unsigned walking = static_cast<unsigned>(walking_blocks<false>(p, plan, sms));
   with_types(p, [&](auto t, auto w) {
     using T = decltype(t);
@@ -253,6 +281,7 @@ int flce_b200_norm_backward(const flce_norm_t* p, const void* grad_y, int64_t ld
   a.offset = p->offset;
   a.round_xhat = p->round_xhat;
   a.log2_group = plan.log2_group;
+  a.group_warps = plan.warps;
   const unsigned walking = static_cast<unsigned>(blocks);
   with_types(p, [&](auto t, auto w) {
     using T = decltype(t);

@@ -16,8 +16,8 @@
 // registers; blocks leave one partial sum per column, added up in block order by a second kernel: no atomics, the same
 // bits in every run.
 //
-// Four forms: rows of aligned 16-byte vectors, streamed (wide) or in registers (narrow), rows without that alignment (scalar), and
-// rows longer than a block's threads hold (long).
+// Five forms: rows of aligned 16-byte vectors, streamed (wide) or in registers (narrow); rows without that alignment, through
+// windows (wide) or element by element (tiny); and rows longer than a block's threads hold (long).
 #pragma once
 
 #include <type_traits>
@@ -44,7 +44,8 @@ struct NormForwardArgs {
   int hidden;
   float eps, offset;
   int round_xhat;      // xhat is rounded to the rows' type before it meets the weight ("llama" casting)
-  int log2_group;
+  int log2_group;      // threads that share a row
+  int group_warps;     // the same in warps, where they need not be a power of two
 };
 
 struct NormBackwardArgs {
@@ -63,6 +64,7 @@ struct NormBackwardArgs {
   float offset;
   int round_xhat;
   int log2_group;
+  int group_warps;
 };
 
 template <typename T>
@@ -96,23 +98,26 @@ __device__ __forceinline__ float norm_lane_four_sums(const float (&v)[4], int la
   return norm_low_lane_sum(__shfl_xor_sync(0xffffffffu, right ? a0 : a1, quarter) + (right ? a1 : a0), quarter);
 }
 
-// Over a group of 1 << log2_group threads, 4 or more.  Warps meet in one of two buffers taken in turn: a thread writes a buffer
+// Over the `warps` whole warps of group g.  Warps meet in one of two buffers taken in turn: a thread writes a buffer
 // again only behind the barrier of the call in between, which the readers of the older sums reach after reading them, so
 // one barrier per call is enough.
-__device__ __forceinline__ float norm_group_four_sums(const float (&v)[4], int log2_group, float (*scratch)[kNormMaxWarps * 4], int& phase) {
-  float sum = norm_lane_four_sums(v, log2_group < 5 ? 1 << log2_group : 32);
-  if (log2_group <= 5) return sum;
-  const int lane = static_cast<int>(threadIdx.x) & 31, warps = 1 << (log2_group - 5), g = static_cast<int>(threadIdx.x) >> log2_group;
+__device__ __forceinline__ float norm_warps_four_sums(const float (&v)[4], int warps, int g, float (*scratch)[kNormMaxWarps * 4], int& phase) {
+  float sum = norm_lane_four_sums(v, 32);
+  if (warps == 1) return sum;
+  const int lane = static_cast<int>(threadIdx.x) & 31;
   float* buf = scratch[phase];
   phase ^= 1;
   if ((lane & 7) == 0) buf[(threadIdx.x >> 5) * 4 + (lane >> 3)] = sum;
-  named_barrier(1 + g, 1 << log2_group);
+  named_barrier(1 + g, warps * 32);
   const float* of = buf + g * warps * 4 + (lane >> 3);
   sum = 0.f;
   for (int w = lane & 7; w < warps; w += 8) sum += of[w * 4];
   return norm_low_lane_sum(sum, 8);
 }
-// sum number i of those, from a lane that holds it
+// sum number i of those, from a lane of the warp that holds it
+__device__ __forceinline__ float norm_warp_of_four(float sums, int i) { return __shfl_sync(0xffffffffu, sums, i * 8); }
+
+// the same from a lane of a group of 1 << log2_group lanes
 __device__ __forceinline__ float norm_of_four(float sums, int i, int log2_group) {
   const int lanes = log2_group < 5 ? 1 << log2_group : 32;
   return __shfl_sync(0xffffffffu, sums, (static_cast<int>(threadIdx.x) & 31 & ~(lanes - 1)) | i * (lanes >> 2));
@@ -191,7 +196,7 @@ norm_forward_stream_kernel(NormForwardArgs a) {
       const bool live = base + r < a.n_rows;
       const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (live ? base + r : 0) * a.ld_x) + first;
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) async_copy16(&cell(slot, r, u), x + u * 32, live && first + u * 32 < vectors);
+      for (int u = 0; u < kUnits; ++u) async_copy16(&cell(slot, r, u), x + u * 32, live && first + u * 32 < vectors ? 16 : 0);
     }
     async_commit();
   };
@@ -249,7 +254,7 @@ norm_forward_stream_kernel(NormForwardArgs a) {
     float mean = part_sum * part_inv;       // of row lane >> 3, once the parts have met
     if (warps > 1) {
       float *buf = scratch[phase], *buf_sums = scratch_sums[kCentered ? phase : 0];
-      phase ^= 1;                           // taken in turn: see norm_group_four_sums
+      phase ^= 1;                           // taken in turn: see norm_warps_four_sums
       if ((lane & 7) == 0) {
         buf[(threadIdx.x >> 5) * 4 + (lane >> 3)] = square;
         if (kCentered) buf_sums[(threadIdx.x >> 5) * 4 + (lane >> 3)] = part_sum;
@@ -362,8 +367,8 @@ norm_backward_stream_kernel(NormBackwardArgs a) {
       const uint4* dy = reinterpret_cast<const uint4*>(static_cast<const T*>(a.dy) + (live ? row : 0) * a.ld_dy) + first;
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
-        async_copy16(&cell(slot, r, 0, u), x + u * 32, live && first + u * 32 < vectors);
-        async_copy16(&cell(slot, r, 1, u), dy + u * 32, live && first + u * 32 < vectors);
+        async_copy16(&cell(slot, r, 0, u), x + u * 32, live && first + u * 32 < vectors ? 16 : 0);
+        async_copy16(&cell(slot, r, 1, u), dy + u * 32, live && first + u * 32 < vectors ? 16 : 0);
       }
     }
     async_commit();
@@ -422,7 +427,7 @@ norm_backward_stream_kernel(NormBackwardArgs a) {
       v[2 * r] = f2_lo(s_mx) + f2_hi(s_mx);
       if (kCentered) v[2 * r + 1] = f2_lo(s_m) + f2_hi(s_m);
     }
-    const float sum = norm_group_four_sums(v, a.log2_group, scratch, phase);
+    const float sum = norm_warps_four_sums(v, warps, g, scratch, phase);
     const float inv = 1.f / static_cast<float>(a.hidden);
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
@@ -703,219 +708,390 @@ norm_backward_narrow_kernel(NormBackwardArgs a) {
   }
 }
 
-// ---- rows that do not start on 16-byte boundaries or do not hold whole vectors: element by element
+// ---- rows that do not start on 16-byte boundaries or do not hold whole vectors
 //
-// Neighbouring lanes take neighbouring elements, so a warp still moves whole sectors; what counts is that enough of the narrow
-// loads are under way.  Columns are fixed per thread here too, several rows share a barrier, and the next rows are
-// loaded into registers while the current ones are reduced.  Groups of 4 to 512 threads.
-constexpr int kScalarThreads = 512;
-template <int kEpt, bool kGrad>
-struct Scalar {
-  static constexpr int kRows = kEpt >= 16 ? 1 : (kGrad ? 2 : 4);
-  static constexpr int kBlocksPerSm = kEpt >= 16 ? 1 : 2;
+// A warp fetches its part of a row as the aligned 16-byte pieces that hold it, with cp.async, into a window of its own in shared
+// memory, rounds ahead like the streaming kernels, and reads its elements from there at whatever shift the row has: lane by
+// lane neighbouring elements, which is free of bank conflicts.  (The first piece may begin up to 14 bytes before the row: in the
+// same 16-byte granule, which belongs to the same allocation.)  Results leave as neighbouring elements, whole sectors at a
+// time.  Direct element loads into registers, a round ahead, left too little under way: 10007 x 1537 fp16 35 us forward, 77 us
+// backward.  A part is 32 * kEpt columns, a row `warps` parts, as many rows side by side as the block's 16 warps hold.
+constexpr int kWindowThreads = 512;
+constexpr int kWindowWarps = kWindowThreads / 32;
+template <typename T, int kEpt, bool kGrad>
+struct Window {
+  static constexpr int kRows = (kEpt <= 8 ? 4 : 2) / (kGrad ? 2 : 1);
+  static constexpr int kPieces = 32 * kEpt * static_cast<int>(sizeof(T)) / 16 + 1;     // of one window
+  static constexpr int kRoundPieces = kRows * (kGrad ? 2 : 1) * kWindowWarps * kPieces;
+  static constexpr int kSlots = 6 * kRoundPieces * 16 <= 200 * 1024 ? 6 : (4 * kRoundPieces * 16 <= 200 * 1024 ? 4 : 2);
+  static constexpr int kFoldBytes = kWindowWarps * 32 * kEpt * 4;
+  static constexpr int kRingBytes = kSlots * kRoundPieces * 16 > kFoldBytes ? kSlots * kRoundPieces * 16 : kFoldBytes;
 };
 
+// the pieces of `count` elements from `src`, asked for by the lanes of a warp
+template <typename T, int kPieces>
+__device__ __forceinline__ void window_fetch(uint4* window, const T* src, int count, int lane) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(src);
+  const int end = static_cast<int>(at & 15) + count * static_cast<int>(sizeof(T));
+  const char* base = reinterpret_cast<const char*>(at & ~static_cast<uintptr_t>(15));
+#pragma unroll
+  for (int i = 0; i < kPieces; i += 32) {
+    const int piece = i + lane;
+    if (piece * 16 < end) async_copy16(window + piece, base + piece * 16, end - piece * 16 < 16 ? end - piece * 16 : 16);
+  }
+}
+// kEpt elements of this lane, in pairs, zeros behind the end
+template <typename T, int kEpt>
+__device__ __forceinline__ void window_read(const uint4* window, const T* src, int count, int lane, F2 (&v)[kEpt / 2]) {
+  const T* e = reinterpret_cast<const T*>(reinterpret_cast<const char*>(window) + (reinterpret_cast<uintptr_t>(src) & 15)) + lane;
+#pragma unroll
+  for (int i = 0; i < kEpt / 2; ++i)
+    v[i] = f2(lane + 64 * i < count ? CeElem<T>::load(e + 64 * i) : 0.f, lane + 64 * i + 32 < count ? CeElem<T>::load(e + 64 * i + 32) : 0.f);
+}
+
 template <typename T, typename W, bool kCentered, int kEpt>
-__global__ void __launch_bounds__(kScalarThreads, (Scalar<kEpt, false>::kBlocksPerSm))
-norm_forward_scalar_kernel(NormForwardArgs a) {
-  constexpr int kRows = Scalar<kEpt, false>::kRows;
+__global__ void __launch_bounds__(kWindowThreads, 1)
+norm_forward_window_kernel(NormForwardArgs a) {
+  typedef Window<T, kEpt, false> Shape;
+  constexpr int kRows = Shape::kRows, kSlots = Shape::kSlots, kPairs = kEpt / 2;
+  FLCE_DYNAMIC_SHARED(uint4, stream_ring);                    // [slot][row][warp][piece]
   __shared__ float scratch[2][kNormMaxWarps * 4];
-  const int group = 1 << a.log2_group;
-  const int groups = kScalarThreads >> a.log2_group;
-  const int g = static_cast<int>(threadIdx.x) >> a.log2_group;
-  const int t = static_cast<int>(threadIdx.x) & (group - 1);
-  const int first = kEpt == 1 ? t : (t >> 5) * 32 * kEpt + (t & 31);
+  const int warps = a.group_warps;
+  const int groups = kWindowWarps / warps;
+  const int lane = static_cast<int>(threadIdx.x) & 31, warp = static_cast<int>(threadIdx.x) >> 5;
+  const int g = warp / warps;
+  if (g >= groups) return;                                    // warps that make no whole group: there is no block-wide barrier
+  const int column = (warp - g * warps) * 32 * kEpt;
+  const int count = a.hidden - column < 32 * kEpt ? a.hidden - column : 32 * kEpt;      // of this warp's part
   const long long step = static_cast<long long>(gridDim.x) * groups * kRows;
   const bool rounded = !kCentered && a.round_xhat != 0;
   const float inv = 1.f / static_cast<float>(a.hidden);
-  float gain[kEpt], bias[kCentered ? kEpt : 1];
+  F2 gain[kPairs], bias[kCentered ? kPairs : 1];
+  {
+    float w[kEpt], b[kEpt];
 #pragma unroll
-  for (int e = 0; e < kEpt; ++e) {
-    const bool in = first + 32 * e < a.hidden;
-    gain[e] = in && a.w != nullptr ? a.offset + CeElem<W>::load(static_cast<const W*>(a.w) + first + 32 * e) : 1.f;
-    if (kCentered) bias[e] = in && a.b != nullptr ? CeElem<W>::load(static_cast<const W*>(a.b) + first + 32 * e) : 0.f;
+    for (int e = 0; e < kEpt; ++e) {
+      const bool in = lane + 32 * e < count;
+      w[e] = in && a.w != nullptr ? a.offset + CeElem<W>::load(static_cast<const W*>(a.w) + column + lane + 32 * e) : 1.f;
+      b[e] = in && a.b != nullptr ? CeElem<W>::load(static_cast<const W*>(a.b) + column + lane + 32 * e) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      gain[i] = f2(w[2 * i], w[2 * i + 1]);
+      if (kCentered) bias[i] = f2(b[2 * i], b[2 * i + 1]);
+    }
   }
-  T next[kRows][kEpt];
-  auto fetch = [&](long long base) {
+  auto window = [&](int slot, int r) { return stream_ring + ((slot * kRows + r) * kWindowWarps + warp) * Shape::kPieces; };
+  auto source = [&](long long row) { return static_cast<const T*>(a.x) + row * a.ld_x + column; };
+  auto fetch = [&](long long base, int slot) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const bool live = base + r < a.n_rows;
-      const T* x = static_cast<const T*>(a.x) + (live ? base + r : 0) * a.ld_x + first;
-#pragma unroll
-      for (int e = 0; e < kEpt; ++e) {
-        CeElem<T>::store(&next[r][e], 0.f);
-        if (live && first + 32 * e < a.hidden) next[r][e] = x[32 * e];
-      }
+      if (base + r < a.n_rows) window_fetch<T, Shape::kPieces>(window(slot, r), source(base + r), count, lane);
     }
+    async_commit();
   };
-  // the same number of rounds in every thread of the block: groups of less than a warp share its shuffles
-  long long round = static_cast<long long>(blockIdx.x) * groups * kRows;
-  const int mine = g * kRows;
-  fetch(round + mine);
-  int phase = 0;
-  for (; round < a.n_rows; round += step) {
-    const long long row = round + mine;
-    float x[kRows][kEpt], v[4] = {0.f, 0.f, 0.f, 0.f};
+  long long row = (static_cast<long long>(blockIdx.x) * groups + g) * kRows;
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
+  for (int s = 0; s < kSlots - 1; ++s) fetch(row + s * step, s);
+  int slot = 0, phase = 0;
+  for (; row < a.n_rows; row += step) {
+    // into the slot of the round before this one: all lanes have read it, they have exchanged sums since
+    fetch(row + (kSlots - 1) * step, slot == 0 ? kSlots - 1 : slot - 1);
+    async_wait<kSlots - 1>();
+    warp_sync();
+    F2 x[kRows][kPairs];
+    float v[4] = {0.f, 0.f, 0.f, 0.f}, mean = 0.f;            // mean of row lane >> 3
 #pragma unroll
-      for (int e = 0; e < kEpt; ++e) x[r][e] = CeElem<T>::load(&next[r][e]);
-    }
-    fetch(row + step);
-    float mean = 0.f;                       // of the row that this lane's sum belongs to
+    for (int r = 0; r < kRows; ++r)
+      window_read<T, kEpt>(window(slot, r), source(row + r), row + r < a.n_rows ? count : 0, lane, x[r]);
     if constexpr (kCentered) {
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
+        F2 acc = x[r][0];
 #pragma unroll
-        for (int e = 0; e < kEpt; ++e) v[r] += x[r][e];
+        for (int i = 1; i < kPairs; ++i) acc = add2(acc, x[r][i]);
+        v[r] = f2_lo(acc) + f2_hi(acc);
       }
-      mean = norm_group_four_sums(v, a.log2_group, scratch, phase) * inv;
+      mean = norm_warps_four_sums(v, warps, g, scratch, phase) * inv;
     }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const float m = kCentered ? norm_of_four(mean, r, a.log2_group) : 0.f;
-      v[r] = 0.f;
+      if constexpr (kCentered) {
+        const F2 minus_mean = both(-norm_warp_of_four(mean, r));
 #pragma unroll
-      for (int e = 0; e < kEpt; ++e) {
-        if (kCentered) x[r][e] = first + 32 * e < a.hidden ? x[r][e] - m : 0.f;
-        v[r] = fmaf(x[r][e], x[r][e], v[r]);
+        for (int i = 0; i < kPairs; ++i) {
+          x[r][i] = add2(x[r][i], minus_mean);
+          // the columns behind the end hold zeros still
+          if (lane + 64 * i + 32 >= count) x[r][i] = f2(lane + 64 * i < count ? f2_lo(x[r][i]) : 0.f, 0.f);
+        }
       }
+      F2 acc = both(0.f);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) acc = fma2(x[r][i], x[r][i], acc);
+      v[r] = f2_lo(acc) + f2_hi(acc);
     }
-    const float rstd = norm_rsqrt(fmaf(norm_group_four_sums(v, a.log2_group, scratch, phase), inv, a.eps));
+    const float rstd = norm_rsqrt(fmaf(norm_warps_four_sums(v, warps, g, scratch, phase), inv, a.eps));
     {
-      const int quarter = a.log2_group < 5 ? group >> 2 : 8;
-      const int r = t / quarter;
-      if (t % quarter == 0 && r < kRows && row + r < a.n_rows) {
+      const int r = lane >> 3;
+      if (column == 0 && (lane & 7) == 0 && r < kRows && row + r < a.n_rows) {
         if (kCentered && a.mean != nullptr) a.mean[row + r] = mean;
         if (a.rstd != nullptr) a.rstd[row + r] = rstd;
       }
     }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const float scale = norm_of_four(rstd, r, a.log2_group);
+      const F2 scale = both(norm_warp_of_four(rstd, r));
       if (row + r >= a.n_rows) continue;
-      T* y = static_cast<T*>(a.y) + (row + r) * a.hidden + first;
+      T* y = static_cast<T*>(a.y) + (row + r) * a.hidden + column + lane;
 #pragma unroll
-      for (int e = 0; e < kEpt; ++e) {
-        float o = x[r][e] * scale;
-        if (rounded) o = norm_round<T>(o);
-        o = kCentered ? fmaf(o, gain[e], bias[e]) : o * gain[e];
-        if (first + 32 * e < a.hidden) CeElem<T>::store(y + 32 * e, o);
+      for (int i = 0; i < kPairs; ++i) {
+        F2 o = mul2(x[r][i], scale);
+        if (rounded) o = f2(norm_round<T>(f2_lo(o)), norm_round<T>(f2_hi(o)));
+        if constexpr (kCentered) o = fma2(o, gain[i], bias[i]);
+        else o = mul2(o, gain[i]);
+        if (lane + 64 * i < count) CeElem<T>::store(y + 64 * i, f2_lo(o));
+        if (lane + 64 * i + 32 < count) CeElem<T>::store(y + 64 * i + 32, f2_hi(o));
       }
     }
+    slot = slot + 1 == kSlots ? 0 : slot + 1;
   }
+  async_wait<0>();
 }
 
 template <typename T, typename W, bool kCentered, int kEpt>
-__global__ void __launch_bounds__(kScalarThreads, (Scalar<kEpt, true>::kBlocksPerSm))
-norm_backward_scalar_kernel(NormBackwardArgs a) {
-  constexpr int kRows = Scalar<kEpt, true>::kRows;
+__global__ void __launch_bounds__(kWindowThreads, 1)
+norm_backward_window_kernel(NormBackwardArgs a) {
+  typedef Window<T, kEpt, true> Shape;
+  constexpr int kRows = Shape::kRows, kSlots = Shape::kSlots, kPairs = kEpt / 2;
+  FLCE_DYNAMIC_SHARED(uint4, stream_ring);                    // [slot][row][x, dy][warp][piece]; at the end: the groups' sums
   __shared__ float scratch[2][kNormMaxWarps * 4];
-  __shared__ float fold[kScalarThreads / 2 * kEpt];
-  const int group = 1 << a.log2_group;
-  const int groups = kScalarThreads >> a.log2_group;
-  const int g = static_cast<int>(threadIdx.x) >> a.log2_group;
-  const int t = static_cast<int>(threadIdx.x) & (group - 1);
-  const int first = kEpt == 1 ? t : (t >> 5) * 32 * kEpt + (t & 31);
+  const int warps = a.group_warps;
+  const int groups = kWindowWarps / warps;
+  const int lane = static_cast<int>(threadIdx.x) & 31, warp = static_cast<int>(threadIdx.x) >> 5;
+  const int g = warp / warps;
+  const int column = (warp - g * warps) * 32 * kEpt;
+  const int count = a.hidden - column < 32 * kEpt ? a.hidden - column : 32 * kEpt;
   const long long step = static_cast<long long>(gridDim.x) * groups * kRows;
   const bool rounded = !kCentered && a.round_xhat != 0;
   const float inv = 1.f / static_cast<float>(a.hidden);
-  float gain[kEpt], dw[kEpt], db[kCentered ? kEpt : 1];
+  F2 gain[kPairs], dw[kPairs], db[kCentered ? kPairs : 1];
 #pragma unroll
-  for (int e = 0; e < kEpt; ++e) {
-    gain[e] = first + 32 * e < a.hidden && a.w != nullptr ? a.offset + CeElem<W>::load(static_cast<const W*>(a.w) + first + 32 * e) : 1.f;
-    dw[e] = 0.f;
-    if (kCentered) db[e] = 0.f;
+  for (int i = 0; i < kPairs; ++i) {
+    float w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = lane + 64 * i + 32 * h;
+      w[h] = c < count && a.w != nullptr ? a.offset + CeElem<W>::load(static_cast<const W*>(a.w) + column + c) : 1.f;
+    }
+    gain[i] = f2(w[0], w[1]);
+    dw[i] = both(0.f);
+    if (kCentered) db[i] = both(0.f);
   }
-  T next_x[kRows][kEpt], next_dy[kRows][kEpt];
+  auto window = [&](int slot, int r, int which) {
+    return stream_ring + (((slot * kRows + r) * 2 + which) * kWindowWarps + warp) * Shape::kPieces;
+  };
+  auto source_x = [&](long long row) { return static_cast<const T*>(a.x) + row * a.ld_x + column; };
+  auto source_dy = [&](long long row) { return static_cast<const T*>(a.dy) + row * a.ld_dy + column; };
+  auto fetch = [&](long long base, int slot) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      if (base + r < a.n_rows) {
+        window_fetch<T, Shape::kPieces>(window(slot, r, 0), source_x(base + r), count, lane);
+        window_fetch<T, Shape::kPieces>(window(slot, r, 1), source_dy(base + r), count, lane);
+      }
+    }
+    async_commit();
+  };
   float next_mean[kRows], next_rstd[kRows];
-  auto fetch = [&](long long base) {
+  auto fetch_statistics = [&](long long base) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       const bool live = base + r < a.n_rows;
-      const T* x = static_cast<const T*>(a.x) + (live ? base + r : 0) * a.ld_x + first;
-      const T* dy = static_cast<const T*>(a.dy) + (live ? base + r : 0) * a.ld_dy + first;
-#pragma unroll
-      for (int e = 0; e < kEpt; ++e) {
-        CeElem<T>::store(&next_x[r][e], 0.f);
-        CeElem<T>::store(&next_dy[r][e], 0.f);
-        if (live && first + 32 * e < a.hidden) {
-          next_x[r][e] = x[32 * e];
-          next_dy[r][e] = dy[32 * e];
-        }
-      }
       next_mean[r] = kCentered && live ? __ldg(a.mean + base + r) : 0.f;
       next_rstd[r] = live ? __ldg(a.rstd + base + r) : 0.f;
     }
   };
-  long long round = static_cast<long long>(blockIdx.x) * groups * kRows;
-  const int mine = g * kRows;
-  fetch(round + mine);
-  int phase = 0;
-  for (; round < a.n_rows; round += step) {
-    const long long row = round + mine;
-    float xhat[kRows][kEpt], m[kRows][kEpt], rstd[kRows], v[4] = {0.f, 0.f, 0.f, 0.f};
+  long long row = g < groups ? (static_cast<long long>(blockIdx.x) * groups + g) * kRows : a.n_rows;
+  if (g < groups) {                                           // warps that make no whole group wait for the end
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      rstd[r] = next_rstd[r];
-#pragma unroll
-      for (int e = 0; e < kEpt; ++e) {
-        xhat[r][e] = (CeElem<T>::load(&next_x[r][e]) - next_mean[r]) * rstd[r];
-        m[r][e] = CeElem<T>::load(&next_dy[r][e]);
-      }
-    }
-    fetch(row + step);
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-#pragma unroll
-      for (int e = 0; e < kEpt; ++e) {
-        // behind the row's end dy is zero, which keeps xhat out of every sum
-        dw[e] = fmaf(m[r][e], rounded ? norm_round<T>(xhat[r][e]) : xhat[r][e], dw[e]);
-        if (kCentered) db[e] += m[r][e];
-        m[r][e] *= gain[e];
-        v[2 * r] = fmaf(m[r][e], xhat[r][e], v[2 * r]);
-        if (kCentered) v[2 * r + 1] += m[r][e];
-      }
-    }
-    const float sums = norm_group_four_sums(v, a.log2_group, scratch, phase) * inv;
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      const float c = norm_of_four(sums, 2 * r, a.log2_group);
-      const float mm = kCentered ? norm_of_four(sums, 2 * r + 1, a.log2_group) : 0.f;
-      if (row + r >= a.n_rows) continue;
-      T* dx = static_cast<T*>(a.dx) + (row + r) * a.hidden + first;
-#pragma unroll
-      for (int e = 0; e < kEpt; ++e) {
-        if (first + 32 * e < a.hidden) CeElem<T>::store(dx + 32 * e, rstd[r] * (fmaf(-xhat[r][e], c, m[r][e]) - mm));
-      }
-    }
+    for (int s = 0; s < kSlots - 1; ++s) fetch(row + s * step, s);
+    fetch_statistics(row);
   }
-  // the groups of the block, folded in halves in a fixed order
-  auto leave = [&](float (&acc)[kEpt], float* partial) {
-    for (int half = groups >> 1; half > 0; half >>= 1) {
-      __syncthreads();
-      if (g >= half && g < 2 * half) {
+  int slot = 0, phase = 0;
+  for (; row < a.n_rows; row += step) {
+    fetch(row + (kSlots - 1) * step, slot == 0 ? kSlots - 1 : slot - 1);
+    async_wait<kSlots - 1>();
+    warp_sync();
+    F2 xhat[kRows][kPairs], m[kRows][kPairs];
+    float rstd[kRows], v[4] = {0.f, 0.f, 0.f, 0.f};           // (sum m xhat, sum m) of each row
 #pragma unroll
-        for (int e = 0; e < kEpt; ++e) fold[((g - half) * kEpt + e) * group + t] = acc[e];
+    for (int r = 0; r < kRows; ++r) {
+      const int n = row + r < a.n_rows ? count : 0;
+      window_read<T, kEpt>(window(slot, r, 0), source_x(row + r), n, lane, xhat[r]);
+      window_read<T, kEpt>(window(slot, r, 1), source_dy(row + r), n, lane, m[r]);
+      rstd[r] = next_rstd[r];
+      const F2 minus_mean = both(-next_mean[r]);
+      F2 s_mx = both(0.f), s_m = both(0.f);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        // behind the row's end dy is zero, which keeps xhat out of every sum
+        if (kCentered) xhat[r][i] = add2(xhat[r][i], minus_mean);
+        xhat[r][i] = mul2(xhat[r][i], both(rstd[r]));
+        F2 xw = xhat[r][i];
+        if (rounded) xw = f2(norm_round<T>(f2_lo(xw)), norm_round<T>(f2_hi(xw)));
+        dw[i] = fma2(m[r][i], xw, dw[i]);
+        if (kCentered) db[i] = add2(db[i], m[r][i]);
+        m[r][i] = mul2(m[r][i], gain[i]);
+        s_mx = fma2(m[r][i], xhat[r][i], s_mx);
+        if (kCentered) s_m = add2(s_m, m[r][i]);
       }
-      __syncthreads();
-      if (g < half) {
+      v[2 * r] = f2_lo(s_mx) + f2_hi(s_mx);
+      v[2 * r + 1] = f2_lo(s_m) + f2_hi(s_m);
+    }
+    fetch_statistics(row + step);
+    const float sums = norm_warps_four_sums(v, warps, g, scratch, phase) * -inv;
 #pragma unroll
-        for (int e = 0; e < kEpt; ++e) acc[e] += fold[(g * kEpt + e) * group + t];
+    for (int r = 0; r < kRows; ++r) {
+      const F2 minus_c = both(norm_warp_of_four(sums, 2 * r));
+      const F2 minus_m = both(kCentered ? norm_warp_of_four(sums, 2 * r + 1) : 0.f);
+      if (row + r >= a.n_rows) continue;
+      T* dx = static_cast<T*>(a.dx) + (row + r) * a.hidden + column + lane;
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        F2 o = m[r][i];
+        if (kCentered) o = add2(o, minus_m);
+        o = mul2(fma2(xhat[r][i], minus_c, o), both(rstd[r]));
+        if (lane + 64 * i < count) CeElem<T>::store(dx + 64 * i, f2_lo(o));
+        if (lane + 64 * i + 32 < count) CeElem<T>::store(dx + 64 * i + 32, f2_hi(o));
       }
     }
-    if (g == 0) {
-      float* out = partial + static_cast<size_t>(blockIdx.x) * a.hidden + first;
+    slot = slot + 1 == kSlots ? 0 : slot + 1;
+  }
+  async_wait<0>();
+  // the groups' sums, added up by the threads of the block in the groups' order
+  float* fold = reinterpret_cast<float*>(stream_ring);
+  auto leave = [&](F2* acc, float* partial) {
+    __syncthreads();
+    if (g < groups) {
 #pragma unroll
-      for (int e = 0; e < kEpt; ++e) {
-        if (first + 32 * e < a.hidden) out[32 * e] = acc[e];
+      for (int i = 0; i < kPairs; ++i) {
+        fold[warp * 32 * kEpt + lane + 64 * i] = f2_lo(acc[i]);
+        fold[warp * 32 * kEpt + lane + 64 * i + 32] = f2_hi(acc[i]);
       }
+    }
+    __syncthreads();
+    float* out = partial + static_cast<size_t>(blockIdx.x) * a.hidden;
+    for (int c = static_cast<int>(threadIdx.x); c < a.hidden; c += kWindowThreads) {
+      float s = 0.f;
+      for (int k = 0; k < groups; ++k) s += fold[k * warps * 32 * kEpt + c];
+      out[c] = s;
     }
   };
   if (a.dw_partial != nullptr) leave(dw, a.dw_partial);
   if constexpr (kCentered) {
     if (a.db_partial != nullptr) leave(db, a.db_partial);
   }
+}
+
+// ---- rows of at most 32 elements without that alignment: one element per lane, groups of 4 to 32 lanes, several rows at a time
+template <typename T, typename W, bool kCentered>
+__global__ void __launch_bounds__(kNarrowThreads)
+norm_forward_tiny_kernel(NormForwardArgs a) {
+  constexpr int kRows = kNarrowForwardRows;
+  const int group = 1 << a.log2_group;
+  const int groups = kNarrowThreads >> a.log2_group;
+  const int t = static_cast<int>(threadIdx.x) & (group - 1);
+  const bool column = t < a.hidden;
+  const bool rounded = !kCentered && a.round_xhat != 0;
+  const float inv = 1.f / static_cast<float>(a.hidden);
+  const long long base = static_cast<long long>(blockIdx.x) * groups * kRows + (threadIdx.x >> a.log2_group);
+  const float gain = column && a.w != nullptr ? a.offset + CeElem<W>::load(static_cast<const W*>(a.w) + t) : 1.f;
+  const float bias = column && a.b != nullptr ? CeElem<W>::load(static_cast<const W*>(a.b) + t) : 0.f;
+  float x[kRows], v[4], mean = 0.f;
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const long long row = base + r * groups;
+    x[r] = column && row < a.n_rows ? CeElem<T>::load(static_cast<const T*>(a.x) + row * a.ld_x + t) : 0.f;
+  }
+  if (kCentered) mean = norm_lane_four_sums(x, group) * inv;
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const float m = kCentered ? norm_of_four(mean, r, a.log2_group) : 0.f;
+    x[r] = column ? x[r] - m : 0.f;
+    v[r] = x[r] * x[r];
+  }
+  const float rstd = norm_rsqrt(fmaf(norm_lane_four_sums(v, group), inv, a.eps));
+  {
+    const long long row = base + t / (group >> 2) * groups;
+    if (t % (group >> 2) == 0 && row < a.n_rows) {
+      if (kCentered && a.mean != nullptr) a.mean[row] = mean;
+      if (a.rstd != nullptr) a.rstd[row] = rstd;
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const long long row = base + r * groups;
+    float o = x[r] * norm_of_four(rstd, r, a.log2_group);
+    if (rounded) o = norm_round<T>(o);
+    o = kCentered ? fmaf(o, gain, bias) : o * gain;
+    if (column && row < a.n_rows) CeElem<T>::store(static_cast<T*>(a.y) + row * a.hidden + t, o);
+  }
+}
+
+template <typename T, typename W, bool kCentered>
+__global__ void __launch_bounds__(kNarrowThreads)
+norm_backward_tiny_kernel(NormBackwardArgs a) {
+  constexpr int kRows = kNarrowBackwardRows;
+  __shared__ float fold[kNarrowThreads];
+  const int group = 1 << a.log2_group;
+  const int groups = kNarrowThreads >> a.log2_group;
+  const int t = static_cast<int>(threadIdx.x) & (group - 1);
+  const int g = static_cast<int>(threadIdx.x) >> a.log2_group;
+  const bool column = t < a.hidden;
+  const bool rounded = !kCentered && a.round_xhat != 0;
+  const float inv = 1.f / static_cast<float>(a.hidden);
+  const float gain = column && a.w != nullptr ? a.offset + CeElem<W>::load(static_cast<const W*>(a.w) + t) : 1.f;
+  float dw = 0.f, db = 0.f;
+  const long long step = static_cast<long long>(gridDim.x) * groups * kRows;
+  for (long long base = static_cast<long long>(blockIdx.x) * groups * kRows; base < a.n_rows; base += step) {
+    float xhat[kRows], m[kRows], rstd[kRows], v[4];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const long long row = base + g + r * groups;
+      const bool live = row < a.n_rows;
+      rstd[r] = live ? __ldg(a.rstd + row) : 0.f;
+      const float mean = kCentered && live ? __ldg(a.mean + row) : 0.f;
+      xhat[r] = column && live ? (CeElem<T>::load(static_cast<const T*>(a.x) + row * a.ld_x + t) - mean) * rstd[r] : 0.f;
+      m[r] = column && live ? CeElem<T>::load(static_cast<const T*>(a.dy) + row * a.ld_dy + t) : 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      dw = fmaf(m[r], rounded ? norm_round<T>(xhat[r]) : xhat[r], dw);
+      db += m[r];
+      m[r] *= gain;
+      v[2 * r] = m[r] * xhat[r];
+      v[2 * r + 1] = m[r];
+    }
+    const float sums = norm_lane_four_sums(v, group) * inv;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const long long row = base + g + r * groups;
+      const float c = norm_of_four(sums, 2 * r, a.log2_group), mm = kCentered ? norm_of_four(sums, 2 * r + 1, a.log2_group) : 0.f;
+      if (column && row < a.n_rows) CeElem<T>::store(static_cast<T*>(a.dx) + row * a.hidden + t, rstd[r] * (fmaf(-xhat[r], c, m[r]) - mm));
+    }
+  }
+  auto leave = [&](float acc, float* partial) {
+    __syncthreads();
+    fold[threadIdx.x] = acc;
+    __syncthreads();
+    if (g == 0 && column) {
+      float s = 0.f;
+      for (int k = 0; k < groups; ++k) s += fold[(k << a.log2_group) + t];
+      partial[static_cast<size_t>(blockIdx.x) * a.hidden + t] = s;
+    }
+  };
+  if (a.dw_partial != nullptr) leave(dw, a.dw_partial);
+  if (kCentered && a.db_partial != nullptr) leave(db, a.db_partial);
 }
 
 // gradient[c] = sum over the blocks' partials; 32 columns per block, each summed by 32 threads in a fixed order.
@@ -949,9 +1125,9 @@ norm_parameter_gradient_kernel(const float* dw_partial, const float* db_partial,
 // two sums over the block, to all its threads
 __device__ __forceinline__ void norm_block_sum(float& s0, float& s1, float (*scratch)[kNormMaxWarps * 4], int& phase) {
   const float v[4] = {s0, s1, 0.f, 0.f};
-  const float sums = norm_group_four_sums(v, 9, scratch, phase);
-  s0 = norm_of_four(sums, 0, 9);
-  s1 = norm_of_four(sums, 1, 9);
+  const float sums = norm_warps_four_sums(v, kNormMaxWarps, 0, scratch, phase);
+  s0 = norm_warp_of_four(sums, 0);
+  s1 = norm_warp_of_four(sums, 1);
 }
 
 template <typename T, typename W, bool kCentered>

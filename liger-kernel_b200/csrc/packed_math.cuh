@@ -93,15 +93,16 @@ struct Pairs<__half> {
 #define FLCE_DYNAMIC_SHARED(type, name) extern __shared__ type name[]
 #endif
 
-// 16 bytes from global to this CTA's shared memory (past L1), or 16 zero bytes if !read; both addresses 16-byte aligned.  A
-// thread sees its own copies after async_wait; groups are waited for in the order they were committed.
-__device__ __forceinline__ void async_copy16(void* dst, const void* src, bool read) {
+// `bytes` (0..16) bytes from global to this CTA's shared memory (past L1), zeros up to 16; both addresses 16-byte aligned.  A
+// thread sees its own copies after async_wait, its warp's after a warp_sync behind that; groups are waited for in the order
+// they were committed.
+__device__ __forceinline__ void async_copy16(void* dst, const void* src, int bytes) {
 #ifdef FLCE_HOST_EMULATION
-  if (read) std::memcpy(dst, src, 16);
-  else std::memset(dst, 0, 16);
+  std::memset(dst, 0, 16);
+  if (bytes > 0) std::memcpy(dst, src, static_cast<size_t>(bytes));
 #else
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src),
-               "r"(read ? 16 : 0)
+               "r"(bytes)
                : "memory");
 #endif
 }
@@ -114,6 +115,14 @@ template <int kPending>
 __device__ __forceinline__ void async_wait() {
 #ifndef FLCE_HOST_EMULATION
   asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+#endif
+}
+
+__device__ __forceinline__ void warp_sync() {
+#ifdef FLCE_HOST_EMULATION
+  emu_warp_sync();
+#else
+  __syncwarp();
 #endif
 }
 

@@ -35,6 +35,7 @@ inline void emu_named_barrier(int id, int threads) {
   named[id].expected = static_cast<unsigned>(threads);
   emu::barrier_wait(named[id]);
 }
+inline void emu_warp_sync() { emu::barrier_wait(emu::t_ctx->warp_bar[emu::linear_tid() >> 5]); }
 inline void* emu_dynamic_shared() {
   alignas(128) static char bytes[227 * 1024];
   return bytes;
