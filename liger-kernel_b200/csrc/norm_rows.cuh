@@ -728,25 +728,43 @@ struct Window {
   static constexpr int kRingBytes = kSlots * kRoundPieces * 16 > kFoldBytes ? kSlots * kRoundPieces * 16 : kFoldBytes;
 };
 
-// the pieces of `count` elements from `src`, asked for by the lanes of a warp
+// the pieces of `count` elements from `src`, asked for by the lanes of a warp; zeros in the rest of the window
 template <typename T, int kPieces>
 __device__ __forceinline__ void window_fetch(uint4* window, const T* src, int count, int lane) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(src);
-  const int end = static_cast<int>(at & 15) + count * static_cast<int>(sizeof(T));
+  const int end = count > 0 ? static_cast<int>(at & 15) + count * static_cast<int>(sizeof(T)) : 0;
   const char* base = reinterpret_cast<const char*>(at & ~static_cast<uintptr_t>(15));
 #pragma unroll
   for (int i = 0; i < kPieces; i += 32) {
-    const int piece = i + lane;
-    if (piece * 16 < end) async_copy16(window + piece, base + piece * 16, end - piece * 16 < 16 ? end - piece * 16 : 16);
+    const int left = end - (i + lane) * 16;
+    if (i + 32 <= kPieces || i + lane < kPieces)
+      async_copy16(window + i + lane, left > 0 ? base + (i + lane) * 16 : base, left < 0 ? 0 : (left < 16 ? left : 16));
   }
 }
 // kEpt elements of this lane, in pairs, zeros behind the end
 template <typename T, int kEpt>
-__device__ __forceinline__ void window_read(const uint4* window, const T* src, int count, int lane, F2 (&v)[kEpt / 2]) {
+__device__ __forceinline__ void window_read(const uint4* window, const T* src, int lane, F2 (&v)[kEpt / 2]) {
   const T* e = reinterpret_cast<const T*>(reinterpret_cast<const char*>(window) + (reinterpret_cast<uintptr_t>(src) & 15)) + lane;
 #pragma unroll
-  for (int i = 0; i < kEpt / 2; ++i)
-    v[i] = f2(lane + 64 * i < count ? CeElem<T>::load(e + 64 * i) : 0.f, lane + 64 * i + 32 < count ? CeElem<T>::load(e + 64 * i + 32) : 0.f);
+  for (int i = 0; i < kEpt / 2; ++i) v[i] = f2(CeElem<T>::load(e + 64 * i), CeElem<T>::load(e + 64 * i + 32));
+}
+// and back; a part that is full, as all but a row's last are, needs no look at the end
+template <typename T, int kEpt>
+__device__ __forceinline__ void window_store(T* dst, int count, int lane, const F2 (&v)[kEpt / 2]) {
+  dst += lane;
+  if (count == 32 * kEpt) {
+#pragma unroll
+    for (int i = 0; i < kEpt / 2; ++i) {
+      CeElem<T>::store(dst + 64 * i, f2_lo(v[i]));
+      CeElem<T>::store(dst + 64 * i + 32, f2_hi(v[i]));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kEpt / 2; ++i) {
+      if (lane + 64 * i < count) CeElem<T>::store(dst + 64 * i, f2_lo(v[i]));
+      if (lane + 64 * i + 32 < count) CeElem<T>::store(dst + 64 * i + 32, f2_hi(v[i]));
+    }
+  }
 }
 
 template <typename T, typename W, bool kCentered, int kEpt>
@@ -786,7 +804,8 @@ norm_forward_window_kernel(NormForwardArgs a) {
   auto fetch = [&](long long base, int slot) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      if (base + r < a.n_rows) window_fetch<T, Shape::kPieces>(window(slot, r), source(base + r), count, lane);
+      const bool live = base + r < a.n_rows;
+      window_fetch<T, Shape::kPieces>(window(slot, r), source(live ? base + r : 0), live ? count : 0, lane);
     }
     async_commit();
   };
@@ -802,8 +821,7 @@ norm_forward_window_kernel(NormForwardArgs a) {
     F2 x[kRows][kPairs];
     float v[4] = {0.f, 0.f, 0.f, 0.f}, mean = 0.f;            // mean of row lane >> 3
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
-      window_read<T, kEpt>(window(slot, r), source(row + r), row + r < a.n_rows ? count : 0, lane, x[r]);
+    for (int r = 0; r < kRows; ++r) window_read<T, kEpt>(window(slot, r), source(row + r < a.n_rows ? row + r : 0), lane, x[r]);
     if constexpr (kCentered) {
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
@@ -819,10 +837,11 @@ norm_forward_window_kernel(NormForwardArgs a) {
       if constexpr (kCentered) {
         const F2 minus_mean = both(-norm_warp_of_four(mean, r));
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          x[r][i] = add2(x[r][i], minus_mean);
-          // the columns behind the end hold zeros still
-          if (lane + 64 * i + 32 >= count) x[r][i] = f2(lane + 64 * i < count ? f2_lo(x[r][i]) : 0.f, 0.f);
+        for (int i = 0; i < kPairs; ++i) x[r][i] = add2(x[r][i], minus_mean);
+        if (count < 32 * kEpt) {            // behind the row's end there is nothing to centre
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i)
+            x[r][i] = f2(lane + 64 * i < count ? f2_lo(x[r][i]) : 0.f, lane + 64 * i + 32 < count ? f2_hi(x[r][i]) : 0.f);
         }
       }
       F2 acc = both(0.f);
@@ -842,16 +861,14 @@ norm_forward_window_kernel(NormForwardArgs a) {
     for (int r = 0; r < kRows; ++r) {
       const F2 scale = both(norm_warp_of_four(rstd, r));
       if (row + r >= a.n_rows) continue;
-      T* y = static_cast<T*>(a.y) + (row + r) * a.hidden + column + lane;
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
         F2 o = mul2(x[r][i], scale);
         if (rounded) o = f2(norm_round<T>(f2_lo(o)), norm_round<T>(f2_hi(o)));
-        if constexpr (kCentered) o = fma2(o, gain[i], bias[i]);
-        else o = mul2(o, gain[i]);
-        if (lane + 64 * i < count) CeElem<T>::store(y + 64 * i, f2_lo(o));
-        if (lane + 64 * i + 32 < count) CeElem<T>::store(y + 64 * i + 32, f2_hi(o));
+        if constexpr (kCentered) x[r][i] = fma2(o, gain[i], bias[i]);
+        else x[r][i] = mul2(o, gain[i]);
       }
+      window_store<T, kEpt>(static_cast<T*>(a.y) + (row + r) * a.hidden + column, count, lane, x[r]);
     }
     slot = slot + 1 == kSlots ? 0 : slot + 1;
   }
@@ -895,10 +912,9 @@ norm_backward_window_kernel(NormBackwardArgs a) {
   auto fetch = [&](long long base, int slot) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      if (base + r < a.n_rows) {
-        window_fetch<T, Shape::kPieces>(window(slot, r, 0), source_x(base + r), count, lane);
-        window_fetch<T, Shape::kPieces>(window(slot, r, 1), source_dy(base + r), count, lane);
-      }
+      const bool live = base + r < a.n_rows;
+      window_fetch<T, Shape::kPieces>(window(slot, r, 0), source_x(live ? base + r : 0), live ? count : 0, lane);
+      window_fetch<T, Shape::kPieces>(window(slot, r, 1), source_dy(live ? base + r : 0), live ? count : 0, lane);
     }
     async_commit();
   };
@@ -926,9 +942,9 @@ norm_backward_window_kernel(NormBackwardArgs a) {
     float rstd[kRows], v[4] = {0.f, 0.f, 0.f, 0.f};           // (sum m xhat, sum m) of each row
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const int n = row + r < a.n_rows ? count : 0;
-      window_read<T, kEpt>(window(slot, r, 0), source_x(row + r), n, lane, xhat[r]);
-      window_read<T, kEpt>(window(slot, r, 1), source_dy(row + r), n, lane, m[r]);
+      const long long from = row + r < a.n_rows ? row + r : 0;
+      window_read<T, kEpt>(window(slot, r, 0), source_x(from), lane, xhat[r]);
+      window_read<T, kEpt>(window(slot, r, 1), source_dy(from), lane, m[r]);
       rstd[r] = next_rstd[r];
       const F2 minus_mean = both(-next_mean[r]);
       F2 s_mx = both(0.f), s_m = both(0.f);
@@ -955,15 +971,12 @@ norm_backward_window_kernel(NormBackwardArgs a) {
       const F2 minus_c = both(norm_warp_of_four(sums, 2 * r));
       const F2 minus_m = both(kCentered ? norm_warp_of_four(sums, 2 * r + 1) : 0.f);
       if (row + r >= a.n_rows) continue;
-      T* dx = static_cast<T*>(a.dx) + (row + r) * a.hidden + column + lane;
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
-        F2 o = m[r][i];
-        if (kCentered) o = add2(o, minus_m);
-        o = mul2(fma2(xhat[r][i], minus_c, o), both(rstd[r]));
-        if (lane + 64 * i < count) CeElem<T>::store(dx + 64 * i, f2_lo(o));
-        if (lane + 64 * i + 32 < count) CeElem<T>::store(dx + 64 * i + 32, f2_hi(o));
+        if (kCentered) m[r][i] = add2(m[r][i], minus_m);
+        m[r][i] = mul2(fma2(xhat[r][i], minus_c, m[r][i]), both(rstd[r]));
       }
+      window_store<T, kEpt>(static_cast<T*>(a.dx) + (row + r) * a.hidden + column, count, lane, m[r]);
     }
     slot = slot + 1 == kSlots ? 0 : slot + 1;
   }
