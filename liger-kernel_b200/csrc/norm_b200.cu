@@ -42,8 +42,9 @@ int log2_group_for(long long pieces, int smallest) {
 }
 
 // Narrow: a lane per vector, rows of up to 32 of them.  Stream: two vectors per thread if a block's 512 threads reach so, else four.
-// Window: of 2, 4, 8 and 16 elements per lane the choice that leaves the fewest of the block's lanes without a column, the most
-// elements among equals (fewer warps to a row wait for each other).  Long: what is left, above 8192 elements.
+// Window: of 2, 4, 8 and 16 elements per lane the cheapest, taking a warp's part of a row to cost 8 elements beside those it
+// holds: 50000 x 300 bf16 forward 45, 33, 29 and 23 us, 10007 x 1537 fp16 43, 31 and 27 us from 4 on, 100000 x 100 bf16 45, 25,
+// 33 and 47 us.  Long: what is left, above 8192 elements.
 NormPlan norm_plan(const flce_norm_t* p, bool vectors) {
   const long long n = p->hidden * element_size(p->dtype) / 16;
   if (vectors && n <= 32) return {kNormNarrow, 1, log2_group_for(n, 2), 0};
@@ -54,13 +55,13 @@ NormPlan norm_plan(const flce_norm_t* p, bool vectors) {
   }
   if (p->hidden <= 32) return {kNormTiny, 1, log2_group_for(p->hidden, 2), 0};
   NormPlan best{kNormLong, 0, 9, kNormMaxWarps};
-  double used = 0.0;
+  double least = 0.0;
   for (int share = 2; share <= 16; share *= 2) {
     const long long warps = ceil_div(p->hidden, 32 * share);
     if (warps > kWindowWarps) continue;
-    const double lanes = static_cast<double>(kWindowWarps / warps) * p->hidden / (32.0 * share * kWindowWarps);
-    if (lanes >= used) {
-      used = lanes;
+    const double cost = (share + 8.0) / static_cast<double>(kWindowWarps / warps);
+    if (best.path == kNormLong || cost < least) {
+      least = cost;
       best = {kNormWindow, share, 0, static_cast<int>(warps)};
     }
   }
