@@ -37,30 +37,48 @@ int check_layers(const flce_balance_t* p, const void* const* logits) {
 }
 
 struct BalanceShape {
-  bool vectors;
-  int ept, log2_group;
+  bool vectors;             // rows of whole, aligned vectors
+  bool tile;                // forward: rows by tiles of 32 per warp
+  int ept, log2_group;      // logits per lane, lanes per row
+  int tile_warps;           // warps per block of the tile kernel, as many as its shared memory holds, 8 at most
 };
 
 // Lanes that share a row: as many as it takes with 8 logits each, and more logits per lane beyond 256 experts.
-BalanceShape balance_shape(const flce_balance_t* p, const void* const* logits, const void* out) {
+BalanceShape balance_shape(const flce_balance_t* p, bool vectors) {
   BalanceShape s;
-  const int vec = 16 / element_size(p->dtype);
-  s.vectors = p->n_experts % vec == 0 && (p->n_tokens <= 1 || p->ld % vec == 0) && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-  for (int64_t l = 0; l < p->n_layers; ++l) s.vectors = s.vectors && (reinterpret_cast<uintptr_t>(logits[l]) & 15) == 0;
+  s.vectors = vectors;
   s.ept = p->n_experts <= 256 ? 8 : (p->n_experts <= 512 ? 16 : 32);
   for (s.log2_group = 0; (s.ept << s.log2_group) < p->n_experts;) ++s.log2_group;
+  s.tile = vectors && p->n_experts % 8 == 0 && p->n_experts >= 32 && p->n_experts <= 256 && p->top_k <= kTileList;
+  s.tile_warps = 220 * 1024 / tile_warp_bytes(static_cast<int>(p->n_experts) * element_size(p->dtype));
+  if (s.tile_warps > kBalWarps) s.tile_warps = kBalWarps;
   return s;
 }
 
-// Blocks per layer: eight per SM over all layers, so that the last wave costs little, but a round of rows each.
-long long balance_blocks(const flce_balance_t* p, int sm_count) {
-  int log2_group = 0;
-  const int ept = p->n_experts <= 256 ? 8 : (p->n_experts <= 512 ? 16 : 32);
-  while ((ept << log2_group) < p->n_experts) ++log2_group;
-  const long long rounds = ceil_div(p->n_tokens, kBalThreads >> log2_group);
-  long long blocks = ceil_div(8ll * sm_count, p->n_layers);
+bool whole_vectors(const flce_balance_t* p, const void* const* logits, const void* out) {
+  const int vec = 16 / element_size(p->dtype);
+  bool yes = p->n_experts % vec == 0 && (p->n_tokens <= 1 || p->ld % vec == 0) && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  for (int64_t l = 0; l < p->n_layers; ++l) yes = yes && (reinterpret_cast<uintptr_t>(logits[l]) & 15) == 0;
+  return yes;
+}
+
+// Blocks per layer of the kernels that walk over the rows: `per_sm` of them per SM over all layers, a round of rows each at least.
+long long walking_blocks(const flce_balance_t* p, long long rows_per_round, int per_sm, int sm_count) {
+  const long long rounds = ceil_div(p->n_tokens, rows_per_round);
+  long long blocks = ceil_div(static_cast<long long>(per_sm) * sm_count, p->n_layers);
   if (blocks > rounds) blocks = rounds;
   return blocks < 1 ? 1 : blocks;
+}
+// Forward leaves a partial sum per block: the plain kernel has eight blocks per SM, so that the last wave costs little; the tile
+// kernel as many as are resident, which its warps share evenly.
+long long forward_blocks(const flce_balance_t* p, const BalanceShape& s, int sm_count) {
+  if (!s.tile) return walking_blocks(p, kBalThreads >> s.log2_group, 8, sm_count);
+  const int bytes = s.tile_warps * tile_warp_bytes(static_cast<int>(p->n_experts) * element_size(p->dtype));
+  const int resident = 220 * 1024 / bytes < 2 ? 1 : 2;
+  const long long slots = static_cast<long long>(resident) * sm_count;
+  const long long blocks = slots / p->n_layers;                  // one wave
+  const long long rounds = ceil_div(p->n_tokens, 32 * s.tile_warps);
+  return blocks > rounds ? (rounds > 0 ? rounds : 1) : (blocks > 0 ? blocks : 1);
 }
 
 BalanceArgs balance_args(const flce_balance_t* p, const void* const* logits, int64_t first_layer, int64_t layers, const BalanceShape& s) {
@@ -93,9 +111,22 @@ void run_forward(const BalanceArgs& a, const BalanceShape& s, dim3 grid, float* 
   }
 }
 
+template <typename T>
+int run_forward_tile(const BalanceArgs& a, const BalanceShape& s, dim3 grid, float* partial, cudaStream_t stream) {
+  const size_t tiles = static_cast<size_t>(s.tile_warps) * tile_warp_bytes(a.experts * static_cast<int>(sizeof(T)));
+  const size_t fold = static_cast<size_t>(s.tile_warps) * (2 * 256 + 2) * 4;
+  return launch_with_shared<balance_forward_tile_kernel<T>>(grid, static_cast<unsigned>(s.tile_warps * 32), tiles > fold ? tiles : fold, stream,
+                                                           a, partial);
+}
+
+// With a group of 4 lanes or more the four-row kernel; smaller groups have rows short enough for a lane or two.
 template <typename T, bool kVectors>
 void run_backward(const BalanceArgs& a, const BalanceShape& s, dim3 grid, const float* coef, const float* up, T* out,
                   cudaStream_t stream) {
+  if (s.ept == 8 && s.log2_group >= 2) {
+    FLCE_LAUNCH((balance_backward_four_kernel<T, kVectors>), grid, kBalThreads, stream, a, coef, up, out);
+    return;
+  }
   switch (s.ept) {
     case 8: FLCE_LAUNCH((balance_backward_kernel<T, kVectors, 8>), grid, kBalThreads, stream, a, coef, up, out); break;
     case 16: FLCE_LAUNCH((balance_backward_kernel<T, kVectors, 16>), grid, kBalThreads, stream, a, coef, up, out); break;
@@ -119,7 +150,9 @@ extern "C" {
 size_t flce_b200_balance_workspace_bytes(const flce_balance_t* p) {
   int sms = 0;
   if (check_balance(p) != FLCE_OK || current_sm_count(&sms) != FLCE_OK) return 0;
-  return workspace_bytes(p, balance_blocks(p, sms));
+  // whether the rows are whole, aligned vectors is not known yet: room for the larger grid
+  const long long plain = forward_blocks(p, balance_shape(p, false), sms), tile = forward_blocks(p, balance_shape(p, true), sms);
+  return workspace_bytes(p, plain > tile ? plain : tile);
 }
 
 int flce_b200_balance_forward(const flce_balance_t* p, const void* const* logits, float* loss, int64_t* counts, float* coef,
@@ -132,7 +165,8 @@ int flce_b200_balance_forward(const flce_balance_t* p, const void* const* logits
   int sms = 0;
   rc = current_sm_count(&sms);
   if (rc != FLCE_OK) return rc;
-  const long long blocks = balance_blocks(p, sms);
+  const BalanceShape s = balance_shape(p, whole_vectors(p, logits, nullptr));
+  const long long blocks = forward_blocks(p, s, sms);
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 7) != 0 || bytes < workspace_bytes(p, blocks))
     return fail(FLCE_ERR_WORKSPACE, "the balance loss needs %zu bytes of 8-byte aligned workspace, got %zu", workspace_bytes(p, blocks),
                 bytes);
@@ -141,7 +175,6 @@ int flce_b200_balance_forward(const flce_balance_t* p, const void* const* logits
   double* sums = static_cast<double*>(workspace);
   long long* kept = reinterpret_cast<long long*>(sums + p->n_layers * (p->n_experts + 1));
   float* partial = reinterpret_cast<float*>(kept + p->n_layers);
-  const BalanceShape s = balance_shape(p, logits, nullptr);
   int launches = 2;
   for (int64_t l = 0; l < p->n_layers; l += kBalMaxLayers) {
     const int64_t layers = p->n_layers - l < kBalMaxLayers ? p->n_layers - l : kBalMaxLayers;
@@ -150,14 +183,17 @@ int flce_b200_balance_forward(const flce_balance_t* p, const void* const* logits
     float* mine = partial + l * blocks * balance_partial_words(experts);
     with_type(p->dtype, [&](auto t) {
       using T = decltype(t);
-      if (s.vectors) run_forward<T, true>(a, s, grid, mine, stream);
+      if (s.tile) rc = run_forward_tile<T>(a, s, grid, mine, stream);
+      else if (s.vectors) run_forward<T, true>(a, s, grid, mine, stream);
       else run_forward<T, false>(a, s, grid, mine, stream);
     });
+    if (rc != FLCE_OK) return rc;
     ++launches;
   }
-  FLCE_LAUNCH((balance_layer_kernel), static_cast<unsigned>(p->n_layers), kBalThreads, stream, partial, static_cast<int>(blocks), experts,
+  const dim3 columns(static_cast<unsigned>(ceil_div(experts + 1, 32)), static_cast<unsigned>(p->n_layers));
+  FLCE_LAUNCH((balance_layer_kernel), columns, dim3(32, kBalFoldLanes), stream, partial, static_cast<int>(blocks), experts,
               reinterpret_cast<long long*>(counts), sums, kept);
-  FLCE_LAUNCH((balance_total_kernel), 1u, kBalThreads, stream, reinterpret_cast<const long long*>(counts), sums, kept,
+  FLCE_LAUNCH((balance_total_kernel), 1u, kBalTotalThreads, stream, reinterpret_cast<const long long*>(counts), sums, kept,
               static_cast<int>(p->n_layers), experts, p->lse_square_scale, loss, coef);
   FLCE_CUDA(cudaGetLastError());
   count_launches(launches);
@@ -178,8 +214,9 @@ int flce_b200_balance_backward(const flce_balance_t* p, const void* const* logit
   rc = current_sm_count(&sms);
   if (rc != FLCE_OK) return rc;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  const BalanceShape s = balance_shape(p, logits, grads);
-  const long long blocks = balance_blocks(p, sms);
+  const BalanceShape s = balance_shape(p, whole_vectors(p, logits, grads));
+  const bool four = s.ept == 8 && s.log2_group >= 2;
+  const long long blocks = walking_blocks(p, (kBalThreads >> s.log2_group) * (four ? 4 : 1), four ? 16 : 8, sms);
   int launches = 0;
   for (int64_t l = 0; l < p->n_layers; l += kBalMaxLayers) {
     const int64_t layers = p->n_layers - l < kBalMaxLayers ? p->n_layers - l : kBalMaxLayers;

@@ -38,20 +38,21 @@ inline int element_size(int dtype) { return dtype == FLCE_FP32 ? 4 : 2; }
 
 // The same for a kernel with `bytes` of dynamic shared memory; the permission for more than 48 KB is asked for once per kernel
 // and device (kKernel names the instantiation).
-template <auto kKernel, class Args>
-int launch_with_shared(dim3 grid, unsigned block, size_t bytes, cudaStream_t stream, const Args& args) {
+constexpr int kMostDynamicShared = 220 * 1024;      // beside what such a kernel declares statically: 227 KB in all
+template <auto kKernel, class... Args>
+int launch_with_shared(dim3 grid, unsigned block, size_t bytes, cudaStream_t stream, const Args&... args) {
 #ifndef FLCE_HOST_EMULATION
   static std::atomic<bool> allowed[64];
   int device = 0;
   FLCE_CUDA(cudaGetDevice(&device));
   if (!allowed[device & 63].load(std::memory_order_acquire)) {
-    FLCE_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+    FLCE_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostDynamicShared));
     allowed[device & 63].store(true, std::memory_order_release);
   }
-  kKernel<<<grid, block, bytes, stream>>>(args);
+  kKernel<<<grid, block, bytes, stream>>>(args...);
 #else
   (void)bytes;
-  FLCE_LAUNCH((kKernel), grid, block, stream, args);
+  FLCE_LAUNCH((kKernel), grid, block, stream, args...);
 #endif
   return FLCE_OK;
 }

@@ -80,29 +80,11 @@ __device__ __forceinline__ float norm_rsqrt(float v) {
   return v < INFINITY ? r * fmaf(-0.5f * v * r, r, 1.5f) : r;
 }
 
-// ---- four sums at a time
-//
-// Lanes that differ in the group's highest bit trade two sums for the other two, those that differ in the next bit one for the
-// other: 5 or 6 exchanges for four sums instead of 16 or 20.  The lane's two highest bits within its group (of its warp, if
-// the group is wider) then name its sum.
-__device__ __forceinline__ float norm_low_lane_sum(float v, int lanes) {      // over `lanes` neighbouring lanes
-  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-__device__ __forceinline__ float norm_lane_four_sums(const float (&v)[4], int lanes) {      // lanes: 4, 8, 16 or 32
-  const int lane = static_cast<int>(threadIdx.x) & 31;
-  const int half = lanes >> 1, quarter = lanes >> 2;
-  const bool up = (lane & half) != 0, right = (lane & quarter) != 0;
-  const float a0 = __shfl_xor_sync(0xffffffffu, up ? v[0] : v[2], half) + (up ? v[2] : v[0]);
-  const float a1 = __shfl_xor_sync(0xffffffffu, up ? v[1] : v[3], half) + (up ? v[3] : v[1]);
-  return norm_low_lane_sum(__shfl_xor_sync(0xffffffffu, right ? a0 : a1, quarter) + (right ? a1 : a0), quarter);
-}
-
 // Over the `warps` whole warps of group g.  Warps meet in one of two buffers taken in turn: a thread writes a buffer
 // again only behind the barrier of the call in between, which the readers of the older sums reach after reading them, so
 // one barrier per call is enough.
 __device__ __forceinline__ float norm_warps_four_sums(const float (&v)[4], int warps, int g, float (*scratch)[kNormMaxWarps * 4], int& phase) {
-  float sum = norm_lane_four_sums(v, 32);
+  float sum = lane_four_sums(v, 32);
   if (warps == 1) return sum;
   const int lane = static_cast<int>(threadIdx.x) & 31;
   float* buf = scratch[phase];
@@ -112,16 +94,10 @@ __device__ __forceinline__ float norm_warps_four_sums(const float (&v)[4], int w
   const float* of = buf + g * warps * 4 + (lane >> 3);
   sum = 0.f;
   for (int w = lane & 7; w < warps; w += 8) sum += of[w * 4];
-  return norm_low_lane_sum(sum, 8);
+  return low_lane_sum(sum, 8);
 }
 // sum number i of those, from a lane of the warp that holds it
 __device__ __forceinline__ float norm_warp_of_four(float sums, int i) { return __shfl_sync(0xffffffffu, sums, i * 8); }
-
-// the same from a lane of a group of 1 << log2_group lanes
-__device__ __forceinline__ float norm_of_four(float sums, int i, int log2_group) {
-  const int lanes = log2_group < 5 ? 1 << log2_group : 32;
-  return __shfl_sync(0xffffffffu, sums, (static_cast<int>(threadIdx.x) & 31 & ~(lanes - 1)) | i * (lanes >> 2));
-}
 
 // ---- rows of whole, aligned 16-byte vectors, more than a warp's worth: streamed through shared memory
 //
@@ -230,7 +206,7 @@ norm_forward_stream_kernel(NormForwardArgs a) {
         }
         v[r] = f2_lo(acc) + f2_hi(acc);
       }
-      part_sum = norm_lane_four_sums(v, 32);
+      part_sum = lane_four_sums(v, 32);
     }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
@@ -250,7 +226,7 @@ norm_forward_stream_kernel(NormForwardArgs a) {
       }
       v[r] = f2_lo(acc) + f2_hi(acc);
     }
-    float square = norm_lane_four_sums(v, 32);
+    float square = lane_four_sums(v, 32);
     float mean = part_sum * part_inv;       // of row lane >> 3, once the parts have met
     if (warps > 1) {
       float *buf = scratch[phase], *buf_sums = scratch_sums[kCentered ? phase : 0];
@@ -266,7 +242,7 @@ norm_forward_stream_kernel(NormForwardArgs a) {
       if constexpr (kCentered) {
         float sum = 0.f;
         for (int w = lane & 7; w < warps; w += 8) sum += buf_sums[of + w * 4];
-        mean = norm_low_lane_sum(sum, 8) * inv;
+        mean = low_lane_sum(sum, 8) * inv;
         for (int w = lane & 7; w < warps; w += 8) {
           const float n = part_elements(w);
           const float off = n > 0.f ? buf_sums[of + w * 4] / n - mean : 0.f;
@@ -275,7 +251,7 @@ norm_forward_stream_kernel(NormForwardArgs a) {
       } else {
         for (int w = lane & 7; w < warps; w += 8) square += buf[of + w * 4];
       }
-      square = norm_low_lane_sum(square, 8);
+      square = low_lane_sum(square, 8);
     }
     const float rstd = norm_rsqrt(fmaf(square, inv, a.eps));
 #pragma unroll
@@ -553,12 +529,12 @@ norm_forward_narrow_kernel(NormForwardArgs a) {
       for (int i = 0; i < kPairs; ++i) acc = add2(acc, Pairs<T>::get(reinterpret_cast<const uint32_t*>(&raw[r]) + i * Pairs<T>::kWords));
       v[r] = f2_lo(acc) + f2_hi(acc);
     }
-    mean = norm_lane_four_sums(v, group) * inv;
+    mean = lane_four_sums(v, group) * inv;
   }
   F2 minus_mean[kRows];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    minus_mean[r] = both(kCentered ? -norm_of_four(mean, r, a.log2_group) : 0.f);
+    minus_mean[r] = both(kCentered ? -of_four(mean, r, a.log2_group) : 0.f);
     F2 acc = both(0.f);
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
@@ -568,7 +544,7 @@ norm_forward_narrow_kernel(NormForwardArgs a) {
     }
     v[r] = column ? f2_lo(acc) + f2_hi(acc) : 0.f;
   }
-  const float rstd = norm_rsqrt(fmaf(norm_lane_four_sums(v, group), inv, a.eps));
+  const float rstd = norm_rsqrt(fmaf(lane_four_sums(v, group), inv, a.eps));
   {
     const int r = t / (group >> 2);
     const long long row = base + r * groups;
@@ -580,7 +556,7 @@ norm_forward_narrow_kernel(NormForwardArgs a) {
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const long long row = base + r * groups;
-    const F2 scale = both(norm_of_four(rstd, r, a.log2_group));
+    const F2 scale = both(of_four(rstd, r, a.log2_group));
     uint4 out;
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
@@ -660,12 +636,12 @@ norm_backward_narrow_kernel(NormBackwardArgs a) {
       v[2 * r] = f2_lo(mx) + f2_hi(mx);
       v[2 * r + 1] = f2_lo(m) + f2_hi(m);
     }
-    const float sums = norm_lane_four_sums(v, group) * -inv;
+    const float sums = lane_four_sums(v, group) * -inv;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       const long long row = base + g + r * groups;
-      const F2 minus_c = both(norm_of_four(sums, 2 * r, a.log2_group));
-      const F2 minus_m = both(kCentered ? norm_of_four(sums, 2 * r + 1, a.log2_group) : 0.f);
+      const F2 minus_c = both(of_four(sums, 2 * r, a.log2_group));
+      const F2 minus_m = both(kCentered ? of_four(sums, 2 * r + 1, a.log2_group) : 0.f);
       uint4 out;
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
@@ -1026,14 +1002,14 @@ norm_forward_tiny_kernel(NormForwardArgs a) {
     const long long row = base + r * groups;
     x[r] = column && row < a.n_rows ? CeElem<T>::load(static_cast<const T*>(a.x) + row * a.ld_x + t) : 0.f;
   }
-  if (kCentered) mean = norm_lane_four_sums(x, group) * inv;
+  if (kCentered) mean = lane_four_sums(x, group) * inv;
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    const float m = kCentered ? norm_of_four(mean, r, a.log2_group) : 0.f;
+    const float m = kCentered ? of_four(mean, r, a.log2_group) : 0.f;
     x[r] = column ? x[r] - m : 0.f;
     v[r] = x[r] * x[r];
   }
-  const float rstd = norm_rsqrt(fmaf(norm_lane_four_sums(v, group), inv, a.eps));
+  const float rstd = norm_rsqrt(fmaf(lane_four_sums(v, group), inv, a.eps));
   {
     const long long row = base + t / (group >> 2) * groups;
     if (t % (group >> 2) == 0 && row < a.n_rows) {
@@ -1044,7 +1020,7 @@ norm_forward_tiny_kernel(NormForwardArgs a) {
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const long long row = base + r * groups;
-    float o = x[r] * norm_of_four(rstd, r, a.log2_group);
+    float o = x[r] * of_four(rstd, r, a.log2_group);
     if (rounded) o = norm_round<T>(o);
     o = kCentered ? fmaf(o, gain, bias) : o * gain;
     if (column && row < a.n_rows) CeElem<T>::store(static_cast<T*>(a.y) + row * a.hidden + t, o);
@@ -1085,11 +1061,11 @@ norm_backward_tiny_kernel(NormBackwardArgs a) {
       v[2 * r] = m[r] * xhat[r];
       v[2 * r + 1] = m[r];
     }
-    const float sums = norm_lane_four_sums(v, group) * inv;
+    const float sums = lane_four_sums(v, group) * inv;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       const long long row = base + g + r * groups;
-      const float c = norm_of_four(sums, 2 * r, a.log2_group), mm = kCentered ? norm_of_four(sums, 2 * r + 1, a.log2_group) : 0.f;
+      const float c = of_four(sums, 2 * r, a.log2_group), mm = kCentered ? of_four(sums, 2 * r + 1, a.log2_group) : 0.f;
       if (column && row < a.n_rows) CeElem<T>::store(static_cast<T*>(a.dx) + row * a.hidden + t, rstd[r] * (fmaf(-xhat[r], c, m[r]) - mm));
     }
   }

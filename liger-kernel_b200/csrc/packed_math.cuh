@@ -1,5 +1,6 @@
 // Arithmetic on pairs of floats in one 64-bit register (add / mul / fma .f32x2: one instruction for two elements on sm_100) and
-// asynchronous 16-byte copies into shared memory, for kernels that are short of issue slots rather than of bandwidth.
+// asynchronous 16-byte copies into shared memory, and four sums over a group of lanes at once, for kernels that are short of issue
+// slots rather than of bandwidth.
 //
 // With FLCE_HOST_EMULATION the pairs are two floats and a copy is done when it is issued.
 #pragma once
@@ -133,6 +134,30 @@ __device__ __forceinline__ void named_barrier(int id, int threads) {
 #else
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 #endif
+}
+
+// ---- four sums at a time
+//
+// Lanes that differ in the group's highest bit trade two sums for the other two, those that differ in the next bit one for the
+// other: 5 or 6 exchanges for four sums instead of 16 or 20.  The lane's two highest bits within its group (of its warp, if
+// the group is wider) then name its sum.
+__device__ __forceinline__ float low_lane_sum(float v, int lanes) {      // over `lanes` neighbouring lanes
+  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float lane_four_sums(const float (&v)[4], int lanes) {      // lanes: 4, 8, 16 or 32
+  const int lane = static_cast<int>(threadIdx.x) & 31;
+  const int half = lanes >> 1, quarter = lanes >> 2;
+  const bool up = (lane & half) != 0, right = (lane & quarter) != 0;
+  const float a0 = __shfl_xor_sync(0xffffffffu, up ? v[0] : v[2], half) + (up ? v[2] : v[0]);
+  const float a1 = __shfl_xor_sync(0xffffffffu, up ? v[1] : v[3], half) + (up ? v[3] : v[1]);
+  return low_lane_sum(__shfl_xor_sync(0xffffffffu, right ? a0 : a1, quarter) + (right ? a1 : a0), quarter);
+}
+
+// sum number i of those of this lane's group of 1 << log2_group lanes, 32 at most
+__device__ __forceinline__ float of_four(float sums, int i, int log2_group) {
+  const int lanes = log2_group < 5 ? 1 << log2_group : 32;
+  return __shfl_sync(0xffffffffu, sums, (static_cast<int>(threadIdx.x) & 31 & ~(lanes - 1)) | i * (lanes >> 2));
 }
 
 }  // namespace flce
