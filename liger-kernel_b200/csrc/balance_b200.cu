@@ -40,7 +40,8 @@ struct BalanceShape {
   bool vectors;             // rows of whole, aligned vectors
   bool tile;                // forward: rows by tiles of 32 per warp
   int ept, log2_group;      // logits per lane, lanes per row
-  int tile_warps;           // warps per block of the tile kernel, as many as its shared memory holds, 8 at most
+  int tile_warps, tile_buffers;     // warps per block of the tile kernel and tiles per warp, as its shared memory allows
+  size_t tile_bytes;
 };
 
 // Lanes that share a row: as many as it takes with 8 logits each, and more logits per lane beyond 256 experts.
@@ -50,8 +51,15 @@ BalanceShape balance_shape(const flce_balance_t* p, bool vectors) {
   s.ept = p->n_experts <= 256 ? 8 : (p->n_experts <= 512 ? 16 : 32);
   for (s.log2_group = 0; (s.ept << s.log2_group) < p->n_experts;) ++s.log2_group;
   s.tile = vectors && p->n_experts % 8 == 0 && p->n_experts >= 32 && p->n_experts <= 256 && p->top_k <= kTileList;
-  s.tile_warps = 220 * 1024 / tile_warp_bytes(static_cast<int>(p->n_experts) * element_size(p->dtype));
-  if (s.tile_warps > kBalWarps) s.tile_warps = kBalWarps;
+  const int row_bytes = static_cast<int>(p->n_experts) * element_size(p->dtype);
+  s.tile_buffers = kTileMaxWarps * tile_warp_bytes(row_bytes, 2) <= kMostDynamicShared ? 2 : 1;
+  s.tile_warps = kMostDynamicShared / tile_warp_bytes(row_bytes, s.tile_buffers);
+  if (s.tile_warps > kTileMaxWarps) s.tile_warps = kTileMaxWarps;
+  const long long tiles = ceil_div(p->n_tokens, 32);       // fewer than that many: a smaller block
+  if (s.tile_warps > tiles) s.tile_warps = tiles > 0 ? static_cast<int>(tiles) : 1;
+  const size_t fold = static_cast<size_t>(s.tile_warps) * (2 * 256 + 2) * 4;
+  s.tile_bytes = static_cast<size_t>(s.tile_warps) * tile_warp_bytes(row_bytes, s.tile_buffers);
+  if (s.tile_bytes < fold) s.tile_bytes = fold;
   return s;
 }
 
@@ -73,9 +81,7 @@ long long walking_blocks(const flce_balance_t* p, long long rows_per_round, int 
 // kernel as many as are resident, which its warps share evenly.
 long long forward_blocks(const flce_balance_t* p, const BalanceShape& s, int sm_count) {
   if (!s.tile) return walking_blocks(p, kBalThreads >> s.log2_group, 8, sm_count);
-  const int bytes = s.tile_warps * tile_warp_bytes(static_cast<int>(p->n_experts) * element_size(p->dtype));
-  const int resident = 220 * 1024 / bytes < 2 ? 1 : 2;
-  const long long slots = static_cast<long long>(resident) * sm_count;
+  const long long slots = sm_count;
   const long long blocks = slots / p->n_layers;                  // one wave
   const long long rounds = ceil_div(p->n_tokens, 32 * s.tile_warps);
   return blocks > rounds ? (rounds > 0 ? rounds : 1) : (blocks > 0 ? blocks : 1);
@@ -113,10 +119,8 @@ void run_forward(const BalanceArgs& a, const BalanceShape& s, dim3 grid, float* 
 
 template <typename T>
 int run_forward_tile(const BalanceArgs& a, const BalanceShape& s, dim3 grid, float* partial, cudaStream_t stream) {
-  const size_t tiles = static_cast<size_t>(s.tile_warps) * tile_warp_bytes(a.experts * static_cast<int>(sizeof(T)));
-  const size_t fold = static_cast<size_t>(s.tile_warps) * (2 * 256 + 2) * 4;
-  return launch_with_shared<balance_forward_tile_kernel<T>>(grid, static_cast<unsigned>(s.tile_warps * 32), tiles > fold ? tiles : fold, stream,
-                                                           a, partial);
+  return launch_with_shared<balance_forward_tile_kernel<T>>(grid, static_cast<unsigned>(s.tile_warps * 32), s.tile_bytes, stream, a,
+                                                           s.tile_buffers, partial);
 }
 
 // With a group of 4 lanes or more the four-row kernel; smaller groups have rows short enough for a lane or two.
@@ -175,7 +179,7 @@ int flce_b200_balance_forward(const flce_balance_t* p, const void* const* logits
   double* sums = static_cast<double*>(workspace);
   long long* kept = reinterpret_cast<long long*>(sums + p->n_layers * (p->n_experts + 1));
   float* partial = reinterpret_cast<float*>(kept + p->n_layers);
-  int launches = 2;
+  int launches = 1;
   for (int64_t l = 0; l < p->n_layers; l += kBalMaxLayers) {
     const int64_t layers = p->n_layers - l < kBalMaxLayers ? p->n_layers - l : kBalMaxLayers;
     const BalanceArgs a = balance_args(p, logits, l, layers, s);
@@ -190,11 +194,16 @@ int flce_b200_balance_forward(const flce_balance_t* p, const void* const* logits
     if (rc != FLCE_OK) return rc;
     ++launches;
   }
-  const dim3 columns(static_cast<unsigned>(ceil_div(experts + 1, 32)), static_cast<unsigned>(p->n_layers));
-  FLCE_LAUNCH((balance_layer_kernel), columns, dim3(32, kBalFoldLanes), stream, partial, static_cast<int>(blocks), experts,
-              reinterpret_cast<long long*>(counts), sums, kept);
-  FLCE_LAUNCH((balance_total_kernel), 1u, kBalTotalThreads, stream, reinterpret_cast<const long long*>(counts), sums, kept,
-              static_cast<int>(p->n_layers), experts, p->lse_square_scale, loss, coef);
+  // few partials: the last kernel adds them up itself
+  const bool few = p->n_layers * blocks <= 32;
+  if (!few) {
+    const dim3 columns(static_cast<unsigned>(ceil_div(experts + 1, 32)), static_cast<unsigned>(p->n_layers));
+    FLCE_LAUNCH((balance_layer_kernel), columns, dim3(32, kBalFoldLanes), stream, partial, static_cast<int>(blocks), experts,
+                reinterpret_cast<long long*>(counts), sums, kept);
+    ++launches;
+  }
+  FLCE_LAUNCH((balance_total_kernel), 1u, kBalTotalThreads, stream, few ? partial : nullptr, static_cast<int>(blocks),
+              reinterpret_cast<long long*>(counts), sums, kept, static_cast<int>(p->n_layers), experts, p->lse_square_scale, loss, coef);
   FLCE_CUDA(cudaGetLastError());
   count_launches(launches);
   return FLCE_OK;

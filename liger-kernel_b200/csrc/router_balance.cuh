@@ -274,6 +274,8 @@ balance_forward_kernel(BalanceArgs a, float* partial) {
 // network and merges them into a sorted list.  16-bit logits go through the network two to a word, the even and the odd columns
 // as two lists, which meet at the end.  Only the top_k-th largest logit and the largest are handed on; with them the warp
 // goes over the tile once more, rows shared by groups of lanes with 8 columns each, for the softmax and the sums per expert.
+// Where shared memory holds two tiles for each of 16 warps, the next one is fetched while this one is worked on; else one, and
+// the other warps cover the wait: more warps count for more than the second tile.
 constexpr int kTileList = 8;
 
 template <typename T>
@@ -339,22 +341,23 @@ __device__ __forceinline__ void tile_merge(typename TileWord<T>::Word (&v)[8]) {
 
 // bytes from one row of a tile to the next: an odd number of vectors, so that 8 lanes reading a vector of 8 rows meet all banks
 __host__ __device__ inline int tile_pitch(int row_bytes) { return (row_bytes / 16 | 1) * 16; }
-__host__ __device__ inline int tile_warp_bytes(int row_bytes) { return 2 * 32 * tile_pitch(row_bytes) + 32 * 8; }
+__host__ __device__ inline int tile_warp_bytes(int row_bytes, int buffers) { return buffers * 32 * tile_pitch(row_bytes) + 32 * 8; }
+constexpr int kTileMaxWarps = 16;
 
 template <typename T>
-__global__ void __launch_bounds__(kBalThreads)
-balance_forward_tile_kernel(BalanceArgs a, float* partial) {
+__global__ void __launch_bounds__(kTileMaxWarps * 32, 1)
+balance_forward_tile_kernel(BalanceArgs a, int buffers, float* partial) {
   typedef TileWord<T> Tile;
   typedef typename Tile::Word Word;
   constexpr int kVec = CeElem<T>::kVec;
   constexpr int kVectors = 8 / kVec;                          // of the 8 columns of a lane
-  FLCE_DYNAMIC_SHARED(uint4, tile_shared);                    // per warp: two tiles, and (top_k-th logit, largest) of 32 rows
+  FLCE_DYNAMIC_SHARED(uint4, tile_shared);                    // per warp: one or two tiles, and (top_k-th logit, largest) of 32 rows
   const int lane = static_cast<int>(threadIdx.x) & 31, warp = static_cast<int>(threadIdx.x) >> 5;
   const int warps = static_cast<int>(blockDim.x) >> 5;
   const int vectors = a.experts / kVec;                       // of a row
   const int pitch = tile_pitch(vectors * 16) / 16;
-  uint4* tiles = tile_shared + warp * (tile_warp_bytes(vectors * 16) / 16);
-  float2* chosen_of = reinterpret_cast<float2*>(tiles + 2 * 32 * pitch);
+  uint4* tiles = tile_shared + warp * (tile_warp_bytes(vectors * 16, buffers) / 16);
+  float2* chosen_of = reinterpret_cast<float2*>(tiles + buffers * 32 * pitch);
   const T* logits = static_cast<const T*>(a.logits[blockIdx.y]);
 
   const int group = 1 << a.log2_group, groups = 32 >> a.log2_group;
@@ -389,8 +392,12 @@ balance_forward_tile_kernel(BalanceArgs a, float* partial) {
   for (; tile * 32 < a.n_tokens; tile += step) {
     const unsigned next_kept = __ballot_sync(0xffffffffu, after);
     after = balance_kept(a, (tile + 2 * step) * 32 + lane);
-    fetch(tile + step, next_kept, tiles + (which ^ 1) * 32 * pitch);
-    async_wait<1>();
+    if (buffers == 2) {
+      fetch(tile + step, next_kept, tiles + (which ^ 1) * 32 * pitch);
+      async_wait<1>();
+    } else {
+      async_wait<0>();
+    }
     warp_sync();
     const uint4* here = tiles + which * 32 * pitch;
     if (kept != 0) {
@@ -505,9 +512,10 @@ balance_forward_tile_kernel(BalanceArgs a, float* partial) {
         }
       }
     }
-    warp_sync();        // the tile's last readers, before the fetch after the next overwrites it
+    warp_sync();        // the tile's last readers, before a fetch overwrites it
+    if (buffers == 2) which ^= 1;
+    else fetch(tile + step, next_kept, tiles);
     kept = next_kept;
-    which ^= 1;
   }
   async_wait<0>();
   // the warp's groups, then the block's warps, in a fixed order
@@ -551,8 +559,8 @@ balance_forward_tile_kernel(BalanceArgs a, float* partial) {
 }
 
 // counts[layer][:], sums[layer][:] = S_e and the sum of lse^2 of that layer, kept[layer]: one block per layer (blockIdx.y) and 32
-// columns, each added up by 8 threads in a fixed order
-constexpr int kBalFoldLanes = 8;
+// columns, each added up by 32 threads in a fixed order
+constexpr int kBalFoldLanes = 32;
 __global__ void __launch_bounds__(32 * kBalFoldLanes)
 balance_layer_kernel(const float* partial, int blocks, int experts, long long* counts, double* sums, long long* kept) {
   __shared__ double part_s[kBalFoldLanes][32];
@@ -584,28 +592,49 @@ balance_layer_kernel(const float* partial, int blocks, int experts, long long* c
 }
 
 // out[0] = loss, out[1] = its lse^2 term; coef[e] = a_e, coef[experts] = 2 lambda / N.  No kept token: all zero.  One block: a
-// thread per expert and share of the layers.
+// thread per expert and share of the layers.  With few partials (partial != nullptr) it adds them up itself, in the place of
+// balance_layer_kernel, and leaves the counts.
 constexpr int kBalTotalThreads = 1024;
 __global__ void __launch_bounds__(kBalTotalThreads)
-balance_total_kernel(const long long* counts, const double* sums, const long long* kept, int layers, int experts, float lambda,
-                     float* out, float* coef) {
-  __shared__ double scratch[kBalTotalThreads / 32];
+balance_total_kernel(const float* partial, int blocks, long long* counts, const double* sums, const long long* kept, int layers, int experts,
+                     float lambda, float* out, float* coef) {
+  __shared__ double scratch[4][kBalTotalThreads / 32];
   __shared__ double part_c[kBalTotalThreads], part_s[kBalTotalThreads];
   const int tid = static_cast<int>(threadIdx.x);
+  const long long words = balance_partial_words(experts);
   int wide = 32;
   while (wide < experts) wide *= 2;
   const int e = tid & (wide - 1), shares = kBalTotalThreads / wide;
-  double c = 0.0, s = 0.0, tokens = 0.0, z = 0.0;
+  double c = 0.0, s = 0.0, v[4] = {0.0, 0.0, 0.0, 0.0};      // v: sum C S, sum C, N, sum lse^2
   if (e < experts) {
 #pragma unroll 4
     for (int l = tid / wide; l < layers; l += shares) {
-      c += static_cast<double>(counts[static_cast<long long>(l) * experts + e]);
-      s += sums[static_cast<long long>(l) * (experts + 1) + e];
+      if (partial != nullptr) {
+        long long here = 0;
+        for (int b = 0; b < blocks; ++b) {
+          const float* row = partial + (static_cast<long long>(l) * blocks + b) * words + e;
+          s += row[0];
+          here += reinterpret_cast<const int*>(row)[experts + 1];
+        }
+        counts[static_cast<long long>(l) * experts + e] = here;
+        c += static_cast<double>(here);
+      } else {
+        c += static_cast<double>(counts[static_cast<long long>(l) * experts + e]);
+        s += sums[static_cast<long long>(l) * (experts + 1) + e];
+      }
     }
   }
-  for (int l = tid; l < layers; l += kBalTotalThreads) {
-    tokens += static_cast<double>(kept[l]);
-    z += sums[static_cast<long long>(l) * (experts + 1) + experts];
+  if (partial != nullptr) {
+    for (int r = tid; r < layers * blocks; r += kBalTotalThreads) {
+      const float* row = partial + r * words + experts;
+      v[3] += row[0];
+      v[2] += reinterpret_cast<const int*>(row)[experts + 1];
+    }
+  } else {
+    for (int l = tid; l < layers; l += kBalTotalThreads) {
+      v[2] += static_cast<double>(kept[l]);
+      v[3] += sums[static_cast<long long>(l) * (experts + 1) + experts];
+    }
   }
   part_c[tid] = c;
   part_s[tid] = s;
@@ -615,29 +644,28 @@ balance_total_kernel(const long long* counts, const double* sums, const long lon
       c += part_c[k * wide + tid];
       s += part_s[k * wide + tid];
     }
-  } else {
-    c = s = 0.0;
+    v[0] = c * s;
+    v[1] = c;
   }
-  auto block_sum = [&](double v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();                     // the sums of the call before have been read
-    if ((tid & 31) == 0) scratch[tid >> 5] = v;
-    __syncthreads();
-    v = scratch[tid & 31];
+  for (int i = 0; i < 4; ++i) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-  };
-  const double dot = block_sum(c * s), all = block_sum(c);
-  tokens = block_sum(tokens);
-  z = block_sum(z);
-  const double inv = tokens > 0.0 ? 1.0 / tokens : 0.0;
+    for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    if ((tid & 31) == 0) scratch[i][tid >> 5] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = scratch[i][tid & 31];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  }
+  const double inv = v[2] > 0.0 ? 1.0 / v[2] : 0.0;
   const double scale = experts * inv * inv;
-  if (tid < experts) coef[tid] = static_cast<float>(scale * (c - all / experts));
+  if (tid < experts) coef[tid] = static_cast<float>(scale * (c - v[1] / experts));
   if (tid == 0) {
-    out[0] = static_cast<float>(scale * dot + lambda * inv * z);
-    out[1] = static_cast<float>(lambda * inv * z);
+    out[0] = static_cast<float>(scale * v[0] + lambda * inv * v[3]);
+    out[1] = static_cast<float>(lambda * inv * v[3]);
     coef[experts] = static_cast<float>(2.0 * lambda * inv);
   }
 }

@@ -297,8 +297,9 @@ struct BalanceBackward : public torch::autograd::Node {
     Tensor all = at::empty({o.p.n_layers, o.p.n_tokens, num_experts}, x[0].options().memory_format(at::MemoryFormat::Contiguous));
     check(g_lib.balance_backward(&o.p, o.pointers.data(), coef.const_data_ptr<float>(), up.const_data_ptr<float>(), all.data_ptr(),
                                  on.stream));
+    const std::vector<Tensor> layers = all.unbind(0);
     for (size_t l = 0; l < x.size(); ++l) {
-      if (task_should_compute_output(l)) out[l] = all.select(0, static_cast<int64_t>(l)).reshape(x[l].sizes());
+      if (task_should_compute_output(l)) out[l] = x[l].dim() == 2 ? layers[l] : layers[l].view(x[l].sizes());
     }
     return once_differentiable(std::move(out), recording);
   }
@@ -315,15 +316,16 @@ std::tuple<Tensor, Tensor, Tensor> load_balancing_loss(at::TensorList logits, in
     const BalanceOperands o = balance_operands(logits, num_experts, top_k, mask, lse_square_scale);
     OnDevice on(logits[0]);
     const auto options = o.logits[0].options();
-    const Tensor out = at::empty({2}, options.dtype(at::kFloat));
+    // one buffer for the loss, its lse^2 term and what backward needs
+    const Tensor out = at::empty({num_experts + 3}, options.dtype(at::kFloat));
     counts = at::empty({o.p.n_layers, num_experts}, options.dtype(at::kLong));
-    coef = at::empty({num_experts + 1}, options.dtype(at::kFloat));
     const size_t bytes = g_lib.balance_workspace_bytes(&o.p);
     const Tensor workspace = at::empty({static_cast<int64_t>(bytes)}, options.dtype(at::kByte));
-    check(g_lib.balance_forward(&o.p, o.pointers.data(), out.data_ptr<float>(), counts.data_ptr<int64_t>(), coef.data_ptr<float>(),
+    check(g_lib.balance_forward(&o.p, o.pointers.data(), out.data_ptr<float>(), counts.data_ptr<int64_t>(), out.data_ptr<float>() + 2,
                                 workspace.data_ptr(), bytes, on.stream));
     loss = out.select(0, 0);
     z_loss = out.select(0, 1);
+    if (recording) coef = out.narrow(0, 2, num_experts + 1);
   }
   if (recording) {
     auto node = std::shared_ptr<BalanceBackward>(new BalanceBackward(), torch::autograd::deleteNode);
