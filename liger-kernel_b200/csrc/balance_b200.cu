@@ -50,7 +50,8 @@ BalanceShape balance_shape(const flce_balance_t* p, bool vectors) {
   s.vectors = vectors;
   s.ept = p->n_experts <= 256 ? 8 : (p->n_experts <= 512 ? 16 : 32);
   for (s.log2_group = 0; (s.ept << s.log2_group) < p->n_experts;) ++s.log2_group;
-  s.tile = vectors && p->n_experts % 8 == 0 && p->n_experts >= 32 && p->n_experts <= 256 && p->top_k <= kTileList;
+  s.tile = vectors && p->n_experts % 8 == 0 && p->n_experts >= 32 && p->n_experts <= 256 && p->top_k <= kTileList &&
+           p->n_tokens <= 1 << 24;
   const int row_bytes = static_cast<int>(p->n_experts) * element_size(p->dtype);
   s.tile_buffers = kTileMaxWarps * tile_warp_bytes(row_bytes, 2) <= kMostDynamicShared ? 2 : 1;
   s.tile_warps = kMostDynamicShared / tile_warp_bytes(row_bytes, s.tile_buffers);

@@ -364,13 +364,11 @@ balance_forward_tile_kernel(BalanceArgs a, int buffers, float* partial) {
   const int quarter = group >> 2;
   const int t = lane & (group - 1), q = lane >> a.log2_group;
   const bool column = t * 8 < a.experts;
-  F2 s[4];
-  int c[8], n = 0;
+  F2 s[4], c[4];            // c counts in floats, exactly: a lane sees at most 2^24 rows
+  int n = 0;
   float z = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) s[i] = both(0.f);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) c[e] = 0;
+  for (int i = 0; i < 4; ++i) s[i] = c[i] = both(0.f);
 
   // rows of a fetch side by side in the warp, for row lengths up to 32 vectors; longer rows go one at a time
   const int side = vectors < 32 ? 32 / vectors : 1;
@@ -444,70 +442,75 @@ balance_forward_tile_kernel(BalanceArgs a, int buffers, float* partial) {
       for (int r0 = q; r0 < 32; r0 += 4 * groups) {
         F2 x[4][4];
         float kth[4], total[4], taken[4];
-        unsigned ge[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int row = r0 + r * groups;
           uint4 raw[kVectors];
 #pragma unroll
           for (int i = 0; i < kVectors; ++i) {
-            raw[i] = make_uint4(0u, 0u, 0u, 0u);
+            raw[i] = make_uint4(~0u, ~0u, ~0u, ~0u);          // NaN behind the row's end: it compares with nothing
             if (column) raw[i] = here[row * pitch + t * kVectors + i];
           }
           const float2 of = chosen_of[row];
-          kth[r] = of.x;
-          ge[r] = 0;
+          const F2 counted = both((kept >> row & 1u) != 0 ? 1.f : 0.f);
           const F2 shift = both(-of.y * kLog2e);
-          F2 sum = both(0.f);
+          F2 sum = both(0.f), many = both(0.f);
+          kth[r] = of.x;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            x[r][i] = Pairs<T>::get(reinterpret_cast<const uint32_t*>(raw) + i * Pairs<T>::kWords);
-            const float lo = f2_lo(x[r][i]), hi = f2_hi(x[r][i]);
-            ge[r] |= (lo >= of.x ? 1u << 2 * i : 0u) | (hi >= of.x ? 2u << 2 * i : 0u);
-            const F2 d = fma2(x[r][i], both(kLog2e), shift);
+            const F2 v = Pairs<T>::get(reinterpret_cast<const uint32_t*>(raw) + i * Pairs<T>::kWords);
+            const F2 in = f2(f2_lo(v) >= of.x ? 1.f : 0.f, f2_hi(v) >= of.x ? 1.f : 0.f);
+            many = add2(many, in);
+            c[i] = fma2(in, counted, c[i]);
+            const F2 d = fma2(v, both(kLog2e), shift);
             x[r][i] = f2(ex2_approx(f2_lo(d)), ex2_approx(f2_hi(d)));
             sum = add2(sum, x[r][i]);
           }
-          if (!column) ge[r] = 0;
           total[r] = column ? f2_lo(sum) + f2_hi(sum) : 0.f;
-          taken[r] = static_cast<float>(__popc(ge[r]));
+          taken[r] = f2_lo(many) + f2_hi(many);
         }
         const float sums = lane_four_sums(total, group);
-        const float count = lane_four_sums(taken, group);
-        const float inv = 1.f / sums;
-        if ((t & (quarter - 1)) == 0) {                       // the lane that stands for its sum's row
-          const int row = r0 + t / quarter * groups;
-          if (kept >> row & 1u) {
-            ++n;
-            if (a.want_lse) {
-              const float lse = chosen_of[row].y + ln_approx(sums);
-              z = fmaf(lse, lse, z);
-            }
+        const float extra = lane_four_sums(taken, group) - static_cast<float>(a.top_k);
+        float inv = 1.f / sums;
+        const int row_of_sum = r0 + t / quarter * groups;     // the row that this lane's sums belong to
+        const bool kept_of_sum = (kept >> row_of_sum & 1u) != 0;
+        if (!kept_of_sum) inv = 0.f;
+        if ((t & (quarter - 1)) == 0 && kept_of_sum) {
+          ++n;
+          if (a.want_lse) {
+            const float lse = chosen_of[row_of_sum].y + ln_approx(sums);
+            z = fmaf(lse, lse, z);
           }
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int row = r0 + r * groups;
-          const bool counted = (kept >> row & 1u) != 0;
           const F2 scale = both(of_four(inv, r, a.log2_group));
-          int drop = static_cast<int>(of_four(count, r, a.log2_group)) - a.top_k;
-          if (!counted) drop = 0;
-          // more logits equal the last one chosen than there are places: the highest columns give way
-          while (__any_sync(0xffffffffu, drop > 0)) {
-            const uint4* row_here = here + row * pitch + t * kVectors;
-            unsigned equal = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) equal |= CeElem<T>::load(reinterpret_cast<const T*>(row_here) + (column ? e : -t * 8)) == kth[r] ? 1u << e : 0u;
-            equal &= ge[r];
-            const unsigned have = __ballot_sync(0xffffffffu, equal != 0 && drop > 0) >> (q << a.log2_group) & (group == 32 ? 0xffffffffu : (1u << group) - 1u);
-            if (drop > 0 && t == 31 - __clz(have)) ge[r] &= ~(0x80000000u >> __clz(equal));
-            --drop;
-          }
-          if (counted) {
+          if (kept >> (r0 + r * groups) & 1u) {               // a row that was left out may hold anything
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[i] = fma2(x[r][i], scale, s[i]);
+          }
+        }
+        // more logits equal the last one chosen than there are places: those of the highest columns give way
+        if (__any_sync(0xffffffffu, extra > 0.f && kept_of_sum)) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) c[e] += ge[r] >> e & 1u;
+          for (int r = 0; r < 4; ++r) {
+            int drop = static_cast<int>(of_four(kept_of_sum ? extra : 0.f, r, a.log2_group));
+            if (!__any_sync(0xffffffffu, drop > 0)) continue;
+            const T* row_here = reinterpret_cast<const T*>(here + (r0 + r * groups) * pitch) + (column ? t * 8 : 0);
+            unsigned equal = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) equal |= CeElem<T>::load(row_here + e) == kth[r] ? 1u << e : 0u;
+            if (!column) equal = 0;
+            do {
+              const unsigned have = __ballot_sync(0xffffffffu, equal != 0) >> (q << a.log2_group) & (group == 32 ? 0xffffffffu : (1u << group) - 1u);
+              if (drop > 0 && t == 31 - __clz(have)) {
+                const int last = 31 - __clz(equal);
+                equal &= ~(1u << last);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) c[i] = add2(c[i], f2(last == 2 * i ? -1.f : 0.f, last == 2 * i + 1 ? -1.f : 0.f));
+              }
+              --drop;
+            } while (__any_sync(0xffffffffu, drop > 0));
           }
         }
       }
@@ -523,9 +526,10 @@ balance_forward_tile_kernel(BalanceArgs a, int buffers, float* partial) {
   float* fold = reinterpret_cast<float*>(tile_shared);        // [warp][2 * 256 + 2]
   for (int o = group; o < 32; o <<= 1) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = add2(s[i], f2(__shfl_xor_sync(0xffffffffu, f2_lo(s[i]), o), __shfl_xor_sync(0xffffffffu, f2_hi(s[i]), o)));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) c[e] += __shfl_xor_sync(0xffffffffu, c[e], o);
+    for (int i = 0; i < 4; ++i) {
+      s[i] = add2(s[i], f2(__shfl_xor_sync(0xffffffffu, f2_lo(s[i]), o), __shfl_xor_sync(0xffffffffu, f2_hi(s[i]), o)));
+      c[i] = add2(c[i], f2(__shfl_xor_sync(0xffffffffu, f2_lo(c[i]), o), __shfl_xor_sync(0xffffffffu, f2_hi(c[i]), o)));
+    }
   }
   for (int o = 16; o > 0; o >>= 1) {
     z += __shfl_xor_sync(0xffffffffu, z, o);
@@ -536,7 +540,7 @@ balance_forward_tile_kernel(BalanceArgs a, int buffers, float* partial) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       mine[t * 8 + e] = e % 2 ? f2_hi(s[e / 2]) : f2_lo(s[e / 2]);
-      mine[256 + t * 8 + e] = __uint_as_float(static_cast<unsigned>(c[e]));
+      mine[256 + t * 8 + e] = __uint_as_float(static_cast<unsigned>(e % 2 ? f2_hi(c[e / 2]) : f2_lo(c[e / 2])));
     }
   }
   if (lane == 0) {
