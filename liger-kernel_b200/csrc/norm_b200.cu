@@ -129,11 +129,8 @@ int run_forward(const NormForwardArgs& a, const NormPlan& plan, unsigned walking
       if (plan.share == 2)
         return launch_with_shared<norm_forward_stream_kernel<T, W, kCentered, 2>>(grid, kStreamThreads, Stream<2, false>::kRingBytes, stream, a);
       return launch_with_shared<norm_forward_stream_kernel<T, W, kCentered, 4>>(grid, kStreamThreads, Stream<4, false>::kRingBytes, stream, a);
-    case kNormNarrow: {
-      const unsigned all = static_cast<unsigned>(ceil_div(a.n_rows, rows_per_round<false>(plan)));
-      FLCE_LAUNCH((norm_forward_narrow_kernel<T, W, kCentered>), all, kNarrowThreads, stream, a);
-      return FLCE_OK;
-    }
+    case kNormNarrow:
+      return launch_with_shared<norm_forward_narrow_kernel<T, W, kCentered>>(grid, kNarrowThreads, kNarrowRingBytes, stream, a);
     case kNormTiny: {
       const unsigned all = static_cast<unsigned>(ceil_div(a.n_rows, rows_per_round<false>(plan)));
       FLCE_LAUNCH((norm_forward_tiny_kernel<T, W, kCentered>), all, kNarrowThreads, stream, a);
@@ -160,8 +157,7 @@ int run_backward(const NormBackwardArgs& a, const NormPlan& plan, unsigned walki
         return launch_with_shared<norm_backward_stream_kernel<T, W, kCentered, 2>>(grid, kStreamThreads, Stream<2, true>::kRingBytes, stream, a);
       return launch_with_shared<norm_backward_stream_kernel<T, W, kCentered, 4>>(grid, kStreamThreads, Stream<4, true>::kRingBytes, stream, a);
     case kNormNarrow:
-      FLCE_LAUNCH((norm_backward_narrow_kernel<T, W, kCentered>), grid, kNarrowThreads, stream, a);
-      return FLCE_OK;
+      return launch_with_shared<norm_backward_narrow_kernel<T, W, kCentered>>(grid, kNarrowThreads, kNarrowRingBytes, stream, a);
     case kNormTiny:
       FLCE_LAUNCH((norm_backward_tiny_kernel<T, W, kCentered>), grid, kNarrowThreads, stream, a);
       return FLCE_OK;
