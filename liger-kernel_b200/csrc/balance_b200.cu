@@ -199,12 +199,16 @@ int flce_b200_balance_forward(const flce_balance_t* p, const void* const* logits
   const bool few = p->n_layers * blocks <= 32;
   if (!few) {
     const dim3 columns(static_cast<unsigned>(ceil_div(experts + 1, 32)), static_cast<unsigned>(p->n_layers));
-    FLCE_LAUNCH((balance_layer_kernel), columns, dim3(32, kBalFoldLanes), stream, partial, static_cast<int>(blocks), experts,
-                reinterpret_cast<long long*>(counts), sums, kept);
+    rc = launch_dependent<balance_layer_kernel>(columns, dim3(32, kBalFoldLanes), stream, static_cast<const float*>(partial),
+                                                static_cast<int>(blocks), experts, reinterpret_cast<long long*>(counts), sums, kept);
+    if (rc != FLCE_OK) return rc;
     ++launches;
   }
-  FLCE_LAUNCH((balance_total_kernel), 1u, kBalTotalThreads, stream, few ? partial : nullptr, static_cast<int>(blocks),
-              reinterpret_cast<long long*>(counts), sums, kept, static_cast<int>(p->n_layers), experts, p->lse_square_scale, loss, coef);
+  rc = launch_dependent<balance_total_kernel>(dim3(1), dim3(kBalTotalThreads), stream, static_cast<const float*>(few ? partial : nullptr),
+                                              static_cast<int>(blocks), reinterpret_cast<long long*>(counts), static_cast<const double*>(sums),
+                                              static_cast<const long long*>(kept), static_cast<int>(p->n_layers), experts,
+                                              p->lse_square_scale, loss, coef);
+  if (rc != FLCE_OK) return rc;
   FLCE_CUDA(cudaGetLastError());
   count_launches(launches);
   return FLCE_OK;

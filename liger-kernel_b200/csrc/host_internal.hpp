@@ -36,7 +36,27 @@ inline int element_size(int dtype) { return dtype == FLCE_FP32 ? 4 : 2; }
   emu::launch(emu_dim3(grid), emu_dim3(block), [&]() { (void)(stream), (kernel)(__VA_ARGS__); })
 #endif
 
-// The same for a kernel with `bytes` of dynamic shared memory; the permission for more than 48 KB is asked for once per kernel
+// A launch that may start while the kernel in front of it drains; the kernel calls wait_for_previous_kernel() first.
+template <auto kKernel, class... Args>
+int launch_dependent(dim3 grid, dim3 block, cudaStream_t stream, const Args&... args) {
+#ifndef FLCE_HOST_EMULATION
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.stream = stream;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  FLCE_CUDA(cudaLaunchKernelEx(&config, kKernel, args...));
+#else
+  FLCE_LAUNCH((kKernel), grid, block, stream, args...);
+#endif
+  return FLCE_OK;
+}
+
+// A launch with `bytes` of dynamic shared memory; the permission for more than 48 KB is asked for once per kernel
 // and device (kKernel names the instantiation).
 constexpr int kMostDynamicShared = 220 * 1024;      // beside what such a kernel declares statically: 227 KB in all
 template <auto kKernel, class... Args>

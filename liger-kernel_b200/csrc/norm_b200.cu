@@ -287,8 +287,9 @@ int flce_b200_norm_backward(const flce_norm_t* p, const void* grad_y, int64_t ld
     if (rc != FLCE_OK) return;
     if (parameters) {
       const dim3 columns(static_cast<unsigned>(ceil_div(p->hidden, 32)), centered ? 2 : 1);
-      FLCE_LAUNCH((norm_parameter_gradient_kernel<W>), columns, dim3(32, kNormReduceLanes), stream, 
-          a.dw_partial, a.db_partial, static_cast<int>(walking), a.hidden, static_cast<W*>(grad_weight), static_cast<W*>(grad_bias));
+      rc = launch_dependent<norm_parameter_gradient_kernel<W>>(
+          columns, dim3(32, kNormReduceLanes), stream, static_cast<const float*>(a.dw_partial), static_cast<const float*>(a.db_partial),
+          static_cast<int>(walking), a.hidden, static_cast<W*>(grad_weight), static_cast<W*>(grad_bias));
     }
   });
   if (rc != FLCE_OK) return rc;

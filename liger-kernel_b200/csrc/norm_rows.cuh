@@ -299,6 +299,7 @@ norm_forward_stream_kernel(NormForwardArgs a) {
 template <typename T, typename W, bool kCentered, int kUnits>
 __global__ void __launch_bounds__(kStreamThreads, 1)
 norm_backward_stream_kernel(NormBackwardArgs a) {
+  allow_dependents();      // the small kernel that adds up the partial sums
   constexpr int kRows = Stream<kUnits, true>::kRows, kSlots = Stream<kUnits, true>::kSlots;
   constexpr int kVec = CeElem<T>::kVec;
   constexpr int kPairs = kVec / 2;
@@ -598,6 +599,7 @@ norm_forward_narrow_kernel(NormForwardArgs a) {
 template <typename T, typename W, bool kCentered>
 __global__ void __launch_bounds__(kNarrowThreads, kNarrowBlocksPerSm)
 norm_backward_narrow_kernel(NormBackwardArgs a) {
+  allow_dependents();      // the small kernel that adds up the partial sums
   constexpr int kRows = kNarrowBackwardRows;
   constexpr int kVec = CeElem<T>::kVec;
   constexpr int kPairs = kVec / 2;
@@ -910,6 +912,7 @@ norm_forward_window_kernel(NormForwardArgs a) {
 template <typename T, typename W, bool kCentered, int kEpt>
 __global__ void __launch_bounds__(kWindowThreads, 1)
 norm_backward_window_kernel(NormBackwardArgs a) {
+  allow_dependents();      // the small kernel that adds up the partial sums
   typedef Window<T, kEpt, true> Shape;
   constexpr int kRows = Shape::kRows, kSlots = Shape::kSlots, kPairs = kEpt / 2;
   FLCE_DYNAMIC_SHARED(uint4, stream_ring);                    // [slot][row][x, dy][warp][piece]; at the end: the groups' sums
@@ -1086,6 +1089,7 @@ norm_forward_tiny_kernel(NormForwardArgs a) {
 template <typename T, typename W, bool kCentered>
 __global__ void __launch_bounds__(kNarrowThreads)
 norm_backward_tiny_kernel(NormBackwardArgs a) {
+  allow_dependents();      // the small kernel that adds up the partial sums
   constexpr int kRows = kNarrowBackwardRows;
   __shared__ float fold[kNarrowThreads];
   const int group = 1 << a.log2_group;
@@ -1146,13 +1150,14 @@ template <typename W>
 __global__ void __launch_bounds__(32 * kNormReduceLanes)
 norm_parameter_gradient_kernel(const float* dw_partial, const float* db_partial, int blocks, int hidden, W* dw, W* db) {
   __shared__ float part[kNormReduceLanes][33];
+  wait_for_previous_kernel();
   const float* partial = blockIdx.y == 0 ? dw_partial : db_partial;
   W* out = blockIdx.y == 0 ? dw : db;
   if (out == nullptr) return;
   const int col = static_cast<int>(blockIdx.x) * 32 + static_cast<int>(threadIdx.x);
   float s = 0.f;
   if (col < hidden) {
-#pragma unroll 4
+#pragma unroll 8
     for (int b = static_cast<int>(threadIdx.y); b < blocks; b += kNormReduceLanes) s += partial[static_cast<size_t>(b) * hidden + col];
   }
   part[threadIdx.y][threadIdx.x] = s;
@@ -1244,6 +1249,7 @@ norm_backward_long_kernel(NormBackwardArgs a) {
 template <typename T, bool kCentered>
 __global__ void __launch_bounds__(kNormColumnThreads)
 norm_parameter_partial_long_kernel(NormBackwardArgs a) {
+  allow_dependents();      // the small kernel that adds up the partial sums
   const int c = static_cast<int>(blockIdx.x * blockDim.x + threadIdx.x);
   if (c >= a.hidden) return;
   const T* x = static_cast<const T*>(a.x);

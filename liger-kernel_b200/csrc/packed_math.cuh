@@ -119,6 +119,20 @@ __device__ __forceinline__ void async_wait() {
 #endif
 }
 
+// Programmatic dependent launch.  A kernel launched as a dependent may start before the kernel in front of it on the stream has
+// ended (when all of that kernel's blocks have called allow_dependents or returned) and must wait before it touches anything
+// that kernel, or one before it, reads or writes.
+__device__ __forceinline__ void wait_for_previous_kernel() {
+#ifndef FLCE_HOST_EMULATION
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+#endif
+}
+__device__ __forceinline__ void allow_dependents() {
+#ifndef FLCE_HOST_EMULATION
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+#endif
+}
+
 __device__ __forceinline__ void warp_sync() {
 #ifdef FLCE_HOST_EMULATION
   emu_warp_sync();

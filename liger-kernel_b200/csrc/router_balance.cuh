@@ -160,6 +160,7 @@ __host__ __device__ inline long long balance_partial_words(int experts) { return
 template <typename T, bool kVectors, int kEpt>
 __global__ void __launch_bounds__(kBalThreads)
 balance_forward_kernel(BalanceArgs a, float* partial) {
+  allow_dependents();      // the small kernels that add up the partial sums
   __shared__ float fold_s[kBalWarps][32 * kEpt];      // taken twice: for S, then for C
   __shared__ float fold_z[kBalWarps];
   __shared__ int fold_n[kBalWarps];
@@ -347,6 +348,7 @@ constexpr int kTileMaxWarps = 16;
 template <typename T>
 __global__ void __launch_bounds__(kTileMaxWarps * 32, 1)
 balance_forward_tile_kernel(BalanceArgs a, int buffers, float* partial) {
+  allow_dependents();      // the small kernels that add up the partial sums
   typedef TileWord<T> Tile;
   typedef typename Tile::Word Word;
   constexpr int kVec = CeElem<T>::kVec;
@@ -569,6 +571,8 @@ __global__ void __launch_bounds__(32 * kBalFoldLanes)
 balance_layer_kernel(const float* partial, int blocks, int experts, long long* counts, double* sums, long long* kept) {
   __shared__ double part_s[kBalFoldLanes][32];
   __shared__ long long part_c[kBalFoldLanes][32];
+  allow_dependents();
+  wait_for_previous_kernel();
   const long long layer = blockIdx.y;
   const int e = static_cast<int>(blockIdx.x * 32 + threadIdx.x);
   double s = 0.0;
@@ -604,6 +608,7 @@ balance_total_kernel(const float* partial, int blocks, long long* counts, const 
                      float lambda, float* out, float* coef) {
   __shared__ double scratch[4][kBalTotalThreads / 32];
   __shared__ double part_c[kBalTotalThreads], part_s[kBalTotalThreads];
+  wait_for_previous_kernel();
   const int tid = static_cast<int>(threadIdx.x);
   const long long words = balance_partial_words(experts);
   int wide = 32;
