@@ -19,6 +19,7 @@ import torch
 from transformers.modeling_outputs import CausalLMOutputWithPast, MoeCausalLMOutputWithPast
 
 from ..fsdp import run_inside_fsdp_forward
+from ..functional import liger_load_balancing_loss
 from .loss_utils import LigerForCausalLMLoss, unpack_cross_entropy_result
 
 
@@ -144,9 +145,23 @@ def _make_lce_forward(softcap_from_config: bool = False, moe_balancing_loss=None
 
 
 def _mixtral_balancing_loss():
+    return router_balancing_loss
+
+
+def router_balancing_loss(router_logits, num_experts, top_k, attention_mask=None):
+    """The router's auxiliary loss of the mixture-of-experts families: ``liger_load_balancing_loss`` for router logits on the GPU,
+    the model library's own function for what that does not cover (logits on the CPU, masks that are not one element per
+    token, more than 1024 experts)."""
+    if isinstance(router_logits, (tuple, list)) and len(router_logits) > 0 and num_experts <= 1024:
+        head = router_logits[0]
+        tokens = head.numel() // num_experts
+        one_per_token = attention_mask is None or (attention_mask.dim() == 2 and attention_mask.numel() == tokens)
+        if head.is_cuda and head.dtype in (torch.bfloat16, torch.float16, torch.float32) and one_per_token:
+            # layers of a model that is spread over devices meet on the first one, as in the library's function
+            return liger_load_balancing_loss(tuple(t.to(head.device) for t in router_logits), num_experts, top_k, attention_mask)
     from transformers.models.mixtral.modeling_mixtral import load_balancing_loss_func
 
-    return load_balancing_loss_func
+    return load_balancing_loss_func(router_logits, num_experts, top_k, attention_mask)
 
 
 dense_lce_forward = _make_lce_forward()

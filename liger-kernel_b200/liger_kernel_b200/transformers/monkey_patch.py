@@ -8,8 +8,9 @@ wrappers and hybrid state-space models are not.
 
 The ``fused_linear_cross_entropy`` switch and the ``cross_entropy`` switch (logits kept, loss through the
 stand-alone cross-entropy operator) are implemented by this package; the other flags (rope, rms_norm,
-swiglu / geglu, layer_norm, relu_squared) belong to kernels outside this package and are accepted so existing
-call sites keep working: when set they are reported once and otherwise ignored.
+swiglu / geglu, layer_norm, relu_squared) are accepted so existing call sites keep working: when set they are reported once
+and otherwise ignored.  (Layer norm and RMSNorm exist as operators and modules; a model's norms are not switched to them
+here.)  The router's load-balancing loss of the mixture-of-experts forwards runs on this package's operator.
 
 ``install()`` additionally rebinds the operator symbol inside an installed ``liger_kernel`` so that
 code which imports Liger directly (e.g. ``Trainer(use_liger_kernel=True)``) reaches this
@@ -199,6 +200,10 @@ _INSTALL_SITES = {
     "LigerFusedLinearJSDFunction": (
         "liger_kernel.ops", "liger_kernel.transformers.functional", "liger_kernel.transformers.fused_linear_jsd"),
     "LigerFusedLinearScaledCrossEntropyFunction": ("liger_kernel.ops",),
+    "LigerLayerNormFunction": (
+        "liger_kernel.ops", "liger_kernel.transformers.functional", "liger_kernel.transformers.layer_norm"),
+    "LigerRMSNormFunction": (
+        "liger_kernel.ops", "liger_kernel.transformers.functional", "liger_kernel.transformers.rms_norm"),
 }
 
 
@@ -228,16 +233,17 @@ def _install_preference_losses() -> bool:
 
 
 def install(cross_entropy: bool = False, fused_linear_jsd: bool = False, fused_linear_scaled_cross_entropy: bool = False,
-            chunked_loss: bool = False) -> bool:
+            chunked_loss: bool = False, layer_norm: bool = False, rms_norm: bool = False) -> bool:
     """Rebind ``LigerFusedLinearCrossEntropyFunction`` inside an importable ``liger_kernel`` package
     at the three places that bind it at import time (``liger_kernel.ops``,
     ``liger_kernel.transformers.functional``, ``liger_kernel.transformers.fused_linear_cross_entropy``), and on request
-    the stand-alone cross-entropy, fused linear JSD and fused linear scaled cross-entropy operators at theirs;
+    the stand-alone cross-entropy, fused linear JSD, fused linear scaled cross-entropy, layer norm and RMSNorm operators at theirs;
     ``chunked_loss=True`` also rebinds the DPO / ORPO / SimPO / CPO / KTO / GRPO / JSD / cosine-similarity classes of ``liger_kernel.chunked_loss``.
     Returns False when no ``liger_kernel`` is installed."""
     from ..ops.cross_entropy import LigerCrossEntropyFunction
     from ..ops.fused_linear_jsd import LigerFusedLinearJSDFunction
     from ..ops.fused_linear_scaled_cross_entropy import LigerFusedLinearScaledCrossEntropyFunction
+    from ..ops.norm import LigerLayerNormFunction, LigerRMSNormFunction
 
     wanted = {"LigerFusedLinearCrossEntropyFunction": LigerFusedLinearCrossEntropyFunction}
     if cross_entropy:
@@ -246,6 +252,10 @@ def install(cross_entropy: bool = False, fused_linear_jsd: bool = False, fused_l
         wanted["LigerFusedLinearJSDFunction"] = LigerFusedLinearJSDFunction
     if fused_linear_scaled_cross_entropy:
         wanted["LigerFusedLinearScaledCrossEntropyFunction"] = LigerFusedLinearScaledCrossEntropyFunction
+    if layer_norm:
+        wanted["LigerLayerNormFunction"] = LigerLayerNormFunction
+    if rms_norm:
+        wanted["LigerRMSNormFunction"] = LigerRMSNormFunction
     try:
         modules = {name: importlib.import_module(name) for symbol in wanted for name in _INSTALL_SITES[symbol]}
     except ImportError:

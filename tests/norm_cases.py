@@ -174,6 +174,12 @@ def case_shapes_and_views(device):
         w.grad = None
         fn(frozen, w).sum().backward()
         assert w.grad is not None
+        row = torch.randn(16, generator=g).to(device).requires_grad_(True)       # one row seen as five
+        fn(row.expand(5, 16), w.detach()).square().sum().backward()
+        five = row.detach().repeat(5, 1).requires_grad_(True)
+        fn(five, w.detach()).square().sum().backward()
+        assert float((row.grad - five.grad.sum(0)).abs().max()) <= 8 * U * float(five.grad.abs().sum(0).max())
+        assert torch.equal(fn(row.detach(), w.detach()), fn(row.detach()[None], w.detach())[0])
     same = torch.randn(3, 16, generator=g).to(device)
     assert torch.equal(lk.liger_layer_norm(torch.full((2, 8), 5.0, device=device), None, None, 1e-6), torch.zeros(2, 8, device=device))
     layer, rms = lk.LigerLayerNorm(16, bias=True).to(device), lk.LigerRMSNorm(16, offset=1.0, init_fn="zeros").to(device)
