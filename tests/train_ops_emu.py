@@ -25,11 +25,13 @@ def load():
     sources = _SOURCES + [os.path.join(_CSRC, f) for f in os.listdir(_CSRC)]
     if not os.path.exists(_OUT) or any(os.path.getmtime(s) > os.path.getmtime(_OUT) for s in sources):
         os.makedirs(os.path.dirname(_OUT), exist_ok=True)
+        fresh = f"{_OUT}.{os.getpid()}"            # put in place whole: tests may run in several processes
         cmd = ["g++", "-x", "c++", "-std=c++20", "-O1", "-w", "-fPIC", "-shared", "-I", _CUDA_INCLUDE, "-I", _CSRC,
-               "-I", os.path.join(_ROOT, "include"), "-o", _OUT, _SOURCES[0]]
+               "-I", os.path.join(_ROOT, "include"), "-o", fresh, _SOURCES[0]]
         done = subprocess.run(cmd, capture_output=True, text=True)
         if done.returncode != 0:
             raise RuntimeError("building the emulation failed:\n" + done.stderr[-4000:])
+        os.replace(fresh, _OUT)
     lib = C.CDLL(_OUT)
     for name in real.EXPORTS:
         if hasattr(lib, name):
