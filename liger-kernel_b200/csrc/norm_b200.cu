@@ -92,7 +92,13 @@ int rows_per_round(const NormPlan& plan) {
   }
 }
 int blocks_per_sm(const NormPlan& plan) {
-  return plan.path == kNormStream || plan.path == kNormWindow ? 1 : (plan.path == kNormLong ? 2 : 4);
+  switch (plan.path) {
+    case kNormStream:
+    case kNormWindow: return 1;
+    case kNormNarrow: return kNarrowBlocksPerSm;
+    case kNormLong: return 2;
+    default: return 4;
+  }
 }
 
 // Blocks that walk over the rows: as many as are resident together.  Those of the backward kernel leave `hidden` partial sums

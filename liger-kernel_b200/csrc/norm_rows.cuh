@@ -479,13 +479,14 @@ norm_backward_stream_kernel(NormBackwardArgs a) {
 
 // ---- rows of at most 32 aligned 16-byte vectors: one vector per lane, several rows to a warp, kRows of them per thread in a round,
 // no barrier at all.  Groups of 4 to 32 lanes.  The rounds ahead are in a ring as above: with the rows of the round loaded into
-// registers, 262144 x 128 bf16 took 29 us forward and 56 us backward.
+// registers, 262144 x 128 bf16 took 29 us forward and 56 us backward; now 25 and 41 us with three blocks per SM, 27 and 49 us with
+// four, whose registers do not hold it all.
 
 constexpr int kNarrowThreads = 256;
 constexpr int kNarrowForwardRows = 4, kNarrowBackwardRows = 2;      // four sums either way
 constexpr int kNarrowSlots = 3;
-constexpr int kNarrowRingBytes = kNarrowSlots * 4 * kNarrowThreads * 16;      // 48 KB: four blocks per SM
-constexpr int kNarrowBlocksPerSm = 4;
+constexpr int kNarrowRingBytes = kNarrowSlots * 4 * kNarrowThreads * 16;      // 48 KB
+constexpr int kNarrowBlocksPerSm = 3;
 
 template <typename T, typename W, bool kCentered>
 __global__ void __launch_bounds__(kNarrowThreads, kNarrowBlocksPerSm)
