@@ -33,6 +33,7 @@ enum NormPath { kNormStream, kNormNarrow, kNormWindow, kNormTiny, kNormLong };
 struct NormPlan {
   NormPath path;
   int share, log2_group, warps;
+  bool few;       // stream, forward: a row per group and round
 };
 
 int log2_group_for(long long pieces, int smallest) {
@@ -45,16 +46,17 @@ int log2_group_for(long long pieces, int smallest) {
 // Window: of 2, 4, 8 and 16 elements per lane the cheapest, taking a warp's part of a row to cost 8 elements beside those it
 // holds: 50000 x 300 bf16 forward 45, 33, 29 and 23 us, 10007 x 1537 fp16 43, 31 and 27 us from 4 on, 100000 x 100 bf16 45, 25,
 // 33 and 47 us.  Long: what is left, above 8192 elements.
-NormPlan norm_plan(const flce_norm_t* p, bool vectors) {
+NormPlan norm_plan(const flce_norm_t* p, bool vectors, int sm_count) {
   const long long n = p->hidden * element_size(p->dtype) / 16;
-  if (vectors && n <= 32) return {kNormNarrow, 1, log2_group_for(n, 2), 0};
+  if (vectors && n <= 32) return {kNormNarrow, 1, log2_group_for(n, 2), 0, false};
   if (vectors && n <= 4 * kStreamThreads) {
     const int share = n <= 2 * kStreamThreads ? 2 : 4;
     const int log2_group = log2_group_for(ceil_div(n, share), 5);
-    return {kNormStream, share, log2_group, 1 << (log2_group - 5)};
+    const bool few = share == 2 && p->n_rows <= (static_cast<long long>(sm_count) * kStreamThreads >> log2_group);
+    return {kNormStream, share, log2_group, 1 << (log2_group - 5), few};
   }
-  if (p->hidden <= 32) return {kNormTiny, 1, log2_group_for(p->hidden, 2), 0};
-  NormPlan best{kNormLong, 0, 9, kNormMaxWarps};
+  if (p->hidden <= 32) return {kNormTiny, 1, log2_group_for(p->hidden, 2), 0, false};
+  NormPlan best{kNormLong, 0, 9, kNormMaxWarps, false};
   double least = 0.0;
   for (int share = 2; share <= 16; share *= 2) {
     const long long warps = ceil_div(p->hidden, 32 * share);
@@ -62,7 +64,7 @@ NormPlan norm_plan(const flce_norm_t* p, bool vectors) {
     const double cost = (share + 8.0) / static_cast<double>(kWindowWarps / warps);
     if (best.path == kNormLong || cost < least) {
       least = cost;
-      best = {kNormWindow, share, 0, static_cast<int>(warps)};
+      best = {kNormWindow, share, 0, static_cast<int>(warps), false};
     }
   }
   return best;
@@ -85,7 +87,7 @@ int rows_per_round(const NormPlan& plan) {
   switch (plan.path) {
     case kNormNarrow:
     case kNormTiny: return (kNarrowThreads >> plan.log2_group) * (kGrad ? kNarrowBackwardRows : kNarrowForwardRows);
-    case kNormStream: return (kStreamThreads >> plan.log2_group) * (plan.share == 2 ? Stream<2, kGrad>::kRows : Stream<4, kGrad>::kRows);
+    case kNormStream: return (kStreamThreads >> plan.log2_group) * (!kGrad && plan.few ? 1 : (plan.share == 2 ? Stream<2, kGrad>::kRows : Stream<4, kGrad>::kRows));
     case kNormWindow:
       return kWindowWarps / plan.warps * with_share(plan.share, [](auto e) { return Window<float, decltype(e)::value, kGrad>::kRows; });
     default: return 1;
@@ -132,9 +134,11 @@ int run_forward(const NormForwardArgs& a, const NormPlan& plan, unsigned walking
   const dim3 grid(walking);
   switch (plan.path) {
     case kNormStream:
+      if (plan.share == 2 && plan.few)
+        return launch_with_shared<norm_forward_stream_kernel<T, W, kCentered, 2, true>>(grid, kStreamThreads, Stream<2, false, true>::kRingBytes, stream, a);
       if (plan.share == 2)
-        return launch_with_shared<norm_forward_stream_kernel<T, W, kCentered, 2>>(grid, kStreamThreads, Stream<2, false>::kRingBytes, stream, a);
-      return launch_with_shared<norm_forward_stream_kernel<T, W, kCentered, 4>>(grid, kStreamThreads, Stream<4, false>::kRingBytes, stream, a);
+        return launch_with_shared<norm_forward_stream_kernel<T, W, kCentered, 2, false>>(grid, kStreamThreads, Stream<2, false>::kRingBytes, stream, a);
+      return launch_with_shared<norm_forward_stream_kernel<T, W, kCentered, 4, false>>(grid, kStreamThreads, Stream<4, false>::kRingBytes, stream, a);
     case kNormNarrow:
       return launch_with_shared<norm_forward_narrow_kernel<T, W, kCentered>>(grid, kNarrowThreads, kNarrowRingBytes, stream, a);
     case kNormTiny: {
@@ -212,7 +216,7 @@ int flce_b200_norm_forward(const flce_norm_t* p, void* y, float* mean, float* rs
   a.eps = p->eps;
   a.offset = p->offset;
   a.round_xhat = p->round_xhat;
-  const NormPlan plan = norm_plan(p, whole_vectors(p, y, p->hidden));
+  const NormPlan plan = norm_plan(p, whole_vectors(p, y, p->hidden), sms);
   a.log2_group = plan.log2_group;
   a.group_warps = plan.warps;
   const unsigned walking = static_cast<unsigned>(walking_blocks<false>(p, plan, sms));
@@ -232,8 +236,8 @@ size_t flce_b200_norm_workspace_bytes(const flce_norm_t* p) {
   int sms = 0;
   if (current_sm_count(&sms) != FLCE_OK) return 0;
   // the row's spread may turn out either way (the gradient's alignment is not known yet): room for the larger grid
-  const long long blocks_vec = walking_blocks<true>(p, norm_plan(p, true), sms);
-  const long long blocks_one = walking_blocks<true>(p, norm_plan(p, false), sms);
+  const long long blocks_vec = walking_blocks<true>(p, norm_plan(p, true, sms), sms);
+  const long long blocks_one = walking_blocks<true>(p, norm_plan(p, false, sms), sms);
   const long long blocks = blocks_vec > blocks_one ? blocks_vec : blocks_one;
   return static_cast<size_t>(blocks) * static_cast<size_t>(p->hidden) * sizeof(float) * (p->kind == FLCE_LAYER_NORM ? 2 : 1);
 }
@@ -259,7 +263,7 @@ int flce_b200_norm_backward(const flce_norm_t* p, const void* grad_y, int64_t ld
   int sms = 0;
   rc = current_sm_count(&sms);
   if (rc != FLCE_OK) return rc;
-  const NormPlan plan = norm_plan(p, whole_vectors(p, grad_y, ld_grad) && aligned16(grad_x));
+  const NormPlan plan = norm_plan(p, whole_vectors(p, grad_y, ld_grad) && aligned16(grad_x), sms);
   const long long blocks = walking_blocks<true>(p, plan, sms);
   const bool parameters = grad_weight != nullptr || grad_bias != nullptr;
   const size_t plane = static_cast<size_t>(blocks) * static_cast<size_t>(p->hidden);

@@ -23,6 +23,15 @@ def test_matches_definition(kind, n, hidden, dtype, wdtype, pitch):
         cases.case_matches_definition("cpu", kind, n, hidden, dtype, wdtype, True, True, 0.0, pitch)
 
 
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("n,hidden,dtype,wdtype,pitch", [
+    (101, 264, BF16, BF16, 16), (57, 520, FP16, FP32, 0), (27, 1024, FP32, FP32, 4), (11, 4104, BF16, BF16, 0), (7, 8200, FP16, FP16, 0),
+    (300, 40, BF16, BF16, 0), (90, 33, FP16, FP16, 0), (31, 513, BF16, FP32, 1), (200, 12, BF16, BF16, 1)])
+def test_more_rows_than_a_round_takes(kind, n, hidden, dtype, wdtype, pitch):
+    with train_ops_emu.installed():
+        cases.case_matches_definition("cpu", kind, n, hidden, dtype, wdtype, True, True, 0.0, pitch)
+
+
 @pytest.mark.parametrize("kind,weight,bias,offset,mode", [
     ("layer", True, False, 1.0, "gemma"), ("layer", False, False, 0.0, "gemma"), ("layer", False, True, 0.0, "gemma"),
     ("rms", True, False, 1.0, "llama"), ("rms", False, False, 0.0, "llama"), ("rms", True, False, 1.0, "gemma")])
