@@ -173,11 +173,19 @@ def case_gradient_against_differences(device):
 def case_nan_reaches_the_loss(device):
     import liger_kernel_b200 as lk
 
-    x = make(1, 12, 16, torch.bfloat16)
-    x[0, 3, 2] = float("nan")
-    t = x[0].to(device).requires_grad_(True)
-    loss = lk.liger_load_balancing_loss(t, 16, 4)
-    assert math.isnan(float(loss.detach()))
+    for experts in (16, 64):
+        for bad in (float("nan"), float("inf")):              # softmax of an infinite logit is inf / inf
+            x = make(1, 12, experts, torch.bfloat16)
+            x[0, 3, 2] = bad
+            t = x[0].to(device).requires_grad_(True)
+            loss = lk.liger_load_balancing_loss(t, experts, 4)
+            assert math.isnan(float(loss.detach()))
+            (grad,) = torch.autograd.grad(loss, (t,))
+            assert bool(torch.isnan(grad[3]).any())
+            # the same row left out: nothing of it shows
+            mask = torch.ones(12, dtype=torch.int64)
+            mask[3] = 0
+            case_matches_definition(device, make(1, 12, experts, torch.bfloat16), 4, mask=mask.tolist())
 
 
 def case_refusals(device):
