@@ -34,6 +34,7 @@ struct NormPlan {
   NormPath path;
   int share, log2_group, warps;
   bool few;       // stream, forward: a row per group and round
+  bool wide;      // fp32 rows
 };
 
 int log2_group_for(long long pieces, int smallest) {
@@ -47,16 +48,17 @@ int log2_group_for(long long pieces, int smallest) {
 // holds: 50000 x 300 bf16 forward 45, 33, 29 and 23 us, 10007 x 1537 fp16 43, 31 and 27 us from 4 on, 100000 x 100 bf16 45, 25,
 // 33 and 47 us.  Long: what is left, above 8192 elements.
 NormPlan norm_plan(const flce_norm_t* p, bool vectors, int sm_count) {
+  const bool wide = p->dtype == FLCE_FP32;
   const long long n = p->hidden * element_size(p->dtype) / 16;
-  if (vectors && n <= 32) return {kNormNarrow, 1, log2_group_for(n, 2), 0, false};
+  if (vectors && n <= 32) return {kNormNarrow, 1, log2_group_for(n, 2), 0, false, wide};
   if (vectors && n <= 4 * kStreamThreads) {
     const int share = n <= 2 * kStreamThreads ? 2 : 4;
     const int log2_group = log2_group_for(ceil_div(n, share), 5);
     const bool few = share == 2 && p->n_rows <= (static_cast<long long>(sm_count) * kStreamThreads >> log2_group);
-    return {kNormStream, share, log2_group, 1 << (log2_group - 5), few};
+    return {kNormStream, share, log2_group, 1 << (log2_group - 5), few, wide};
   }
-  if (p->hidden <= 32) return {kNormTiny, 1, log2_group_for(p->hidden, 2), 0, false};
-  NormPlan best{kNormLong, 0, 9, kNormMaxWarps, false};
+  if (p->hidden <= 32) return {kNormTiny, 1, log2_group_for(p->hidden, 2), 0, false, wide};
+  NormPlan best{kNormLong, 0, 9, kNormMaxWarps, false, wide};
   double least = 0.0;
   for (int share = 2; share <= 16; share *= 2) {
     const long long warps = ceil_div(p->hidden, 32 * share);
@@ -64,7 +66,7 @@ NormPlan norm_plan(const flce_norm_t* p, bool vectors, int sm_count) {
     const double cost = (share + 8.0) / static_cast<double>(kWindowWarps / warps);
     if (best.path == kNormLong || cost < least) {
       least = cost;
-      best = {kNormWindow, share, 0, static_cast<int>(warps), false};
+      best = {kNormWindow, share, 0, static_cast<int>(warps), false, wide};
     }
   }
   return best;
@@ -89,7 +91,10 @@ int rows_per_round(const NormPlan& plan) {
     case kNormTiny: return (kNarrowThreads >> plan.log2_group) * (kGrad ? kNarrowBackwardRows : kNarrowForwardRows);
     case kNormStream: return (kStreamThreads >> plan.log2_group) * (!kGrad && plan.few ? 1 : (plan.share == 2 ? Stream<2, kGrad>::kRows : Stream<4, kGrad>::kRows));
     case kNormWindow:
-      return kWindowWarps / plan.warps * with_share(plan.share, [](auto e) { return Window<float, decltype(e)::value, kGrad>::kRows; });
+      return kWindowWarps / plan.warps * with_share(plan.share, [&](auto e) {
+               constexpr int kEpt = decltype(e)::value;
+               return plan.wide ? Window<float, kEpt, kGrad>::kRows : Window<__half, kEpt, kGrad>::kRows;
+             });
     default: return 1;
   }
 }
@@ -149,7 +154,7 @@ int run_forward(const NormForwardArgs& a, const NormPlan& plan, unsigned walking
     case kNormWindow:
       return with_share(plan.share, [&](auto e) {
         constexpr int kEpt = decltype(e)::value;
-        return launch_with_shared<norm_forward_window_kernel<T, W, kCentered, kEpt>>(grid, kWindowThreads, Window<T, kEpt, false>::kRingBytes,
+        return launch_with_shared<norm_forward_window_kernel<T, W, kCentered, kEpt>>(grid, kWindowThreads, Window<T, kEpt, false>::kBytes,
                                                                                     stream, a);
       });
     default:
@@ -174,7 +179,7 @@ int run_backward(const NormBackwardArgs& a, const NormPlan& plan, unsigned walki
     case kNormWindow:
       return with_share(plan.share, [&](auto e) {
         constexpr int kEpt = decltype(e)::value;
-        return launch_with_shared<norm_backward_window_kernel<T, W, kCentered, kEpt>>(grid, kWindowThreads, Window<T, kEpt, true>::kRingBytes,
+        return launch_with_shared<norm_backward_window_kernel<T, W, kCentered, kEpt>>(grid, kWindowThreads, Window<T, kEpt, true>::kBytes,
                                                                                      stream, a);
       });
     default:

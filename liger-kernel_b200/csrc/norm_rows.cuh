@@ -96,6 +96,44 @@ __device__ __forceinline__ float norm_warps_four_sums(const float (&v)[4], int w
   for (int w = lane & 7; w < warps; w += 8) sum += of[w * 4];
   return low_lane_sum(sum, 8);
 }
+// Rows whose warps have centred their parts on the parts' own means meet: `sum` and `square` of this warp's part of row lane >> 3
+// become the mean and the sum (x - mean)^2 of the whole row.  Warp w holds part_elements(w) of the row's elements.
+struct NormPartScratch {
+  float sums[kNormMaxWarps * 4], squares[kNormMaxWarps * 4];
+};
+template <bool kCentered, class PartElements>
+__device__ __forceinline__ void norm_meet(float& sum, float& square, int warps, int g, NormPartScratch (&scratch)[2], int& phase,
+                                          float inv_hidden, float part_inv, PartElements part_elements) {
+  if (warps == 1) {
+    sum *= part_inv;
+    return;
+  }
+  const int lane = static_cast<int>(threadIdx.x) & 31;
+  NormPartScratch& buf = scratch[phase];
+  phase ^= 1;                               // taken in turn, as above
+  if ((lane & 7) == 0) {
+    buf.squares[(threadIdx.x >> 5) * 4 + (lane >> 3)] = square;
+    if (kCentered) buf.sums[(threadIdx.x >> 5) * 4 + (lane >> 3)] = sum;
+  }
+  named_barrier(1 + g, warps * 32);
+  // eight lanes add up a row's parts
+  const int of = g * warps * 4 + (lane >> 3);
+  square = 0.f;
+  if constexpr (kCentered) {
+    sum = 0.f;
+    for (int w = lane & 7; w < warps; w += 8) sum += buf.sums[of + w * 4];
+    sum = low_lane_sum(sum, 8) * inv_hidden;
+    for (int w = lane & 7; w < warps; w += 8) {
+      const float n = part_elements(w);
+      const float off = n > 0.f ? buf.sums[of + w * 4] / n - sum : 0.f;
+      square += fmaf(n * off, off, buf.squares[of + w * 4]);
+    }
+  } else {
+    for (int w = lane & 7; w < warps; w += 8) square += buf.squares[of + w * 4];
+  }
+  square = low_lane_sum(square, 8);
+}
+
 // sum number i of those, from a lane of the warp that holds it
 __device__ __forceinline__ float norm_warp_of_four(float sums, int i) { return __shfl_sync(0xffffffffu, sums, i * 8); }
 
@@ -148,8 +186,7 @@ norm_forward_stream_kernel(NormForwardArgs a) {
   constexpr int kPairs = kVec / 2;
   constexpr int kWVecs = kVec * static_cast<int>(sizeof(W)) / 16;
   FLCE_DYNAMIC_SHARED(uint4, stream_ring);                    // [slot][row][unit][thread]
-  __shared__ float scratch[2][kNormMaxWarps * 4];
-  __shared__ float scratch_sums[2][kCentered ? kNormMaxWarps * 4 : 1];
+  __shared__ NormPartScratch scratch[2];
   const int group = 1 << a.log2_group;
   const int warps = group >> 5;
   const int groups = kStreamThreads >> a.log2_group;
@@ -229,32 +266,8 @@ norm_forward_stream_kernel(NormForwardArgs a) {
       v[r] = f2_lo(acc) + f2_hi(acc);
     }
     float square = lane_four_sums(v, 32);
-    float mean = part_sum * part_inv;       // of row lane >> 3, once the parts have met
-    if (warps > 1) {
-      float *buf = scratch[phase], *buf_sums = scratch_sums[kCentered ? phase : 0];
-      phase ^= 1;                           // taken in turn: see norm_warps_four_sums
-      if ((lane & 7) == 0) {
-        buf[(threadIdx.x >> 5) * 4 + (lane >> 3)] = square;
-        if (kCentered) buf_sums[(threadIdx.x >> 5) * 4 + (lane >> 3)] = part_sum;
-      }
-      named_barrier(1 + g, group);
-      // eight lanes add up a row's parts
-      const int of = g * warps * 4 + (lane >> 3);
-      square = 0.f;
-      if constexpr (kCentered) {
-        float sum = 0.f;
-        for (int w = lane & 7; w < warps; w += 8) sum += buf_sums[of + w * 4];
-        mean = low_lane_sum(sum, 8) * inv;
-        for (int w = lane & 7; w < warps; w += 8) {
-          const float n = part_elements(w);
-          const float off = n > 0.f ? buf_sums[of + w * 4] / n - mean : 0.f;
-          square += fmaf(n * off, off, buf[of + w * 4]);
-        }
-      } else {
-        for (int w = lane & 7; w < warps; w += 8) square += buf[of + w * 4];
-      }
-      square = low_lane_sum(square, 8);
-    }
+    norm_meet<kCentered>(part_sum, square, warps, g, scratch, phase, inv, part_inv, part_elements);
+    const float mean = part_sum;            // of row lane >> 3
     const float rstd = norm_rsqrt(fmaf(square, inv, a.eps));
 #pragma unroll
     for (int r = 0; r < kRows; ++r) minus_mean[r] = both(kCentered ? -__shfl_sync(0xffffffffu, mean, r * 8) : 0.f);
@@ -755,14 +768,19 @@ norm_backward_narrow_kernel(NormBackwardArgs a) {
 // backward.  A part is 32 * kEpt columns, a row `warps` parts, as many rows side by side as the block's 16 warps hold.
 constexpr int kWindowThreads = 512;
 constexpr int kWindowWarps = kWindowThreads / 32;
+// What a round costs beside its elements (asking for the pieces, sums, barrier) is most of it, so it takes as many rows as registers
+// and shared memory hold; the parameters are read from shared memory, once per round, for that.
 template <typename T, int kEpt, bool kGrad>
 struct Window {
-  static constexpr int kRows = (kEpt <= 8 ? 4 : 2) / (kGrad ? 2 : 1);
   static constexpr int kPieces = 32 * kEpt * static_cast<int>(sizeof(T)) / 16 + 1;     // of one window
-  static constexpr int kRoundPieces = kRows * (kGrad ? 2 : 1) * kWindowWarps * kPieces;
-  static constexpr int kSlots = 6 * kRoundPieces * 16 <= 200 * 1024 ? 6 : (4 * kRoundPieces * 16 <= 200 * 1024 ? 4 : 2);
-  static constexpr int kFoldBytes = kWindowWarps * 32 * kEpt * 4;
-  static constexpr int kRingBytes = kSlots * kRoundPieces * 16 > kFoldBytes ? kSlots * kRoundPieces * 16 : kFoldBytes;
+  static constexpr int kRows = (kEpt == 16 && sizeof(T) == 4 ? 2 : 4) / (kGrad ? 2 : 1);
+  static constexpr int kRoundBytes = kRows * (kGrad ? 2 : 1) * kWindowWarps * kPieces * 16;
+  static constexpr int kParameterBytes = kWindowWarps * 32 * kEpt * (kGrad ? 4 : 8);
+  static constexpr int kRoom = 216 * 1024 - kParameterBytes;
+  static constexpr int kSlots = 6 * kRoundBytes <= kRoom ? 6 : (4 * kRoundBytes <= kRoom ? 4 : (3 * kRoundBytes <= kRoom ? 3 : 2));
+  static constexpr int kRingBytes = kSlots * kRoundBytes;          // at the end also: the groups' sums, a float per lane and element
+  static constexpr int kBytes = kRingBytes + kParameterBytes;
+  static_assert(kBytes <= 220 * 1024 && kRingBytes >= kWindowWarps * 32 * kEpt * 4, "shared memory");
 };
 
 // the pieces of `count` elements from `src`, asked for by the lanes of a warp; zeros in the rest of the window
@@ -809,33 +827,26 @@ __global__ void __launch_bounds__(kWindowThreads, 1)
 norm_forward_window_kernel(NormForwardArgs a) {
   typedef Window<T, kEpt, false> Shape;
   constexpr int kRows = Shape::kRows, kSlots = Shape::kSlots, kPairs = kEpt / 2;
-  FLCE_DYNAMIC_SHARED(uint4, stream_ring);                    // [slot][row][warp][piece]
+  FLCE_DYNAMIC_SHARED(uint4, stream_ring);                    // [slot][row][warp][piece], then (gain, bias) of every column
   __shared__ float scratch[2][kNormMaxWarps * 4];
   const int warps = a.group_warps;
   const int groups = kWindowWarps / warps;
   const int lane = static_cast<int>(threadIdx.x) & 31, warp = static_cast<int>(threadIdx.x) >> 5;
   const int g = warp / warps;
-  if (g >= groups) return;                                    // warps that make no whole group: there is no block-wide barrier
   const int column = (warp - g * warps) * 32 * kEpt;
   const int count = a.hidden - column < 32 * kEpt ? a.hidden - column : 32 * kEpt;      // of this warp's part
   const long long step = static_cast<long long>(gridDim.x) * groups * kRows;
   const bool rounded = !kCentered && a.round_xhat != 0;
   const float inv = 1.f / static_cast<float>(a.hidden);
-  F2 gain[kPairs], bias[kCentered ? kPairs : 1];
-  {
-    float w[kEpt], b[kEpt];
-#pragma unroll
-    for (int e = 0; e < kEpt; ++e) {
-      const bool in = lane + 32 * e < count;
-      w[e] = in && a.w != nullptr ? a.offset + CeElem<W>::load(static_cast<const W*>(a.w) + column + lane + 32 * e) : 1.f;
-      b[e] = in && a.b != nullptr ? CeElem<W>::load(static_cast<const W*>(a.b) + column + lane + 32 * e) : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < kPairs; ++i) {
-      gain[i] = f2(w[2 * i], w[2 * i + 1]);
-      if (kCentered) bias[i] = f2(b[2 * i], b[2 * i + 1]);
-    }
+  float2* parameters = reinterpret_cast<float2*>(stream_ring + Shape::kRingBytes / 16);
+  for (int c = static_cast<int>(threadIdx.x); c < warps * 32 * kEpt; c += kWindowThreads) {
+    const bool in = c < a.hidden;
+    parameters[c] = make_float2(in && a.w != nullptr ? a.offset + CeElem<W>::load(static_cast<const W*>(a.w) + c) : 1.f,
+                                in && a.b != nullptr ? CeElem<W>::load(static_cast<const W*>(a.b) + c) : 0.f);
   }
+  __syncthreads();
+  if (g >= groups) return;                                    // warps that make no whole group: no block-wide barrier follows
+  parameters += column + lane;
   auto window = [&](int slot, int r) { return stream_ring + ((slot * kRows + r) * kWindowWarps + warp) * Shape::kPieces; };
   auto source = [&](long long row) { return static_cast<const T*>(a.x) + row * a.ld_x + column; };
   auto fetch = [&](long long base, int slot) {
@@ -894,18 +905,23 @@ norm_forward_window_kernel(NormForwardArgs a) {
         if (a.rstd != nullptr) a.rstd[row + r] = rstd;
       }
     }
+    F2 scale[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) scale[r] = both(norm_warp_of_four(rstd, r));
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const float2 lo = parameters[64 * i], hi = parameters[64 * i + 32];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        F2 o = mul2(x[r][i], scale[r]);
+        if (rounded) o = f2(norm_round<T>(f2_lo(o)), norm_round<T>(f2_hi(o)));
+        if constexpr (kCentered) x[r][i] = fma2(o, f2(lo.x, hi.x), f2(lo.y, hi.y));
+        else x[r][i] = mul2(o, f2(lo.x, hi.x));
+      }
+    }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const F2 scale = both(norm_warp_of_four(rstd, r));
-      if (row + r >= a.n_rows) continue;
-#pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
-        F2 o = mul2(x[r][i], scale);
-        if (rounded) o = f2(norm_round<T>(f2_lo(o)), norm_round<T>(f2_hi(o)));
-        if constexpr (kCentered) x[r][i] = fma2(o, gain[i], bias[i]);
-        else x[r][i] = mul2(o, gain[i]);
-      }
-      window_store<T, kEpt>(static_cast<T*>(a.y) + (row + r) * a.hidden + column, count, lane, x[r]);
+      if (row + r < a.n_rows) window_store<T, kEpt>(static_cast<T*>(a.y) + (row + r) * a.hidden + column, count, lane, x[r]);
     }
     slot = slot + 1 == kSlots ? 0 : slot + 1;
   }
@@ -918,7 +934,7 @@ norm_backward_window_kernel(NormBackwardArgs a) {
   allow_dependents();      // the small kernel that adds up the partial sums
   typedef Window<T, kEpt, true> Shape;
   constexpr int kRows = Shape::kRows, kSlots = Shape::kSlots, kPairs = kEpt / 2;
-  FLCE_DYNAMIC_SHARED(uint4, stream_ring);                    // [slot][row][x, dy][warp][piece]; at the end: the groups' sums
+  FLCE_DYNAMIC_SHARED(uint4, stream_ring);                    // [slot][row][x, dy][warp][piece], then the gain of every column
   __shared__ float scratch[2][kNormMaxWarps * 4];
   const int warps = a.group_warps;
   const int groups = kWindowWarps / warps;
@@ -929,16 +945,14 @@ norm_backward_window_kernel(NormBackwardArgs a) {
   const long long step = static_cast<long long>(gridDim.x) * groups * kRows;
   const bool rounded = !kCentered && a.round_xhat != 0;
   const float inv = 1.f / static_cast<float>(a.hidden);
-  F2 gain[kPairs], dw[kPairs], db[kCentered ? kPairs : 1];
+  float* gains = reinterpret_cast<float*>(stream_ring + Shape::kRingBytes / 16);
+  for (int c = static_cast<int>(threadIdx.x); c < warps * 32 * kEpt; c += kWindowThreads)
+    gains[c] = c < a.hidden && a.w != nullptr ? a.offset + CeElem<W>::load(static_cast<const W*>(a.w) + c) : 1.f;
+  __syncthreads();
+  gains += column + lane;
+  F2 dw[kPairs], db[kCentered ? kPairs : 1];
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) {
-    float w[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = lane + 64 * i + 32 * h;
-      w[h] = c < count && a.w != nullptr ? a.offset + CeElem<W>::load(static_cast<const W*>(a.w) + column + c) : 1.f;
-    }
-    gain[i] = f2(w[0], w[1]);
     dw[i] = both(0.f);
     if (kCentered) db[i] = both(0.f);
   }
@@ -976,7 +990,7 @@ norm_backward_window_kernel(NormBackwardArgs a) {
     fetch(row + (kSlots - 1) * step, slot == 0 ? kSlots - 1 : slot - 1);
     async_wait<kSlots - 1>();
     warp_sync();
-    F2 xhat[kRows][kPairs], m[kRows][kPairs];
+    F2 xhat[kRows][kPairs], m[kRows][kPairs], minus_mean[kRows], s_mx[kRows], s_m[kRows];
     float rstd[kRows], v[4] = {0.f, 0.f, 0.f, 0.f};           // (sum m xhat, sum m) of each row
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
@@ -984,23 +998,30 @@ norm_backward_window_kernel(NormBackwardArgs a) {
       window_read<T, kEpt>(window(slot, r, 0), source_x(from), lane, xhat[r]);
       window_read<T, kEpt>(window(slot, r, 1), source_dy(from), lane, m[r]);
       rstd[r] = next_rstd[r];
-      const F2 minus_mean = both(-next_mean[r]);
-      F2 s_mx = both(0.f), s_m = both(0.f);
+      minus_mean[r] = both(-next_mean[r]);
+      s_mx[r] = s_m[r] = both(0.f);
+    }
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
+    for (int i = 0; i < kPairs; ++i) {
+      const F2 gain = f2(gains[64 * i], gains[64 * i + 32]);
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
         // behind the row's end dy is zero, which keeps xhat out of every sum
-        if (kCentered) xhat[r][i] = add2(xhat[r][i], minus_mean);
+        if (kCentered) xhat[r][i] = add2(xhat[r][i], minus_mean[r]);
         xhat[r][i] = mul2(xhat[r][i], both(rstd[r]));
         F2 xw = xhat[r][i];
         if (rounded) xw = f2(norm_round<T>(f2_lo(xw)), norm_round<T>(f2_hi(xw)));
         dw[i] = fma2(m[r][i], xw, dw[i]);
         if (kCentered) db[i] = add2(db[i], m[r][i]);
-        m[r][i] = mul2(m[r][i], gain[i]);
-        s_mx = fma2(m[r][i], xhat[r][i], s_mx);
-        if (kCentered) s_m = add2(s_m, m[r][i]);
+        m[r][i] = mul2(m[r][i], gain);
+        s_mx[r] = fma2(m[r][i], xhat[r][i], s_mx[r]);
+        if (kCentered) s_m[r] = add2(s_m[r], m[r][i]);
       }
-      v[2 * r] = f2_lo(s_mx) + f2_hi(s_mx);
-      v[2 * r + 1] = f2_lo(s_m) + f2_hi(s_m);
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      v[2 * r] = f2_lo(s_mx[r]) + f2_hi(s_mx[r]);
+      v[2 * r + 1] = f2_lo(s_m[r]) + f2_hi(s_m[r]);
     }
     fetch_statistics(row + step);
     const float sums = norm_warps_four_sums(v, warps, g, scratch, phase) * -inv;
