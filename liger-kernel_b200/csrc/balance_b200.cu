@@ -50,7 +50,7 @@ BalanceShape balance_shape(const flce_balance_t* p, bool vectors) {
   s.vectors = vectors;
   s.ept = p->n_experts <= 256 ? 8 : (p->n_experts <= 512 ? 16 : 32);
   for (s.log2_group = 0; (s.ept << s.log2_group) < p->n_experts;) ++s.log2_group;
-  s.tile = vectors && p->n_experts % 8 == 0 && p->n_experts >= 32 && p->n_experts <= 256 && p->top_k <= kTileList &&
+  s.tile = vectors && p->n_experts % 8 == 0 && p->n_experts >= 32 && p->n_experts <= 256 && p->top_k <= kTileListMost &&
            p->n_tokens <= 1 << 24;
   const int row_bytes = static_cast<int>(p->n_experts) * element_size(p->dtype);
   s.tile_buffers = kTileMaxWarps * tile_warp_bytes(row_bytes, 2) <= kMostDynamicShared ? 2 : 1;
@@ -120,8 +120,9 @@ void run_forward(const BalanceArgs& a, const BalanceShape& s, dim3 grid, float* 
 
 template <typename T>
 int run_forward_tile(const BalanceArgs& a, const BalanceShape& s, dim3 grid, float* partial, cudaStream_t stream) {
-  return launch_with_shared<balance_forward_tile_kernel<T>>(grid, static_cast<unsigned>(s.tile_warps * 32), s.tile_bytes, stream, a,
-                                                           s.tile_buffers, partial);
+  const unsigned threads = static_cast<unsigned>(s.tile_warps * 32);
+  if (a.top_k <= 8) return launch_with_shared<balance_forward_tile_kernel<T, 8>>(grid, threads, s.tile_bytes, stream, a, s.tile_buffers, partial);
+  return launch_with_shared<balance_forward_tile_kernel<T, 16>>(grid, threads, s.tile_bytes, stream, a, s.tile_buffers, partial);
 }
 
 // With a group of 4 lanes or more the four-row kernel; smaller groups have rows short enough for a lane or two.

@@ -267,17 +267,17 @@ balance_forward_kernel(BalanceArgs a, float* partial) {
   }
 }
 
-// ---- 32 to 256 experts in whole vectors, at most 8 of them chosen
+// ---- 32 to 256 experts in whole vectors, at most 16 of them chosen
 //
 // In the kernel above the choice takes most of the time: every round of it is a maximum over lanes that wait for each other
 // (48 x 16384 x 128 bf16, top 8: 351 us against 31 us of memory traffic).  Here a warp fetches 32 rows into shared memory,
-// a tile ahead, and each lane finds the 8 largest logits of a row of its own, in registers: it sorts 8 words at a time with a
-// network and merges them into a sorted list.  16-bit logits go through the network two to a word, the even and the odd columns
+// a tile ahead, and each lane finds the 8 (or 16) largest logits of a row of its own, in registers: it sorts 8 words at a time
+// with a network and merges them into a sorted list.  16-bit logits go through the network two to a word, the even and the odd columns
 // as two lists, which meet at the end.  Only the top_k-th largest logit and the largest are handed on; with them the warp
 // goes over the tile once more, rows shared by groups of lanes with 8 columns each, for the softmax and the sums per expert.
 // Where shared memory holds two tiles for each of 16 warps, the next one is fetched while this one is worked on; else one, and
 // the other warps cover the wait: more warps count for more than the second tile.
-constexpr int kTileList = 8;
+constexpr int kTileListMost = 16;
 
 template <typename T>
 struct TileWord;
@@ -329,12 +329,12 @@ __device__ __forceinline__ void tile_sort(typename TileWord<T>::Word (&v)[8]) {
     }
   }
 }
-template <typename T>
-__device__ __forceinline__ void tile_merge(typename TileWord<T>::Word (&v)[8]) {
+template <typename T, int kN>
+__device__ __forceinline__ void tile_merge(typename TileWord<T>::Word (&v)[kN]) {
 #pragma unroll
-  for (int k = 4; k >= 1; k >>= 1) {
+  for (int k = kN / 2; k >= 1; k >>= 1) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kN; ++i) {
       if ((i & k) == 0) tile_order<T>(v[i], v[i + k]);
     }
   }
@@ -345,7 +345,7 @@ __host__ __device__ inline int tile_pitch(int row_bytes) { return (row_bytes / 1
 __host__ __device__ inline int tile_warp_bytes(int row_bytes, int buffers) { return buffers * 32 * tile_pitch(row_bytes) + 32 * 8; }
 constexpr int kTileMaxWarps = 16;
 
-template <typename T>
+template <typename T, int kList>
 __global__ void __launch_bounds__(kTileMaxWarps * 32, 1)
 balance_forward_tile_kernel(BalanceArgs a, int buffers, float* partial) {
   allow_dependents();      // the small kernels that add up the partial sums
@@ -404,9 +404,9 @@ balance_forward_tile_kernel(BalanceArgs a, int buffers, float* partial) {
       // a row per lane: its 8 largest words
       {
         const uint4* row = here + lane * pitch;
-        Word list[kTileList];
+        Word list[kList];
 #pragma unroll
-        for (int i = 0; i < kTileList; ++i) list[i] = Tile::lowest();
+        for (int i = 0; i < kList; ++i) list[i] = Tile::lowest();
         for (int v = 0; v < vectors; v += 2) {
           Word w[8];
           const uint4 r0 = row[v];
@@ -420,23 +420,23 @@ balance_forward_tile_kernel(BalanceArgs a, int buffers, float* partial) {
           }
           tile_sort<T>(w);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) list[i] = Tile::larger(list[i], w[7 - i]);
-          tile_merge<T>(list);
+          for (int i = 0; i < 8; ++i) list[kList - 8 + i] = Tile::larger(list[kList - 8 + i], w[7 - i]);
+          tile_merge<T, kList>(list);
         }
-        float best[8];
+        float best[kList];
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) best[i] = list[i];
+          for (int i = 0; i < kList; ++i) best[i] = list[i];
         } else {
           // the lists of the even and of the odd columns become one
           const T* e = reinterpret_cast<const T*>(list);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) best[i] = fmaxf(CeElem<T>::load(e + 2 * i), CeElem<T>::load(e + 2 * (7 - i) + 1));
-          tile_merge<float>(best);
+          for (int i = 0; i < kList; ++i) best[i] = fmaxf(CeElem<T>::load(e + 2 * i), CeElem<T>::load(e + 2 * (kList - 1 - i) + 1));
+          tile_merge<float, kList>(best);
         }
         float kth = best[0];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) kth = i < a.top_k ? best[i] : kth;
+        for (int i = 1; i < kList; ++i) kth = i < a.top_k ? best[i] : kth;
         chosen_of[lane] = make_float2(kth, best[0]);
       }
       warp_sync();

@@ -22,7 +22,7 @@ def _emulation():
     (1, 70, 8, 2, BF16, 0), (3, 33, 8, 2, FP32, 0), (2, 50, 16, 4, FP16, 8), (2, 35, 60, 4, FP16, 0), (1, 41, 64, 6, BF16, 0),
     (2, 40, 128, 8, BF16, 0), (1, 19, 128, 8, FP32, 0), (1, 9, 160, 6, BF16, 0), (1, 9, 256, 8, BF16, 0), (1, 6, 257, 9, FP16, 0),
     (1, 5, 384, 8, FP32, 4), (1, 4, 512, 10, BF16, 0), (1, 3, 1000, 4, FP32, 0), (1, 3, 1024, 3, BF16, 0), (1, 37, 5, 1, BF16, 1),
-    (1, 12, 32, 32, BF16, 0), (1, 10, 40, 33, FP32, 0), (2, 7, 2, 1, FP32, 0)])
+    (1, 12, 32, 32, BF16, 0), (1, 10, 40, 33, FP32, 0), (1, 40, 64, 16, BF16, 0), (1, 33, 48, 11, FP32, 0), (1, 34, 32, 17, FP16, 0), (2, 7, 2, 1, FP32, 0)])
 def test_matches_definition(layers, tokens, experts, top_k, dtype, pitch):
     cases.case_matches_definition("cpu", cases.make(layers, tokens, experts, dtype), top_k, z=1e-3, pitch=pitch, up=0.5)
 
@@ -34,7 +34,7 @@ def test_masks(mask_dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
-@pytest.mark.parametrize("experts,top_k", [(8, 2), (16, 5), (60, 4), (128, 8), (300, 8)])
+@pytest.mark.parametrize("experts,top_k", [(8, 2), (16, 5), (60, 4), (128, 8), (64, 12), (300, 8)])
 def test_ties_and_masked_experts(dtype, experts, top_k):
     cases.case_ties("cpu", dtype, experts, top_k)
     cases.case_masked_experts("cpu", dtype, experts, top_k)

@@ -15,7 +15,7 @@ BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
     (4, 4000, 128, 8, BF16, 0), (2, 1900, 128, 8, FP32, 0), (1, 900, 160, 6, BF16, 0), (3, 900, 256, 8, BF16, 0),
     (1, 600, 257, 9, FP16, 0), (1, 500, 384, 8, FP32, 4), (1, 400, 512, 10, BF16, 0), (1, 300, 1000, 4, FP32, 0),
     (1, 300, 1024, 3, BF16, 0), (1, 3700, 5, 1, BF16, 1), (1, 1200, 32, 32, BF16, 0), (1, 1000, 40, 33, FP32, 0), (2, 70, 2, 1, FP32, 0),
-    (40, 257, 96, 8, BF16, 0), (2, 1000, 128, 1, BF16, 0), (2, 1000, 128, 5, FP16, 0), (2, 1000, 128, 16, BF16, 0),
+    (40, 257, 96, 8, BF16, 0), (2, 1000, 128, 1, BF16, 0), (2, 1000, 128, 5, FP16, 0), (2, 1000, 128, 16, BF16, 0), (3, 1000, 128, 10, BF16, 0), (2, 700, 256, 12, FP32, 0), (2, 700, 64, 17, BF16, 0),
     (2, 1000, 120, 8, BF16, 8), (2, 1001, 127, 8, BF16, 1)])
 def test_matches_definition(layers, tokens, experts, top_k, dtype, pitch):
     cases.case_matches_definition("cuda", cases.make(layers, tokens, experts, dtype), top_k, z=1e-3, pitch=pitch, up=0.5)
@@ -29,7 +29,7 @@ def test_masks(mask_dtype, experts):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
-@pytest.mark.parametrize("experts,top_k", [(8, 2), (16, 5), (60, 4), (64, 8), (128, 8), (128, 3), (256, 8), (300, 8)])
+@pytest.mark.parametrize("experts,top_k", [(8, 2), (16, 5), (60, 4), (64, 8), (128, 8), (128, 3), (128, 12), (256, 8), (300, 8)])
 def test_ties_and_masked_experts(dtype, experts, top_k):
     cases.case_ties("cuda", dtype, experts, top_k)
     cases.case_masked_experts("cuda", dtype, experts, top_k)
