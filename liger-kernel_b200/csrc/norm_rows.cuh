@@ -330,6 +330,8 @@ norm_backward_stream_kernel(NormBackwardArgs a) {
   const int vectors = a.hidden / kVec;
   const long long step = static_cast<long long>(gridDim.x) * groups * kRows;
   const bool rounded = !kCentered && a.round_xhat != 0;
+  // rows are counted from the last one: what forward, or the kernel that made dy, touched last is what L2 still holds
+  const long long last = a.n_rows - 1;
 
   uint4 raw_w[kUnits * kWVecs];
   stream_load_parameter<W, kUnits, kWVecs>(a.w, first, vectors, raw_w);
@@ -355,8 +357,8 @@ norm_backward_stream_kernel(NormBackwardArgs a) {
     for (int r = 0; r < kRows; ++r) {
       const long long row = base + r;
       const bool live = row < a.n_rows;
-      const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (live ? row : 0) * a.ld_x) + first;
-      const uint4* dy = reinterpret_cast<const uint4*>(static_cast<const T*>(a.dy) + (live ? row : 0) * a.ld_dy) + first;
+      const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (live ? last - row : 0) * a.ld_x) + first;
+      const uint4* dy = reinterpret_cast<const uint4*>(static_cast<const T*>(a.dy) + (live ? last - row : 0) * a.ld_dy) + first;
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         async_copy16(&cell(slot, r, 0, u), x + u * 32, live && first + u * 32 < vectors ? 16 : 0);
@@ -370,8 +372,8 @@ norm_backward_stream_kernel(NormBackwardArgs a) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       const bool live = base + r < a.n_rows;
-      next_mean[r] = kCentered && live ? __ldg(a.mean + base + r) : 0.f;
-      next_rstd[r] = live ? __ldg(a.rstd + base + r) : 0.f;
+      next_mean[r] = kCentered && live ? __ldg(a.mean + last - base - r) : 0.f;
+      next_rstd[r] = live ? __ldg(a.rstd + last - base - r) : 0.f;
     }
   };
 
@@ -427,7 +429,7 @@ norm_backward_stream_kernel(NormBackwardArgs a) {
       const float m_mean = kCentered ? __shfl_sync(0xffffffffu, sum, r * 16 + 8) * inv : 0.f;
       const long long row = round + mine + r;
       if (row >= a.n_rows) continue;
-      uint4* dx = reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + row * a.hidden) + first;
+      uint4* dx = reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + (last - row) * a.hidden) + first;
       // rstd (m - mean(m) - xhat c), xhat = (x - mean) rstd
       const F2 minus_c = both(-c), minus_m = both(-m_mean);
 #pragma unroll
@@ -627,6 +629,7 @@ norm_backward_narrow_kernel(NormBackwardArgs a) {
   const int g = static_cast<int>(threadIdx.x) >> a.log2_group;
   const bool column = t * kVec < a.hidden;
   const bool rounded = !kCentered && a.round_xhat != 0;
+  const long long last = a.n_rows - 1;      // rows are counted from the last one, as above
   const long long step = static_cast<long long>(gridDim.x) * groups * kRows;
   F2 gain[kPairs], dw[kPairs], db[kPairs];
   {
@@ -653,7 +656,7 @@ norm_backward_narrow_kernel(NormBackwardArgs a) {
     for (int r = 0; r < kRows; ++r) {
       const long long row = base + r * groups;
       const bool live = row < a.n_rows;
-      const long long from = live ? row : 0;
+      const long long from = live ? last - row : 0;
       async_copy16(&cell(slot, r, 0), reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + from * a.ld_x) + t, live && column ? 16 : 0);
       async_copy16(&cell(slot, r, 1), reinterpret_cast<const uint4*>(static_cast<const T*>(a.dy) + from * a.ld_dy) + t, live && column ? 16 : 0);
     }
@@ -664,8 +667,8 @@ norm_backward_narrow_kernel(NormBackwardArgs a) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       const long long row = base + r * groups;
-      next_mean[r] = kCentered && row < a.n_rows ? __ldg(a.mean + row) : 0.f;
-      next_rstd[r] = row < a.n_rows ? __ldg(a.rstd + row) : 0.f;
+      next_mean[r] = kCentered && row < a.n_rows ? __ldg(a.mean + last - row) : 0.f;
+      next_rstd[r] = row < a.n_rows ? __ldg(a.rstd + last - row) : 0.f;
     }
   };
   long long round = static_cast<long long>(blockIdx.x) * groups * kRows;
@@ -721,7 +724,7 @@ norm_backward_narrow_kernel(NormBackwardArgs a) {
         if (kCentered) m = add2(m, minus_m);
         Pairs<T>::set(reinterpret_cast<uint32_t*>(&out) + i * Pairs<T>::kWords, mul2(fma2(xhat_of(r, i), minus_c, m), both(rstd[r])));
       }
-      if (column && row < a.n_rows) reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + row * a.hidden)[t] = out;
+      if (column && row < a.n_rows) reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + (last - row) * a.hidden)[t] = out;
     }
   }
   // the groups of the block, folded in halves in a fixed order
@@ -944,6 +947,7 @@ norm_backward_window_kernel(NormBackwardArgs a) {
   const int count = a.hidden - column < 32 * kEpt ? a.hidden - column : 32 * kEpt;
   const long long step = static_cast<long long>(gridDim.x) * groups * kRows;
   const bool rounded = !kCentered && a.round_xhat != 0;
+  const long long last = a.n_rows - 1;      // rows are counted from the last one, as above
   const float inv = 1.f / static_cast<float>(a.hidden);
   float* gains = reinterpret_cast<float*>(stream_ring + Shape::kRingBytes / 16);
   for (int c = static_cast<int>(threadIdx.x); c < warps * 32 * kEpt; c += kWindowThreads)
@@ -965,8 +969,8 @@ norm_backward_window_kernel(NormBackwardArgs a) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       const bool live = base + r < a.n_rows;
-      window_fetch<T, Shape::kPieces>(window(slot, r, 0), source_x(live ? base + r : 0), live ? count : 0, lane);
-      window_fetch<T, Shape::kPieces>(window(slot, r, 1), source_dy(live ? base + r : 0), live ? count : 0, lane);
+      window_fetch<T, Shape::kPieces>(window(slot, r, 0), source_x(live ? last - base - r : 0), live ? count : 0, lane);
+      window_fetch<T, Shape::kPieces>(window(slot, r, 1), source_dy(live ? last - base - r : 0), live ? count : 0, lane);
     }
     async_commit();
   };
@@ -975,8 +979,8 @@ norm_backward_window_kernel(NormBackwardArgs a) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       const bool live = base + r < a.n_rows;
-      next_mean[r] = kCentered && live ? __ldg(a.mean + base + r) : 0.f;
-      next_rstd[r] = live ? __ldg(a.rstd + base + r) : 0.f;
+      next_mean[r] = kCentered && live ? __ldg(a.mean + last - base - r) : 0.f;
+      next_rstd[r] = live ? __ldg(a.rstd + last - base - r) : 0.f;
     }
   };
   long long row = g < groups ? (static_cast<long long>(blockIdx.x) * groups + g) * kRows : a.n_rows;
@@ -994,7 +998,7 @@ norm_backward_window_kernel(NormBackwardArgs a) {
     float rstd[kRows], v[4] = {0.f, 0.f, 0.f, 0.f};           // (sum m xhat, sum m) of each row
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const long long from = row + r < a.n_rows ? row + r : 0;
+      const long long from = row + r < a.n_rows ? last - row - r : 0;
       window_read<T, kEpt>(window(slot, r, 0), source_x(from), lane, xhat[r]);
       window_read<T, kEpt>(window(slot, r, 1), source_dy(from), lane, m[r]);
       rstd[r] = next_rstd[r];
@@ -1035,7 +1039,7 @@ norm_backward_window_kernel(NormBackwardArgs a) {
         if (kCentered) m[r][i] = add2(m[r][i], minus_m);
         m[r][i] = mul2(fma2(xhat[r][i], minus_c, m[r][i]), both(rstd[r]));
       }
-      window_store<T, kEpt>(static_cast<T*>(a.dx) + (row + r) * a.hidden + column, count, lane, m[r]);
+      window_store<T, kEpt>(static_cast<T*>(a.dx) + (last - row - r) * a.hidden + column, count, lane, m[r]);
     }
     slot = slot + 1 == kSlots ? 0 : slot + 1;
   }
