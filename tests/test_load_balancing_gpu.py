@@ -97,3 +97,28 @@ def test_same_bits_on_another_stream_and_replayed(experts):
     torch.cuda.synchronize()
     for a, c, d, e in zip(first, second, third, captured):
         assert torch.equal(a, c) and torch.equal(a, d) and torch.equal(a, e)
+
+
+@pytest.mark.parametrize("tokens,experts", [(16_000_000, 136), (17_000_000, 128)])
+def test_offsets_beyond_32_bits(tokens, experts):
+    """More than 2^31 logits in a layer, by tiles and without: every expert's count, and the last rows' gradient from the counts."""
+    import liger_kernel_b200 as lk
+
+    x = torch.zeros(tokens, experts, dtype=BF16, device="cuda")
+    favourite = torch.arange(tokens, device="cuda") % 7 * 3                  # 0, 3, .. 18, then the lowest others
+    x.scatter_(1, favourite[:, None], 4.0)
+    x.requires_grad_(True)
+    out = lk.liger_load_balancing_loss(x, experts, 2, return_expert_counts=True)
+    first = torch.bincount(favourite, minlength=experts)
+    second = torch.zeros_like(first)
+    second[0], second[1] = int((favourite != 0).sum()), int((favourite == 0).sum())
+    assert torch.equal(out.expert_counts, first + second)
+    (grad,) = torch.autograd.grad(out.loss, (x,), torch.tensor(1e6, device="cuda"))
+    rows = slice(tokens - 4, tokens)
+    c = out.expert_counts.double()
+    a = 1e6 * experts * (c - c.mean()) / tokens ** 2
+    p = torch.softmax(x.detach()[rows].double(), -1)
+    want = p * (a - (a * p).sum(-1, keepdim=True))
+    # probabilities to (64 + 4 d) u with d = 4, bf16 results to half a step
+    limit = 2 * (64 + 16) * cases.U * p * (a.abs() + (a.abs() * p).sum(-1, keepdim=True)) + 2.0 ** -8 * 1.01 * want.abs()
+    assert bool(((grad[rows].double() - want).abs() <= limit).all())

@@ -86,3 +86,29 @@ def test_same_bits_on_another_stream_and_replayed(hidden):
     torch.cuda.synchronize()
     for a, c, d, e in zip(first, second, third, captured):
         assert torch.equal(a, c) and torch.equal(a, d) and torch.equal(a, e)
+
+
+@pytest.mark.parametrize("kind,hidden,rows", [("layer", 4096, 540000), ("rms", 128, 17_000_000), ("layer", 4097, 530000)])
+def test_offsets_beyond_32_bits(kind, hidden, rows):
+    """More than 2^31 elements, one path each for wide, narrow and unaligned rows: the first and the last rows against the
+    definition (they differ from each other: an offset that wraps would show)."""
+    import liger_kernel_b200 as lk
+
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.empty(rows, hidden, dtype=BF16, device="cuda")
+    dy = torch.empty(rows, hidden, dtype=BF16, device="cuda")
+    x.zero_()
+    dy.zero_()
+    some = list(range(5)) + list(range(rows - 5, rows))
+    x[some] = torch.randn(10, hidden, generator=g, device="cuda").to(BF16)
+    dy[some] = torch.randn(10, hidden, generator=g, device="cuda").to(BF16)
+    w = (1 + 0.1 * torch.randn(hidden, generator=g, device="cuda")).to(BF16)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    y = lk.liger_layer_norm(x, w, None, 1e-6) if kind == "layer" else lk.liger_rms_norm(x, w, 1e-6, casting_mode="gemma")
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    ref = cases.reference(x.detach()[some].cpu(), w.detach().cpu(), None, dy[some].cpu(), 1e-6, 0.0, kind == "layer")
+    cases.compare("y", y.detach()[some], ref["y"], ref["tol"]["y"])
+    cases.compare("dx", dx[some], ref["dx"], ref["tol"]["dx"])
+    cases.compare("dw", dw, ref["dw"], ref["tol"]["dw"])          # all other rows are zero: they add nothing
+    assert not y.detach()[5:-5:9973].any() and not dx[5:-5:9973].any()
