@@ -268,6 +268,15 @@ BalanceOperands balance_operands(at::TensorList logits, int64_t num_experts, int
   return o;
 }
 
+// Dense elements of `whole` from `offset` on, in the given shape, as a tensor that shares its storage: what select and view give,
+// without a trip through the dispatcher for each of dozens of layers.
+Tensor piece_of(const Tensor& whole, int64_t offset, at::IntArrayRef sizes) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  t.unsafeGetTensorImpl()->set_storage_offset(whole.storage_offset() + offset);
+  return t;
+}
+
 struct BalanceBackward : public torch::autograd::Node {
   std::vector<SavedVariable> logits;
   SavedVariable mask;
@@ -304,9 +313,8 @@ struct BalanceBackward : public torch::autograd::Node {
     Tensor all = at::empty({o.p.n_layers, o.p.n_tokens, num_experts}, x[0].options().memory_format(at::MemoryFormat::Contiguous));
     check(g_lib.balance_backward(&o.p, o.pointers.data(), coef.const_data_ptr<float>(), up.const_data_ptr<float>(), all.data_ptr(),
                                  on.stream));
-    const std::vector<Tensor> layers = all.unbind(0);
     for (size_t l = 0; l < x.size(); ++l) {
-      if (task_should_compute_output(l)) out[l] = x[l].dim() == 2 ? layers[l] : layers[l].view(x[l].sizes());
+      if (task_should_compute_output(l)) out[l] = piece_of(all, static_cast<int64_t>(l) * o.p.n_tokens * num_experts, x[l].sizes());
     }
     return once_differentiable(std::move(out), recording);
   }
@@ -330,9 +338,9 @@ std::tuple<Tensor, Tensor, Tensor> load_balancing_loss(at::TensorList logits, in
     const Tensor workspace = at::empty({static_cast<int64_t>(bytes)}, options.dtype(at::kByte));
     check(g_lib.balance_forward(&o.p, o.pointers.data(), out.data_ptr<float>(), counts.data_ptr<int64_t>(), out.data_ptr<float>() + 2,
                                 workspace.data_ptr(), bytes, on.stream));
-    loss = out.select(0, 0);
-    z_loss = out.select(0, 1);
-    if (recording) coef = out.narrow(0, 2, num_experts + 1);
+    loss = piece_of(out, 0, {});
+    z_loss = piece_of(out, 1, {});
+    if (recording) coef = piece_of(out, 2, {num_experts + 1});
   }
   if (recording) {
     auto node = std::shared_ptr<BalanceBackward>(new BalanceBackward(), torch::autograd::deleteNode);
