@@ -205,7 +205,8 @@ int flce_b200_balance_forward(const flce_balance_t* p, const void* const* logits
     if (rc != FLCE_OK) return rc;
     ++launches;
   }
-  rc = launch_dependent<balance_total_kernel>(dim3(1), dim3(kBalTotalThreads), stream, static_cast<const float*>(few ? partial : nullptr),
+  const int threads = few && experts <= 256 ? 256 : kBalTotalThreads;
+  rc = launch_dependent<balance_total_kernel>(dim3(1), dim3(threads), stream, static_cast<const float*>(few ? partial : nullptr),
                                               static_cast<int>(blocks), reinterpret_cast<long long*>(counts), static_cast<const double*>(sums),
                                               static_cast<const long long*>(kept), static_cast<int>(p->n_layers), experts,
                                               p->lse_square_scale, loss, coef);

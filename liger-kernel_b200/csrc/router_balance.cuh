@@ -601,19 +601,19 @@ balance_layer_kernel(const float* partial, int blocks, int experts, long long* c
 
 // out[0] = loss, out[1] = its lse^2 term; coef[e] = a_e, coef[experts] = 2 lambda / N.  No kept token: all zero.  One block: a
 // thread per expert and share of the layers.  With few partials (partial != nullptr) it adds them up itself, in the place of
-// balance_layer_kernel, and leaves the counts.
-constexpr int kBalTotalThreads = 1024;
+// balance_layer_kernel, and leaves the counts; 256 threads then do for up to 256 experts, and are launched sooner.
+constexpr int kBalTotalThreads = 1024;      // at most
 __global__ void __launch_bounds__(kBalTotalThreads)
 balance_total_kernel(const float* partial, int blocks, long long* counts, const double* sums, const long long* kept, int layers, int experts,
                      float lambda, float* out, float* coef) {
   __shared__ double scratch[4][kBalTotalThreads / 32];
   __shared__ double part_c[kBalTotalThreads], part_s[kBalTotalThreads];
   wait_for_previous_kernel();
-  const int tid = static_cast<int>(threadIdx.x);
+  const int tid = static_cast<int>(threadIdx.x), threads = static_cast<int>(blockDim.x);
   const long long words = balance_partial_words(experts);
   int wide = 32;
   while (wide < experts) wide *= 2;
-  const int e = tid & (wide - 1), shares = kBalTotalThreads / wide;
+  const int e = tid & (wide - 1), shares = threads / wide;
   double c = 0.0, s = 0.0, v[4] = {0.0, 0.0, 0.0, 0.0};      // v: sum C S, sum C, N, sum lse^2
   if (e < experts) {
 #pragma unroll 4
@@ -634,13 +634,13 @@ balance_total_kernel(const float* partial, int blocks, long long* counts, const 
     }
   }
   if (partial != nullptr) {
-    for (int r = tid; r < layers * blocks; r += kBalTotalThreads) {
+    for (int r = tid; r < layers * blocks; r += threads) {
       const float* row = partial + r * words + experts;
       v[3] += row[0];
       v[2] += reinterpret_cast<const int*>(row)[experts + 1];
     }
   } else {
-    for (int l = tid; l < layers; l += kBalTotalThreads) {
+    for (int l = tid; l < layers; l += threads) {
       v[2] += static_cast<double>(kept[l]);
       v[3] += sums[static_cast<long long>(l) * (experts + 1) + experts];
     }
@@ -665,7 +665,7 @@ balance_total_kernel(const float* partial, int blocks, long long* counts, const 
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    v[i] = scratch[i][tid & 31];
+    v[i] = (tid & 31) < threads >> 5 ? scratch[i][tid & 31] : 0.0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
   }
