@@ -151,8 +151,8 @@ def _mixtral_balancing_loss():
 def router_balancing_loss(router_logits, num_experts, top_k, attention_mask=None):
     """The router's auxiliary loss of the mixture-of-experts families: ``liger_load_balancing_loss`` for router logits on the GPU,
     the model library's own function for what that does not cover (logits on the CPU, masks that are not one element per
-    token, more than 1024 experts)."""
-    if isinstance(router_logits, (tuple, list)) and len(router_logits) > 0 and num_experts <= 1024:
+    token, more than 1024 experts, a forward that is being traced by torch.compile)."""
+    if not torch.compiler.is_compiling() and isinstance(router_logits, (tuple, list)) and len(router_logits) > 0 and num_experts <= 1024:
         head = router_logits[0]
         tokens = head.numel() // num_experts
         one_per_token = attention_mask is None or (attention_mask.dim() == 2 and attention_mask.numel() == tokens)

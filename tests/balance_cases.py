@@ -1,5 +1,5 @@
 """Shared bodies of the tests of the router's load-balancing loss: run on a B200 (tests/test_load_balancing_gpu.py) and, with the
-library's host side and kernels emulated, on CPU tensors (tests/test_load_balancing_emulation_cpu.py).  The checker is the
+library's host side and kernels emulated, on CPU tensors (tests/test_load_balancing_emulation_cpu.py).  They are held to the
 definition in float64, the choice of experts a sort by (logit, index).
 
 Tolerances.  u = 2^-24.  With d_j = max - x_j: the exponent d_j log2(e) carries two roundings, 2 u d_j in e^-d_j, the device's

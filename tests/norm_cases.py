@@ -1,5 +1,5 @@
 """Shared bodies of the tests of layer norm and RMSNorm: run on a B200 (tests/test_norm_gpu.py) and, with the library's host side
-and kernels emulated, on CPU tensors (tests/test_norm_emulation_cpu.py).  The checker is the definition in float64.
+and kernels emulated, on CPU tensors (tests/test_norm_emulation_cpu.py).  They are held to the definition in float64.
 
 Tolerances.  u = 2^-24, h = half a step of the result's type (finfo.eps / 2).  A row's sums are added in at most 32 + 5 + 16
 steps (elements of a thread, lanes, warps), the rest of an element is below ten operations: C = 64 steps of u against the
