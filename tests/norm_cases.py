@@ -11,6 +11,7 @@ same holds for x - mean.  So, with k = 1 + max|x| rstd of the row,
 (n rows, added one after the other at worst).  "llama" casting rounds xhat once more: h |xhat g| in y and h sum|dy xhat| in dw."""
 
 import torch
+import torch.utils.checkpoint
 
 U, C = 2.0 ** -24, 64
 
@@ -213,3 +214,39 @@ def case_refusals(device):
     (first,) = torch.autograd.grad(lk.liger_layer_norm(xg, w, None, 1e-6).square().sum(), (xg,), create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         first.sum().backward()
+
+
+def case_autograd(device):
+    """A graph kept and used twice, a recomputed one, hooks on what is saved, an input changed in between, a weight alone."""
+    import pytest
+
+    import liger_kernel_b200 as lk
+
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(12, 40, generator=g).to(device).requires_grad_(True)
+    w = torch.randn(40, generator=g).to(device).requires_grad_(True)
+    b = torch.randn(40, generator=g).to(device).requires_grad_(True)
+    dy = torch.randn(12, 40, generator=g).to(device)
+    y = lk.liger_layer_norm(x, w, b, 1e-6)
+    want = torch.autograd.grad(y, (x, w, b), dy, retain_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(want, torch.autograd.grad(y, (x, w, b), dy)))
+    with pytest.raises(RuntimeError, match="second time"):
+        y.backward(dy)
+    again = torch.utils.checkpoint.checkpoint(lambda t: lk.liger_layer_norm(t, w, b, 1e-6), x, use_reentrant=False)
+    assert all(torch.equal(p, q) for p, q in zip(want, torch.autograd.grad(again, (x, w, b), dy)))
+    packed = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: packed.append(t) or t, lambda t: t):
+        y = lk.liger_layer_norm(x, w, b, 1e-6)
+    assert len(packed) == 3 and all(torch.equal(p, q) for p, q in zip(want, torch.autograd.grad(y, (x, w, b), dy)))
+    (only,) = torch.autograd.grad(lk.liger_layer_norm(x, w, b, 1e-6), (b,), dy)
+    assert torch.equal(only, want[2])
+    for fn in (lambda: lk.liger_layer_norm(x, w, b, 1e-6), lambda: lk.liger_rms_norm(x, w, 1e-6)):
+        y = fn()
+        with torch.no_grad():
+            x.mul_(1.5)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward(dy)
+    with torch.no_grad():
+        assert not lk.liger_rms_norm(x, w, 1e-6).requires_grad
+    with torch.inference_mode():
+        assert lk.liger_layer_norm(x, w, b, 1e-6).shape == x.shape

@@ -111,3 +111,8 @@ def test_entry_points_check_their_arguments():
     rms = norm(kind=_lib.FLCE_RMS_NORM, bias=None)
     assert backward(rms, mean=None) == 0 and backward(rms, db=base + 5120) == INVALID
     assert lib.flce_b200_norm_workspace_bytes(C.byref(norm())) >= 2 * 16 * 4
+
+
+def test_autograd():
+    with train_ops_emu.installed():
+        cases.case_autograd("cpu")

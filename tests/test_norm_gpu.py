@@ -112,3 +112,35 @@ def test_offsets_beyond_32_bits(kind, hidden, rows):
     cases.compare("dx", dx[some], ref["dx"], ref["tol"]["dx"])
     cases.compare("dw", dw, ref["dw"], ref["tol"]["dw"])          # all other rows are zero: they add nothing
     assert not y.detach()[5:-5:9973].any() and not dx[5:-5:9973].any()
+
+
+def test_autograd():
+    cases.case_autograd("cuda")
+
+
+def test_two_streams_at_once():
+    """Norms and balance losses under way on two streams at the same time do not touch each other's scratch."""
+    import liger_kernel_b200 as lk
+
+    def inputs(seed):
+        x, w, b, dy = (t.cuda() for t in cases.make(3000, 2048, BF16, BF16, seed=seed))
+        logits = tuple(t.requires_grad_(True) for t in torch.randn(4, 3000, 64, generator=torch.Generator().manual_seed(seed)).to(BF16).cuda())
+        return [t.requires_grad_(True) for t in (x, w, b)], dy, logits
+
+    def step(leaves, dy, logits):
+        y = lk.liger_layer_norm(*leaves, 1e-6)
+        out = lk.liger_load_balancing_loss(logits, 64, 4, return_expert_counts=True)
+        return [y.detach(), out.loss.detach(), out.expert_counts, *torch.autograd.grad(y, leaves, dy), *torch.autograd.grad(out.loss, logits)]
+
+    data = [inputs(1), inputs(2)]
+    want = [step(*d) for d in data]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(5):
+        for k, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[k] = step(*data[k])
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
