@@ -10,6 +10,10 @@
 // difference would be left with few digits.)  Tokens that the mask leaves out are not read: whatever they hold, they add
 // nothing and their gradient is zero.
 //
+// The largest logit is subtracted before the scaling to base 2, in every kernel: -top * log2(e) folded into one fma leaves the rounding of
+// that product in all exponents of the row, |top| 2^-24, which overflows exp2 from |top| of about 1.5e9 on; a row that a mask filled with
+// the type's lowest value is such a row.
+//
 // Forward reads the logits once, backward reads them once and writes as much; nothing per token is kept in between.  A row is
 // shared by a group of 1..32 lanes, each holding kEpt consecutive logits in registers, so the sums over a row are shuffles and
 // several rows share a warp.  A lane keeps its columns for all rows of its block: S and C are sums in registers, left as one
@@ -455,7 +459,7 @@ balance_forward_tile_kernel(BalanceArgs a, int buffers, float* partial) {
           }
           const float2 of = chosen_of[row];
           const F2 counted = both((kept >> row & 1u) != 0 ? 1.f : 0.f);
-          const F2 shift = both(-of.y * kLog2e);
+          const F2 minus_top = both(-of.y);
           F2 sum = both(0.f), many = both(0.f);
           kth[r] = of.x;
 #pragma unroll
@@ -464,7 +468,7 @@ balance_forward_tile_kernel(BalanceArgs a, int buffers, float* partial) {
             const F2 in = f2(f2_lo(v) >= of.x ? 1.f : 0.f, f2_hi(v) >= of.x ? 1.f : 0.f);
             many = add2(many, in);
             c[i] = fma2(in, counted, c[i]);
-            const F2 d = fma2(v, both(kLog2e), shift);
+            const F2 d = mul2(add2(v, minus_top), both(kLog2e));
             x[r][i] = f2(ex2_approx(f2_lo(d)), ex2_approx(f2_hi(d)));
             sum = add2(sum, x[r][i]);
           }
@@ -789,11 +793,11 @@ balance_backward_four_kernel(BalanceArgs a, const float* coef, const float* grad
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const F2 shift = both(-top[r] * kLog2e);
+      const F2 minus_top = both(-top[r]);
       F2 sum = both(0.f), product = both(0.f);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const F2 d = fma2(x[r][i], both(kLog2e), shift);
+        const F2 d = mul2(add2(x[r][i], minus_top), both(kLog2e));
         x[r][i] = f2(ex2_approx(f2_lo(d)), ex2_approx(f2_hi(d)));
         sum = add2(sum, x[r][i]);
         product = fma2(x[r][i], w[i], product);

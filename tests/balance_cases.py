@@ -227,3 +227,34 @@ def case_refusals(device):
         xg.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def case_far_rows(device, dtype, experts, top_k):
+    """Whole rows of -1e10, of +1e10, of the type's lowest and of its largest finite value among ordinary ones: a softmax over equal
+    logits is 1 / experts wherever they lie, and neither the loss nor the gradients of the other rows may suffer.  Then rows whose
+    largest logit is 1e10 above or below the others, or at the other end of the type's range."""
+    import liger_kernel_b200 as lk
+
+    info = torch.finfo(dtype)
+    far = [v for v in (-1e10, 1e10, info.min, info.max) if abs(v) <= info.max]
+    x = make(2, 40, experts, dtype, seed=6)
+    for i, v in enumerate(far):
+        x[i % 2, 3 + i::13] = v
+    case_matches_definition(device, x, top_k, up=0.5)
+    if abs(far[0]) < info.max:                                    # with the lse^2 term, where the square is a finite fp32 number
+        x = make(1, 40, experts, dtype, seed=6)
+        x[0, 3], x[0, 17] = -1e10, 1e10
+        case_matches_definition(device, x, top_k, z=1e-22)
+    x = make(1, 40, experts, dtype, seed=7)
+    x[0, 2, 1], x[0, 5, experts - 1], x[0, 9, 0], x[0, 9, 1] = far[1], far[-1], far[-1], info.min
+    x[0, 12], x[0, 14] = far[0], info.min
+    x[0, 12, 2], x[0, 14, 3] = 1.0, info.max
+    ref = reference(x, top_k, torch.ones(40, dtype=torch.bool), 0.0)
+    t = x[0].to(device).requires_grad_(True)
+    out = lk.liger_load_balancing_loss(t, experts, top_k, return_expert_counts=True)
+    (grad,) = torch.autograd.grad(out.loss, (t,))
+    assert torch.equal(out.expert_counts.cpu(), ref["counts"][0])
+    # beyond d = 104 a probability is below 2^-150 and zero in fp32: r_j p_j is largest before that
+    assert abs(float(out.loss.detach()) - ref["loss"]) <= (40 + 64 + 4 * 104) * U * ref["loss"]
+    limit = ref["tol_grads"][0] * 1.01 + info.eps / 2 * ref["grads"][0].abs() * 1.01 + info.tiny * info.eps
+    assert bool(((grad.cpu().double() - ref["grads"][0]).abs() <= limit).all())

@@ -124,3 +124,9 @@ def test_entry_points_check_their_arguments(_emulation):
     assert backward(balance(), coef=None) == INVALID and backward(balance(), up=None) == INVALID and backward(balance(), grads=None) == INVALID
     assert backward(balance(), grads=base + 2) == INVALID
     assert backward(balance(n_tokens=0)) == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("experts,top_k", [(8, 2), (24, 4), (32, 4), (60, 4), (64, 6), (128, 8), (256, 8), (300, 8)])
+def test_rows_far_from_zero(dtype, experts, top_k):
+    cases.case_far_rows("cpu", dtype, experts, top_k)

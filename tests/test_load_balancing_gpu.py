@@ -122,3 +122,9 @@ def test_offsets_beyond_32_bits(tokens, experts):
     # probabilities to (64 + 4 d) u with d = 4, bf16 results to half a step
     limit = 2 * (64 + 16) * cases.U * p * (a.abs() + (a.abs() * p).sum(-1, keepdim=True)) + 2.0 ** -8 * 1.01 * want.abs()
     assert bool(((grad[rows].double() - want).abs() <= limit).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("experts,top_k", [(8, 2), (24, 4), (32, 4), (60, 4), (64, 6), (128, 8), (128, 12), (256, 8), (300, 8), (512, 10)])
+def test_rows_far_from_zero(dtype, experts, top_k):
+    cases.case_far_rows("cuda", dtype, experts, top_k)
