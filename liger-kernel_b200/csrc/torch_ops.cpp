@@ -231,6 +231,7 @@ struct BalanceOperands {
 
 BalanceOperands balance_operands(at::TensorList logits, int64_t num_experts, int64_t top_k, const Tensor& mask, double lse_square_scale) {
   TORCH_CHECK_VALUE(!logits.empty(), "expected the router logits of at least one layer");
+  TORCH_CHECK_VALUE(num_experts >= 1, "num_experts must be at least 1, got ", num_experts);
   BalanceOperands o;
   const Tensor& head = logits[0];
   require_device(head);
@@ -243,7 +244,6 @@ BalanceOperands balance_operands(at::TensorList logits, int64_t num_experts, int
     o.logits.push_back(as_rows(t, num_experts));
     same_pitch = same_pitch && o.logits.back().stride(0) == o.logits[0].stride(0);
   }
-  TORCH_CHECK_VALUE(num_experts >= 1, "num_experts must be at least 1, got ", num_experts);
   TORCH_CHECK_VALUE(top_k >= 1 && top_k <= num_experts, "top_k must be in [1, ", num_experts, "], got ", top_k);
   TORCH_CHECK_NOT_IMPLEMENTED(num_experts <= 1024, "at most 1024 experts, got ", num_experts);
   o.p.n_layers = static_cast<int64_t>(o.logits.size());

@@ -258,3 +258,20 @@ def case_far_rows(device, dtype, experts, top_k):
     assert abs(float(out.loss.detach()) - ref["loss"]) <= (40 + 64 + 4 * 104) * U * ref["loss"]
     limit = ref["tol_grads"][0] * 1.01 + info.eps / 2 * ref["grads"][0].abs() * 1.01 + info.tiny * info.eps
     assert bool(((grad.cpu().double() - ref["grads"][0]).abs() <= limit).all())
+
+
+def case_counts_out_of_range(device):
+    """No experts, or fewer than none, whatever the number of dimensions and tokens: refused before anything is divided by them."""
+    import pytest
+
+    import liger_kernel_b200 as lk
+
+    for shape in ((0,), (4, 0), (2, 3, 0), (0, 3, 0), (2, 2, 2, 0)):
+        with pytest.raises(ValueError, match="num_experts must be at least 1"):
+            lk.liger_load_balancing_loss(torch.zeros(shape, device=device), 0, 1)
+    with pytest.raises(ValueError, match="num_experts must be at least 1"):
+        lk.liger_load_balancing_loss(torch.zeros(2, 3, 4, device=device), -4, 1)
+    with pytest.raises(ValueError, match="router logits must be"):
+        lk.liger_load_balancing_loss(torch.zeros(2, 3, 0, device=device), 4, 1)
+    with pytest.raises(ValueError, match="router logits must be"):
+        lk.liger_load_balancing_loss(torch.zeros((), device=device), 1, 1)

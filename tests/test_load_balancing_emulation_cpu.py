@@ -130,3 +130,7 @@ def test_entry_points_check_their_arguments(_emulation):
 @pytest.mark.parametrize("experts,top_k", [(8, 2), (24, 4), (32, 4), (60, 4), (64, 6), (128, 8), (256, 8), (300, 8)])
 def test_rows_far_from_zero(dtype, experts, top_k):
     cases.case_far_rows("cpu", dtype, experts, top_k)
+
+
+def test_counts_out_of_range():
+    cases.case_counts_out_of_range("cpu")

@@ -128,3 +128,7 @@ def test_offsets_beyond_32_bits(tokens, experts):
 @pytest.mark.parametrize("experts,top_k", [(8, 2), (24, 4), (32, 4), (60, 4), (64, 6), (128, 8), (128, 12), (256, 8), (300, 8), (512, 10)])
 def test_rows_far_from_zero(dtype, experts, top_k):
     cases.case_far_rows("cuda", dtype, experts, top_k)
+
+
+def test_counts_out_of_range():
+    cases.case_counts_out_of_range("cuda")
