@@ -78,6 +78,12 @@ const void* elements(const Tensor& t, const char* what) {
   return p;
 }
 
+// Tangents of forward-mode differentiation would be lost below autograd, and with them a part of the derivative.
+void refuse_tangent(const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(),
+                              "liger_kernel_b200 has no forward-mode derivatives: the input carries a forward gradient");
+}
+
 // A gradient of a gradient would need the graph of the kernels' own arithmetic, which does not exist: what backward returns
 // under create_graph is attached to a node that says so.
 variable_list once_differentiable(variable_list&& grads, bool recording) {
@@ -190,6 +196,7 @@ struct NormBackward : public torch::autograd::Node {
 Tensor norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, int64_t kind, double eps, double offset,
             bool round_xhat) {
   const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  for (const Tensor* t : {&x, &w, &b}) refuse_tangent(*t);
   const bool recording = torch::autograd::compute_requires_grad(x, w, b);
   Tensor y, stats;
   {
@@ -324,6 +331,7 @@ struct BalanceBackward : public torch::autograd::Node {
 std::tuple<Tensor, Tensor, Tensor> load_balancing_loss(at::TensorList logits, int64_t num_experts, int64_t top_k,
                                                        const optional<Tensor>& attention_mask, double lse_square_scale) {
   const Tensor mask = attention_mask.value_or(Tensor());
+  for (const Tensor& t : logits) refuse_tangent(t);
   const bool recording = torch::autograd::compute_requires_grad(logits);
   Tensor loss, z_loss, counts, coef;
   {

@@ -275,3 +275,23 @@ def case_counts_out_of_range(device):
         lk.liger_load_balancing_loss(torch.zeros(2, 3, 0, device=device), 4, 1)
     with pytest.raises(ValueError, match="router logits must be"):
         lk.liger_load_balancing_loss(torch.zeros((), device=device), 1, 1)
+
+
+def case_forward_mode(device):
+    """A tangent on any layer's logits is refused: dropped, it would be a derivative of zero."""
+    import pytest
+    import torch.autograd.forward_ad as fa
+
+    import liger_kernel_b200 as lk
+
+    x = make(2, 6, 8, torch.float32).to(device)
+    want = lk.liger_load_balancing_loss(tuple(x), 8)
+    with fa.dual_level():
+        dual = fa.make_dual(x[1], torch.ones_like(x[1]))
+        with pytest.raises(NotImplementedError, match="forward"):
+            lk.liger_load_balancing_loss((x[0], dual), 8)
+        with pytest.raises(NotImplementedError, match="forward"):
+            lk.LigerLoadBalancingLoss(8)(dual.clone().requires_grad_(True))
+        assert torch.equal(lk.liger_load_balancing_loss((x[0], fa.unpack_dual(dual).primal), 8), want)
+    with pytest.raises(NotImplementedError, match="forward"):
+        torch.func.jvp(lambda t: lk.liger_load_balancing_loss(t, 8), (x[0],), (torch.ones_like(x[0]),))

@@ -250,3 +250,26 @@ def case_autograd(device):
         assert not lk.liger_rms_norm(x, w, 1e-6).requires_grad
     with torch.inference_mode():
         assert lk.liger_layer_norm(x, w, b, 1e-6).shape == x.shape
+
+
+def case_forward_mode(device):
+    """A tangent on the input or on a parameter is refused: dropped, it would be a derivative of zero."""
+    import pytest
+    import torch.autograd.forward_ad as fa
+
+    import liger_kernel_b200 as lk
+
+    x, w, b = torch.randn(3, 16).to(device), torch.randn(16).to(device), torch.randn(16).to(device)
+    want = lk.liger_layer_norm(x, w, b)
+    with fa.dual_level():
+        for i in range(3):
+            args = [x, w, b]
+            args[i] = fa.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(NotImplementedError, match="forward"):
+                lk.liger_layer_norm(*args)
+            if i < 2:
+                with pytest.raises(NotImplementedError, match="forward"):
+                    lk.liger_rms_norm(*args[:2])
+        assert torch.equal(lk.liger_layer_norm(x, w, b), want)
+    with pytest.raises(NotImplementedError, match="forward"):
+        torch.func.jvp(lambda t: lk.liger_rms_norm(t, w), (x,), (torch.ones_like(x),))

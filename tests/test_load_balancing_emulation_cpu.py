@@ -134,3 +134,7 @@ def test_rows_far_from_zero(dtype, experts, top_k):
 
 def test_counts_out_of_range():
     cases.case_counts_out_of_range("cpu")
+
+
+def test_forward_mode():
+    cases.case_forward_mode("cpu")

@@ -116,3 +116,8 @@ def test_entry_points_check_their_arguments():
 def test_autograd():
     with train_ops_emu.installed():
         cases.case_autograd("cpu")
+
+
+def test_forward_mode():
+    with train_ops_emu.installed():
+        cases.case_forward_mode("cpu")

@@ -144,3 +144,7 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for a, b in zip(want, got):
         assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_forward_mode():
+    cases.case_forward_mode("cuda")
