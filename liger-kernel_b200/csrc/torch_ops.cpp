@@ -5,10 +5,14 @@
 // its kernels last as little as 3 us.  RMSNorm of 64 x 1024 rows through Python: forward 34 us, forward + backward 154 us (most of
 // it in the backward thread); through this binding 10 and 66 us, where torch's own layer norm takes 66.
 //
-// The operators are registered as composites: one dispatch, then this code; autograd nodes are built here.
+// Each operator has an autograd kernel, which looks at no data and no sizes: it goes through the dispatcher once more, to the
+// kernel for CUDA tensors that checks, allocates and launches, and sets up the gradient.  What the dispatcher puts between the two
+// therefore sees the launch as an operator: tracers record it (its results' shapes are given in _torch_ops.py), and torch.func's
+// transforms, nested ones too, find an autograd kernel at each of their levels.
 #include <dlfcn.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/function.h>
@@ -86,14 +90,23 @@ void refuse_tangent(const Tensor& t) {
 
 // A gradient of a gradient would need the graph of the kernels' own arithmetic, which does not exist: what backward returns
 // under create_graph is attached to a node that says so.
-variable_list once_differentiable(variable_list&& grads, bool recording) {
-  if (!recording) return std::move(grads);
-  auto error = std::make_shared<torch::autograd::DelayedError>(
-      "trying to differentiate twice a function that was marked with @once_differentiable", static_cast<int64_t>(grads.size()));
+template <class... Of>
+variable_list once_differentiable(variable_list&& grads, const Of&... of) {
+  if (!torch::autograd::compute_requires_grad(of...)) return std::move(grads);
+  auto error = std::shared_ptr<torch::autograd::Error>(
+      new torch::autograd::Error("trying to differentiate twice a function that was marked with @once_differentiable",
+                                 torch::autograd::collect_next_edges(of...)),
+      torch::autograd::deleteNode);
   for (auto& g : grads) {
-    if (g.defined()) g = g.detach().requires_grad_(true);
+    if (g.defined()) torch::autograd::set_history(g, error);
   }
-  return (*error)(std::move(grads));
+  return std::move(grads);
+}
+
+// the operator of that name, for calls that go through the dispatcher
+template <class Signature>
+c10::TypedOperatorHandle<Signature> operator_of(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>();
 }
 
 // ------------------------------------------------------------------ layer norm and RMSNorm
@@ -144,9 +157,73 @@ NormOperands norm_operands(int64_t kind, const Tensor& x, const Tensor& w, const
   return o;
 }
 
+Tensor norm_rows(const Tensor& x, const Tensor& w, const Tensor& b, int64_t kind, double eps, double offset, bool round_xhat,
+                 Tensor* stats) {
+  const NormOperands o = norm_operands(kind, x, w, b, eps, offset, round_xhat);
+  OnDevice on(x);
+  Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  float *rstd = nullptr, *mean = nullptr;
+  if (stats != nullptr) {
+    *stats = at::empty({kind == FLCE_LAYER_NORM ? 2 : 1, o.p.n_rows}, x.options().dtype(at::kFloat));
+    rstd = stats->data_ptr<float>();
+    mean = kind == FLCE_LAYER_NORM ? rstd + o.p.n_rows : nullptr;
+  }
+  check(g_lib.norm_forward(&o.p, y.data_ptr(), mean, rstd, on.stream));
+  return y;
+}
+
+Tensor norm_launch(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, int64_t kind, double eps, double offset,
+                   bool round_xhat) {
+  return norm_rows(x, weight.value_or(Tensor()), bias.value_or(Tensor()), kind, eps, offset, round_xhat, nullptr);
+}
+
+// y and [2 or 1, rows] fp32: rstd, mean
+std::tuple<Tensor, Tensor> norm_with_statistics_launch(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias,
+                                                       int64_t kind, double eps, double offset, bool round_xhat) {
+  Tensor stats;
+  Tensor y = norm_rows(x, weight.value_or(Tensor()), bias.value_or(Tensor()), kind, eps, offset, round_xhat, &stats);
+  return {y, stats};
+}
+
+// the gradients of x, weight and bias, the latter undefined where not wanted
+std::tuple<Tensor, Tensor, Tensor> norm_backward_launch(const Tensor& grad, const Tensor& x, const optional<Tensor>& weight,
+                                                        const optional<Tensor>& bias, const Tensor& stats, int64_t kind, double eps,
+                                                        double offset, bool round_xhat, bool need_w, bool need_b) {
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  OnDevice on(x);
+  const NormOperands o = norm_operands(kind, x, w, b, eps, offset, round_xhat);
+  const Tensor dy = as_rows(grad, o.p.hidden);
+  Tensor dx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous)), dw, db, workspace;
+  size_t bytes = 0;
+  if (need_w) dw = at::empty_like(o.w);
+  if (need_b) db = at::empty_like(o.b);
+  if (need_w || need_b) {
+    bytes = g_lib.norm_workspace_bytes(&o.p);
+    workspace = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
+  }
+  const float* rstd = stats.const_data_ptr<float>();
+  check(g_lib.norm_backward(&o.p, elements(dy, "the gradient"), dy.stride(0), kind == FLCE_LAYER_NORM ? rstd + o.p.n_rows : nullptr, rstd,
+                            dx.data_ptr(), need_w ? dw.data_ptr() : nullptr, need_b ? db.data_ptr() : nullptr,
+                            workspace.defined() ? workspace.data_ptr() : nullptr, bytes, on.stream));
+  return {dx, need_w ? dw.to(w.scalar_type()) : dw, need_b ? db.to(b.scalar_type()) : db};
+}
+
+std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& grad, const Tensor& x, const optional<Tensor>& weight,
+                                                 const optional<Tensor>& bias, const Tensor& stats, int64_t kind, double eps, double offset,
+                                                 bool round_xhat, bool need_w, bool need_b) {
+  static const auto next = operator_of<decltype(norm_backward_launch)>("liger_b200::_norm_backward");
+  variable_list out(3);
+  {
+    at::AutoDispatchBelowAutograd below;
+    std::tie(out[0], out[1], out[2]) = next.call(grad, x, weight, bias, stats, kind, eps, offset, round_xhat, need_w, need_b);
+  }
+  out = once_differentiable(std::move(out), grad, x, weight.value_or(Tensor()));
+  return {out[0], out[1], out[2]};
+}
+
 struct NormBackward : public torch::autograd::Node {
   SavedVariable x, w, b;
-  Tensor stats;                 // [2 or 1, rows] fp32: rstd, mean
+  Tensor stats;
   int64_t kind = 0;
   double eps = 0, offset = 0;
   bool round_xhat = false;
@@ -161,58 +238,31 @@ struct NormBackward : public torch::autograd::Node {
   }
 
   variable_list apply(variable_list&& grads) override {
+    static const auto backward = operator_of<decltype(norm_backward_launch)>("liger_b200::_norm_backward");
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(3);
     const Tensor& grad = grads[0];
     if (!grad.defined()) return out;
     const Tensor xs = x.unpack(), ws = w.unpack(), bs = b.unpack();
     TORCH_CHECK(stats.defined(), torch::autograd::ERR_BACKWARD_TWICE);
-    const bool recording = at::GradMode::is_enabled() && (grad.requires_grad() || xs.requires_grad() ||
-                                                          (ws.defined() && ws.requires_grad()));
-    at::AutoDispatchBelowAutograd below;
-    OnDevice on(xs);
-    const NormOperands o = norm_operands(kind, xs, ws, bs, eps, offset, round_xhat);
-    const Tensor dy = as_rows(grad, o.p.hidden);
     const bool need_w = ws.defined() && task_should_compute_output(1), need_b = bs.defined() && task_should_compute_output(2);
-    Tensor dx = at::empty(xs.sizes(), xs.options().memory_format(at::MemoryFormat::Contiguous)), dw, db, workspace;
-    size_t bytes = 0;
-    if (need_w) dw = at::empty_like(o.w);
-    if (need_b) db = at::empty_like(o.b);
-    if (need_w || need_b) {
-      bytes = g_lib.norm_workspace_bytes(&o.p);
-      workspace = at::empty({static_cast<int64_t>(bytes)}, xs.options().dtype(at::kByte));
-    }
-    const float* rstd = stats.const_data_ptr<float>();
-    check(g_lib.norm_backward(&o.p, dy.const_data_ptr(), dy.stride(0), kind == FLCE_LAYER_NORM ? rstd + o.p.n_rows : nullptr, rstd,
-                              dx.data_ptr(), need_w ? dw.data_ptr() : nullptr, need_b ? db.data_ptr() : nullptr,
-                              workspace.defined() ? workspace.data_ptr() : nullptr, bytes, on.stream));
-    if (task_should_compute_output(0)) out[0] = dx;
-    if (need_w) out[1] = dw.to(ws.scalar_type());
-    if (need_b) out[2] = db.to(bs.scalar_type());
-    return once_differentiable(std::move(out), recording);
+    std::tie(out[0], out[1], out[2]) = backward.call(grad, xs, ws, bs, stats, kind, eps, offset, round_xhat, need_w, need_b);
+    if (!task_should_compute_output(0)) out[0] = Tensor();
+    return out;
   }
 };
 
-Tensor norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, int64_t kind, double eps, double offset,
-            bool round_xhat) {
+std::tuple<Tensor, Tensor> norm_with_statistics(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, int64_t kind,
+                                                double eps, double offset, bool round_xhat) {
+  static const auto next = operator_of<decltype(norm_with_statistics_launch)>("liger_b200::_norm_with_statistics");
   const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
   for (const Tensor* t : {&x, &w, &b}) refuse_tangent(*t);
-  const bool recording = torch::autograd::compute_requires_grad(x, w, b);
   Tensor y, stats;
   {
     at::AutoDispatchBelowAutograd below;
-    const NormOperands o = norm_operands(kind, x, w, b, eps, offset, round_xhat);
-    OnDevice on(x);
-    y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
-    float *rstd = nullptr, *mean = nullptr;
-    if (recording) {
-      stats = at::empty({kind == FLCE_LAYER_NORM ? 2 : 1, o.p.n_rows}, x.options().dtype(at::kFloat));
-      rstd = stats.data_ptr<float>();
-      mean = kind == FLCE_LAYER_NORM ? rstd + o.p.n_rows : nullptr;
-    }
-    check(g_lib.norm_forward(&o.p, y.data_ptr(), mean, rstd, on.stream));
+    std::tie(y, stats) = next.call(x, weight, bias, kind, eps, offset, round_xhat);
   }
-  if (recording) {
+  if (torch::autograd::compute_requires_grad(x, w, b)) {
     auto node = std::shared_ptr<NormBackward>(new NormBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(x, w, b));
     node->x = SavedVariable(x, false);
@@ -225,7 +275,19 @@ Tensor norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tens
     node->round_xhat = round_xhat;
     torch::autograd::set_history(y, node);
   }
-  return y;
+  return {y, stats};
+}
+
+// the row statistics are kept only where a gradient may be asked for
+Tensor norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, int64_t kind, double eps, double offset,
+            bool round_xhat) {
+  static const auto next = operator_of<decltype(norm_launch)>("liger_b200::norm");
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  if (torch::autograd::compute_requires_grad(x, w, b))
+    return std::get<0>(norm_with_statistics(x, weight, bias, kind, eps, offset, round_xhat));
+  for (const Tensor* t : {&x, &w, &b}) refuse_tangent(*t);
+  at::AutoDispatchBelowAutograd below;
+  return next.call(x, weight, bias, kind, eps, offset, round_xhat);
 }
 
 // ------------------------------------------------------------------ the router's load-balancing loss
@@ -284,6 +346,49 @@ Tensor piece_of(const Tensor& whole, int64_t offset, at::IntArrayRef sizes) {
   return t;
 }
 
+// loss, its lse^2 term, counts [layers, experts], and what backward needs: [experts + 1] fp32
+std::tuple<Tensor, Tensor, Tensor, Tensor> balance_launch(at::TensorList logits, int64_t num_experts, int64_t top_k,
+                                                          const optional<Tensor>& attention_mask, double lse_square_scale) {
+  const BalanceOperands o = balance_operands(logits, num_experts, top_k, attention_mask.value_or(Tensor()), lse_square_scale);
+  OnDevice on(logits[0]);
+  const auto options = o.logits[0].options();
+  // one buffer for the three in fp32
+  const Tensor out = at::empty({num_experts + 3}, options.dtype(at::kFloat));
+  const Tensor counts = at::empty({o.p.n_layers, num_experts}, options.dtype(at::kLong));
+  const size_t bytes = g_lib.balance_workspace_bytes(&o.p);
+  const Tensor workspace = at::empty({static_cast<int64_t>(bytes)}, options.dtype(at::kByte));
+  check(g_lib.balance_forward(&o.p, o.pointers.data(), out.data_ptr<float>(), counts.data_ptr<int64_t>(), out.data_ptr<float>() + 2,
+                              workspace.data_ptr(), bytes, on.stream));
+  return {piece_of(out, 0, {}), piece_of(out, 1, {}), counts, piece_of(out, 2, {num_experts + 1})};
+}
+
+// the gradients of all layers' logits, pieces of one buffer
+std::vector<Tensor> balance_backward_launch(const Tensor& grad, at::TensorList logits, const optional<Tensor>& attention_mask,
+                                            const Tensor& coef, int64_t num_experts, int64_t top_k, double lse_square_scale) {
+  OnDevice on(logits[0]);
+  const BalanceOperands o = balance_operands(logits, num_experts, top_k, attention_mask.value_or(Tensor()), lse_square_scale);
+  const Tensor up = grad.to(at::kFloat).contiguous();
+  Tensor all = at::empty({o.p.n_layers, o.p.n_tokens, num_experts}, logits[0].options().memory_format(at::MemoryFormat::Contiguous));
+  check(g_lib.balance_backward(&o.p, o.pointers.data(), coef.const_data_ptr<float>(), up.const_data_ptr<float>(), all.data_ptr(),
+                               on.stream));
+  std::vector<Tensor> out;
+  out.reserve(logits.size());
+  for (size_t l = 0; l < logits.size(); ++l)
+    out.push_back(piece_of(all, static_cast<int64_t>(l) * o.p.n_tokens * num_experts, logits[l].sizes()));
+  return out;
+}
+
+std::vector<Tensor> balance_backward(const Tensor& grad, at::TensorList logits, const optional<Tensor>& attention_mask, const Tensor& coef,
+                                     int64_t num_experts, int64_t top_k, double lse_square_scale) {
+  static const auto next = operator_of<decltype(balance_backward_launch)>("liger_b200::_load_balancing_loss_backward");
+  variable_list out;
+  {
+    at::AutoDispatchBelowAutograd below;
+    out = next.call(grad, logits, attention_mask, coef, num_experts, top_k, lse_square_scale);
+  }
+  return once_differentiable(std::move(out), grad, logits);
+}
+
 struct BalanceBackward : public torch::autograd::Node {
   std::vector<SavedVariable> logits;
   SavedVariable mask;
@@ -300,74 +405,86 @@ struct BalanceBackward : public torch::autograd::Node {
   }
 
   variable_list apply(variable_list&& grads) override {
+    static const auto backward = operator_of<decltype(balance_backward_launch)>("liger_b200::_load_balancing_loss_backward");
     std::lock_guard<std::mutex> lock(mutex_);
-    variable_list out(logits.size());
     const Tensor& grad = grads[0];
-    if (!grad.defined()) return out;
-    std::vector<Tensor> x;
-    bool recording = grad.requires_grad();
-    for (auto& t : logits) {
-      x.push_back(t.unpack());
-      recording = recording || x.back().requires_grad();
-    }
+    if (!grad.defined()) return variable_list(logits.size());
+    variable_list x;
+    x.reserve(logits.size());
+    for (auto& t : logits) x.push_back(t.unpack());
     const Tensor m = mask.unpack();
     TORCH_CHECK(coef.defined(), torch::autograd::ERR_BACKWARD_TWICE);
-    recording = recording && at::GradMode::is_enabled();
-    at::AutoDispatchBelowAutograd below;
-    OnDevice on(x[0]);
-    const BalanceOperands o = balance_operands(x, num_experts, top_k, m, lse_square_scale);
-    const Tensor up = grad.to(at::kFloat).contiguous();
-    Tensor all = at::empty({o.p.n_layers, o.p.n_tokens, num_experts}, x[0].options().memory_format(at::MemoryFormat::Contiguous));
-    check(g_lib.balance_backward(&o.p, o.pointers.data(), coef.const_data_ptr<float>(), up.const_data_ptr<float>(), all.data_ptr(),
-                                 on.stream));
-    for (size_t l = 0; l < x.size(); ++l) {
-      if (task_should_compute_output(l)) out[l] = piece_of(all, static_cast<int64_t>(l) * o.p.n_tokens * num_experts, x[l].sizes());
+    variable_list out = backward.call(grad, x, m, coef, num_experts, top_k, lse_square_scale);
+    for (size_t l = 0; l < out.size(); ++l) {
+      if (!task_should_compute_output(l)) out[l] = Tensor();
     }
-    return once_differentiable(std::move(out), recording);
+    return out;
   }
 };
 
-// loss, its lse^2 term, counts [layers, experts]
-std::tuple<Tensor, Tensor, Tensor> load_balancing_loss(at::TensorList logits, int64_t num_experts, int64_t top_k,
-                                                       const optional<Tensor>& attention_mask, double lse_square_scale) {
-  const Tensor mask = attention_mask.value_or(Tensor());
+std::tuple<Tensor, Tensor, Tensor, Tensor> balance(at::TensorList logits, int64_t num_experts, int64_t top_k,
+                                                   const optional<Tensor>& attention_mask, double lse_square_scale) {
+  static const auto next = operator_of<decltype(balance_launch)>("liger_b200::_load_balancing_loss");
   for (const Tensor& t : logits) refuse_tangent(t);
-  const bool recording = torch::autograd::compute_requires_grad(logits);
   Tensor loss, z_loss, counts, coef;
   {
     at::AutoDispatchBelowAutograd below;
-    const BalanceOperands o = balance_operands(logits, num_experts, top_k, mask, lse_square_scale);
-    OnDevice on(logits[0]);
-    const auto options = o.logits[0].options();
-    // one buffer for the loss, its lse^2 term and what backward needs
-    const Tensor out = at::empty({num_experts + 3}, options.dtype(at::kFloat));
-    counts = at::empty({o.p.n_layers, num_experts}, options.dtype(at::kLong));
-    const size_t bytes = g_lib.balance_workspace_bytes(&o.p);
-    const Tensor workspace = at::empty({static_cast<int64_t>(bytes)}, options.dtype(at::kByte));
-    check(g_lib.balance_forward(&o.p, o.pointers.data(), out.data_ptr<float>(), counts.data_ptr<int64_t>(), out.data_ptr<float>() + 2,
-                                workspace.data_ptr(), bytes, on.stream));
-    loss = piece_of(out, 0, {});
-    z_loss = piece_of(out, 1, {});
-    if (recording) coef = piece_of(out, 2, {num_experts + 1});
+    std::tie(loss, z_loss, counts, coef) = next.call(logits, num_experts, top_k, attention_mask, lse_square_scale);
   }
-  if (recording) {
+  if (torch::autograd::compute_requires_grad(logits)) {
     auto node = std::shared_ptr<BalanceBackward>(new BalanceBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(logits));
+    node->logits.reserve(logits.size());
     for (const Tensor& t : logits) node->logits.emplace_back(t, false);
-    node->mask = SavedVariable(mask, false);
+    node->mask = SavedVariable(attention_mask.value_or(Tensor()), false);
     node->coef = coef;
     node->num_experts = num_experts;
     node->top_k = top_k;
     node->lse_square_scale = lse_square_scale;
     torch::autograd::set_history(loss, node);
   }
+  return {loss, z_loss, counts, coef};
+}
+
+// loss, its lse^2 term, counts [layers, experts]: a composite, without a kernel of its own
+std::tuple<Tensor, Tensor, Tensor> load_balancing_loss(at::TensorList logits, int64_t num_experts, int64_t top_k,
+                                                       const optional<Tensor>& attention_mask, double lse_square_scale) {
+  static const auto forward = operator_of<decltype(balance_launch)>("liger_b200::_load_balancing_loss");
+  TORCH_CHECK_VALUE(!logits.empty(), "expected the router logits of at least one layer");      // the dispatch goes by their device
+  auto [loss, z_loss, counts, coef] = forward.call(logits, num_experts, top_k, attention_mask, lse_square_scale);
   return {loss, z_loss, counts};
 }
 
 TORCH_LIBRARY(liger_b200, m) {
   m.def("load_balancing_loss(Tensor[] logits, int num_experts, int top_k, Tensor? attention_mask, float lse_square_scale) -> "
         "(Tensor, Tensor, Tensor)", load_balancing_loss);
-  m.def("norm(Tensor x, Tensor? weight, Tensor? bias, int kind, float eps, float offset, bool round_xhat) -> Tensor", norm);
+  m.def("norm(Tensor x, Tensor? weight, Tensor? bias, int kind, float eps, float offset, bool round_xhat) -> Tensor");
+  m.def("_norm_with_statistics(Tensor x, Tensor? weight, Tensor? bias, int kind, float eps, float offset, bool round_xhat) -> "
+        "(Tensor, Tensor)");
+  m.def("_norm_backward(Tensor grad, Tensor x, Tensor? weight, Tensor? bias, Tensor statistics, int kind, float eps, float offset, "
+        "bool round_xhat, bool need_weight, bool need_bias) -> (Tensor, Tensor, Tensor)");
+  m.def("_load_balancing_loss(Tensor[] logits, int num_experts, int top_k, Tensor? attention_mask, float lse_square_scale) -> "
+        "(Tensor, Tensor, Tensor, Tensor)");
+  m.def("_load_balancing_loss_backward(Tensor grad, Tensor[] logits, Tensor? attention_mask, Tensor coefficients, int num_experts, "
+        "int top_k, float lse_square_scale) -> Tensor[]");
+}
+
+// Tensors on the CPU get as far as require_device, which knows whether the library computes there.
+void register_launches(torch::Library& m) {
+  m.impl("norm", norm_launch);
+  m.impl("_norm_with_statistics", norm_with_statistics_launch);
+  m.impl("_norm_backward", norm_backward_launch);
+  m.impl("_load_balancing_loss", balance_launch);
+  m.impl("_load_balancing_loss_backward", balance_backward_launch);
+}
+TORCH_LIBRARY_IMPL(liger_b200, CUDA, m) { register_launches(m); }
+TORCH_LIBRARY_IMPL(liger_b200, CPU, m) { register_launches(m); }
+TORCH_LIBRARY_IMPL(liger_b200, Autograd, m) {
+  m.impl("norm", norm);
+  m.impl("_norm_with_statistics", norm_with_statistics);
+  m.impl("_norm_backward", norm_backward);
+  m.impl("_load_balancing_loss", balance);
+  m.impl("_load_balancing_loss_backward", balance_backward);
 }
 
 }  // namespace

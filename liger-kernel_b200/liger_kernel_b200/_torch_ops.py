@@ -37,5 +37,39 @@ def _load():
 
 _binding = _load()
 bind(_lib.LIB_PATH)
+
+
+# What the operators that launch kernels return, for tracers that run without data (torch.compile, torch.export, make_fx).
+
+
+@torch.library.register_fake("liger_b200::norm")
+def _(x, weight, bias, kind, eps, offset, round_xhat):
+    return x.new_empty(x.shape)
+
+
+@torch.library.register_fake("liger_b200::_norm_with_statistics")
+def _(x, weight, bias, kind, eps, offset, round_xhat):
+    planes = 2 if kind == _lib.FLCE_LAYER_NORM else 1
+    return x.new_empty(x.shape), x.new_empty((planes, x.numel() // x.shape[-1]), dtype=torch.float32)
+
+
+@torch.library.register_fake("liger_b200::_norm_backward")
+def _(grad, x, weight, bias, statistics, kind, eps, offset, round_xhat, need_weight, need_bias):
+    return (x.new_empty(x.shape), weight.new_empty(weight.shape) if need_weight else None,
+            bias.new_empty(bias.shape) if need_bias else None)
+
+
+@torch.library.register_fake("liger_b200::_load_balancing_loss")
+def _(logits, num_experts, top_k, attention_mask, lse_square_scale):
+    x = logits[0]
+    return (x.new_empty((), dtype=torch.float32), x.new_empty((), dtype=torch.float32),
+            x.new_empty((len(logits), num_experts), dtype=torch.int64), x.new_empty((num_experts + 1,), dtype=torch.float32))
+
+
+@torch.library.register_fake("liger_b200::_load_balancing_loss_backward")
+def _(grad, logits, attention_mask, coefficients, num_experts, top_k, lse_square_scale):
+    return [t.new_empty(t.shape) for t in logits]
+
+
 norm = torch.ops.liger_b200.norm.default
 load_balancing_loss = torch.ops.liger_b200.load_balancing_loss.default

@@ -1,0 +1,158 @@
+"""Shared bodies of the tests that trace, compile and transform the norms and the router's balance loss: what the tracers record, and
+what torch.func's transforms compute, has to be what the operators compute when they are called.  Run on a B200
+(tests/test_tracing_gpu.py) and, with the library's host side and kernels emulated, on CPU tensors
+(tests/test_tracing_emulation_cpu.py).  The same kernels run on the same rows either way: results agree bit for bit, unless
+the rows are grouped differently (vmap calls once per slice), where only sums over the rows move by roundings."""
+
+import torch
+from torch.fx.experimental.proxy_tensor import make_fx
+
+EXPERTS, TOP_K = 24, 3
+
+
+def _operators():
+    import liger_kernel_b200 as lk
+
+    return {
+        "layer": lambda x, w, b: lk.liger_layer_norm(x, w, b, 1e-6),
+        "rms": lambda x, w, b: lk.liger_rms_norm(x, w, 1e-6) + b,
+        "balance": lambda x, w, b: lk.liger_load_balancing_loss((x, x * w + b), EXPERTS, TOP_K, lse_square_scale=1e-3),
+    }
+
+
+def _inputs(device, rows, seed, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(rows, EXPERTS, generator=g).to(dtype).to(device)] + [torch.randn(EXPERTS, generator=g).to(dtype).to(device) for _ in range(2)]
+
+
+def _gradients(f, args, allow_unused=False):
+    args = [t.detach().clone().requires_grad_(True) for t in args]
+    y = f(*args)
+    up = torch.linspace(0.5, 1.5, y.numel(), device=y.device).reshape(y.shape).to(y.dtype)
+    return y.detach(), torch.autograd.grad(y, args, up, allow_unused=allow_unused)
+
+
+def case_make_fx(device, name, mode):
+    """The traced program, run on other inputs, forward and backward."""
+    f = _operators()[name]
+    first, second = _inputs(device, 10, 1), _inputs(device, 10, 2)
+    forward = make_fx(f, tracing_mode=mode)(*first)
+    assert torch.equal(forward(*second), f(*second))
+    assert not torch.equal(forward(*second), f(*first))
+
+    def step(x, w, b):
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y = f(*leaves)
+        return (y.detach(), *torch.autograd.grad(y.sum(), leaves))
+
+    traced = make_fx(step, tracing_mode=mode)(*first)
+    for got, want in zip(traced(*second), step(*second)):
+        assert got.shape == want.shape and got.dtype == want.dtype and torch.equal(got, want)
+
+
+def case_make_fx_of_a_bare_norm(device):
+    """Without parameters, where the graph has nothing but the operator in it."""
+    import liger_kernel_b200 as lk
+
+    for f in (lambda x: lk.liger_layer_norm(x), lambda x: lk.liger_rms_norm(x), lambda x: lk.liger_load_balancing_loss(x, EXPERTS)):
+        a, b = (_inputs(device, 5, s)[0] for s in (3, 4))
+        assert torch.equal(make_fx(f)(a)(b), f(b))
+
+
+def case_compile(device, name, backend="aot_eager"):
+    """One graph, forward and backward, also where the number of rows is symbolic."""
+    f = _operators()[name]
+    torch._dynamo.reset()
+    compiled = torch.compile(f, backend=backend, fullgraph=True)
+    for rows in (10, 13, 7):                       # the second size makes the number of rows symbolic
+        args = _inputs(device, rows, rows)
+        (y, grads), (want, want_grads) = _gradients(compiled, args), _gradients(f, args)
+        assert torch.equal(y, want) and all(torch.equal(p, q) for p, q in zip(grads, want_grads))
+    with torch.no_grad():
+        assert torch.equal(compiled(*_inputs(device, 10, 5)), f(*_inputs(device, 10, 5)))
+    torch._dynamo.reset()
+
+
+def case_compile_modules(device, backend="aot_eager"):
+    """The modules inside a model, in the rows' type and with fp32 parameters beside bf16 rows, with a mask and all outputs."""
+    import liger_kernel_b200 as lk
+
+    torch._dynamo.reset()
+    torch.manual_seed(0)
+
+    class Block(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.norm, self.rms = lk.LigerLayerNorm(EXPERTS, bias=True), lk.LigerRMSNorm(EXPERTS, offset=1.0)
+            self.bare = lk.LigerRMSNorm(EXPERTS, elementwise_affine=False, casting_mode="gemma")
+            self.balance = lk.LigerLoadBalancingLoss(EXPERTS, TOP_K, lse_square_scale=1e-2, return_z_loss=True, return_expert_counts=True)
+
+        def forward(self, x, mask):
+            h = self.bare(self.rms(self.norm(x)))
+            out = self.balance((h, h * 0.5), mask)
+            return h, out.loss, out.z_loss, out.expert_counts
+
+    for dtype in (torch.float32, torch.bfloat16):
+        block = Block().to(device)
+        compiled = torch.compile(block, backend=backend, fullgraph=True)
+        x = _inputs(device, 12, 8, dtype)[0].reshape(3, 4, EXPERTS)
+        mask = torch.ones(3, 4, dtype=torch.int64, device=device)
+        mask[1, 2:] = 0
+        results = []
+        for fn in (block, compiled):
+            xx = x.clone().requires_grad_(True)
+            block.zero_grad()
+            h, loss, z_loss, counts = fn(xx, mask)
+            assert counts.dtype == torch.int64 and not z_loss.requires_grad
+            (loss + h.float().square().sum()).backward()
+            results.append([h.detach(), loss.detach(), z_loss, counts, xx.grad, *[p.grad for p in block.parameters()]])
+        for got, want in zip(results[1], results[0]):
+            assert got.dtype == want.dtype and torch.equal(got, want)
+    torch._dynamo.reset()
+
+
+def case_meta(device):
+    """Shapes and types without data."""
+    import liger_kernel_b200 as lk
+
+    x = torch.empty(2, 5, EXPERTS, device="meta", dtype=torch.bfloat16, requires_grad=True)
+    w = torch.empty(EXPERTS, device="meta", requires_grad=True)
+    for y in (lk.liger_layer_norm(x, w, w), lk.liger_rms_norm(x, w)):
+        assert y.device.type == "meta" and y.shape == x.shape and y.dtype == x.dtype
+        dx, dw = torch.autograd.grad(y.sum(), (x, w))
+        assert dx.shape == x.shape and dx.dtype == x.dtype and dw.shape == w.shape and dw.dtype == w.dtype
+    out = lk.liger_load_balancing_loss((x, x), EXPERTS, TOP_K, return_expert_counts=True)
+    assert out.loss.shape == () and out.loss.dtype == torch.float32 and out.expert_counts.shape == (2, EXPERTS)
+    (dx,) = torch.autograd.grad(out.loss, (x,))
+    assert dx.shape == x.shape and dx.dtype == x.dtype
+
+
+def case_functional_gradients(device, name):
+    """torch.func.grad and vjp, and several upstream gradients at once."""
+    f = _operators()[name]
+    args = _inputs(device, 6, 11)
+    y, want = _gradients(f, args)
+    up = torch.linspace(0.5, 1.5, y.numel(), device=y.device).reshape(y.shape)
+    out, pull = torch.func.vjp(f, *args)
+    assert torch.equal(out, y) and all(torch.equal(p, q) for p, q in zip(pull(up), want))
+    grads = torch.func.grad(lambda *a: (f(*a) * up).sum(), argnums=(0, 1, 2))(*args)
+    assert all(torch.equal(p, q) for p, q in zip(grads, want))
+    if name != "balance":                          # torch's loop for operators without a batching rule takes no lists of tensors
+        leaves = [t.clone().requires_grad_(True) for t in args]
+        y = f(*leaves)
+        ups = torch.stack([up, 2 * up, -up])
+        batched = torch.autograd.grad(y, leaves, ups, is_grads_batched=True)
+        for got, ref in zip(batched, want):
+            for k, scale in enumerate((1.0, 2.0, -1.0)):
+                assert torch.equal(got[k], ref * scale)          # multiplying by a power of two commutes with every rounding
+        stacked = torch.stack(_inputs(device, 6, 12)[:1] + args[:1])
+        assert torch.equal(torch.vmap(f, in_dims=(0, None, None))(stacked, *args[1:]), torch.stack([f(t, *args[1:]) for t in stacked]))
+
+
+def case_second_derivative_is_refused(device):
+    import pytest
+
+    for name, f in _operators().items():
+        args = _inputs(device, 6, 11)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            torch.func.grad(lambda x: torch.func.grad(lambda t: f(t, *args[1:]).square().sum())(x).sum())(args[0])
