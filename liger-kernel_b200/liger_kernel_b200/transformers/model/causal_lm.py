@@ -16,6 +16,7 @@ from typing import Optional
 
 import torch
 
+from torch.autograd import forward_ad
 from transformers.modeling_outputs import CausalLMOutputWithPast, MoeCausalLMOutputWithPast
 
 from ..fsdp import run_inside_fsdp_forward
@@ -148,17 +149,37 @@ def _mixtral_balancing_loss():
     return router_balancing_loss
 
 
+def _on_gpu(t):
+    return t.is_cuda
+
+
+def _operator_takes(router_logits, num_experts, top_k, attention_mask):
+    """Whether ``liger_load_balancing_loss`` computes what the model library's function would.  It needs plain tensors (distributed
+    ones and those of torch.func's transforms are wrappers), of one shape and type, without forward-mode tangents; masks of one
+    integer or truth value per token."""
+    if torch.compiler.is_compiling() or not isinstance(router_logits, tuple) or len(router_logits) == 0:
+        return False
+    head = router_logits[0]
+    if type(head) is not torch.Tensor or head.dim() != 2 or head.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        return False
+    if head.shape[1] != num_experts or not 1 <= top_k <= num_experts <= 1024:
+        return False
+    if attention_mask is not None and (type(attention_mask) is not torch.Tensor or attention_mask.is_floating_point()
+                                       or attention_mask.dim() != 2 or attention_mask.numel() != head.shape[0]):
+        return False
+    return all(type(t) is torch.Tensor and _on_gpu(t) and t.shape == head.shape and t.dtype == head.dtype
+               and not torch._C._functorch.is_functorch_wrapped_tensor(t) and forward_ad.unpack_dual(t).tangent is None
+               for t in router_logits)
+
+
 def router_balancing_loss(router_logits, num_experts, top_k, attention_mask=None):
     """The router's auxiliary loss of the mixture-of-experts families: ``liger_load_balancing_loss`` for router logits on the GPU,
-    the model library's own function for what that does not cover (logits on the CPU, masks that are not one element per
-    token, more than 1024 experts, a forward that is being traced by torch.compile)."""
-    if not torch.compiler.is_compiling() and isinstance(router_logits, (tuple, list)) and len(router_logits) > 0 and num_experts <= 1024:
-        head = router_logits[0]
-        tokens = head.numel() // num_experts
-        one_per_token = attention_mask is None or (attention_mask.dim() == 2 and attention_mask.numel() == tokens)
-        if head.is_cuda and head.dtype in (torch.bfloat16, torch.float16, torch.float32) and one_per_token:
-            # layers of a model that is spread over devices meet on the first one, as in the library's function
-            return liger_load_balancing_loss(tuple(t.to(head.device) for t in router_logits), num_experts, top_k, attention_mask)
+    the model library's own function for what that does not cover and in a forward that torch.compile traces.  A mask's integers
+    are 0 or 1, as the model library documents them; the weights of a floating-point mask are left to its function."""
+    if _operator_takes(router_logits, num_experts, top_k, attention_mask):
+        # layers of a model that is spread over devices meet on the first one, as in the library's function
+        device = router_logits[0].device
+        return liger_load_balancing_loss(tuple(t.to(device) for t in router_logits), num_experts, top_k, attention_mask)
     from transformers.models.mixtral.modeling_mixtral import load_balancing_loss_func
 
     return load_balancing_loss_func(router_logits, num_experts, top_k, attention_mask)
