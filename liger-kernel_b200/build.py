@@ -9,6 +9,7 @@ nvcc cross-compiles, so no GPU is needed to build.
 import argparse
 import importlib.util
 import os
+import runpy
 import shutil
 import subprocess
 import sys
@@ -29,9 +30,20 @@ def _deps():
     return deps
 
 
+def _torch_dir():
+    return os.path.dirname(importlib.util.find_spec("torch").origin)
+
+
+def _torch_version():
+    return runpy.run_path(os.path.join(_torch_dir(), "version.py"))["__version__"]
+
+
 def needs_build():
     if not (os.path.exists(OUT) and os.path.exists(BINDING)):
         return True
+    with open(BINDING, "rb") as f:
+        if f"liger_b200 built against torch {_torch_version()};".encode() not in f.read():
+            return True
     built = min(os.path.getmtime(OUT), os.path.getmtime(BINDING))
     return any(os.path.getmtime(d) > built for d in _deps())
 
@@ -66,11 +78,11 @@ def build(force=False, verbose=False, trace=False):
 
 
 def _binding_command(nvcc):
-    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    torch_dir = _torch_dir()
     cuda_dir = os.environ.get("CUDA_HOME") or os.path.dirname(os.path.dirname(os.path.realpath(nvcc)))
     include = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
                os.path.join(cuda_dir, "include"), os.path.join(ROOT, "include")]
-    return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared"] + [f"-I{d}" for d in include] + ["-o", BINDING, BINDING_SOURCE]
+    return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f'-DLIGER_TORCH_VERSION="{_torch_version()}"'] + [f"-I{d}" for d in include] + ["-o", BINDING, BINDING_SOURCE]
             + [f"-L{os.path.join(torch_dir, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ldl"])
 
 

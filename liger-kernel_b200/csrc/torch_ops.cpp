@@ -489,6 +489,9 @@ TORCH_LIBRARY_IMPL(liger_b200, Autograd, m) {
 
 }  // namespace
 
+// torch's C++ interface changes between its versions: the Python side looks for this in the file before it loads it.
+extern "C" __attribute__((used)) const char liger_b200_built_against[] = "liger_b200 built against torch " LIGER_TORCH_VERSION ";";
+
 // Looks the entry points up in the library at `path` (one that is loaded already is not loaded again); host_memory: it is the
 // tests' emulation.  Returns nullptr, or what is missing.  The string is valid until the thread's next call.
 extern "C" const char* liger_b200_bind(const char* path, int host_memory) {
