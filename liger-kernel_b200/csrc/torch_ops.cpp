@@ -346,53 +346,67 @@ Tensor piece_of(const Tensor& whole, int64_t offset, at::IntArrayRef sizes) {
   return t;
 }
 
-// loss, its lse^2 term, counts [layers, experts], and what backward needs: [experts + 1] fp32
-std::tuple<Tensor, Tensor, Tensor, Tensor> balance_launch(at::TensorList logits, int64_t num_experts, int64_t top_k,
-                                                          const optional<Tensor>& attention_mask, double lse_square_scale) {
+// One fp32 buffer: what backward needs, [experts + 1], then the loss and its lse^2 term.
+int64_t loss_at(int64_t num_experts) { return num_experts + 1; }
+
+// that buffer and the counts, [layers, experts]
+std::tuple<Tensor, Tensor> balance_launch(at::TensorList logits, int64_t num_experts, int64_t top_k, const optional<Tensor>& attention_mask,
+                                          double lse_square_scale) {
   const BalanceOperands o = balance_operands(logits, num_experts, top_k, attention_mask.value_or(Tensor()), lse_square_scale);
   OnDevice on(logits[0]);
   const auto options = o.logits[0].options();
-  // one buffer for the three in fp32
-  const Tensor out = at::empty({num_experts + 3}, options.dtype(at::kFloat));
+  const Tensor values = at::empty({loss_at(num_experts) + 2}, options.dtype(at::kFloat));
   const Tensor counts = at::empty({o.p.n_layers, num_experts}, options.dtype(at::kLong));
   const size_t bytes = g_lib.balance_workspace_bytes(&o.p);
   const Tensor workspace = at::empty({static_cast<int64_t>(bytes)}, options.dtype(at::kByte));
-  check(g_lib.balance_forward(&o.p, o.pointers.data(), out.data_ptr<float>(), counts.data_ptr<int64_t>(), out.data_ptr<float>() + 2,
-                              workspace.data_ptr(), bytes, on.stream));
-  return {piece_of(out, 0, {}), piece_of(out, 1, {}), counts, piece_of(out, 2, {num_experts + 1})};
+  float* f = values.data_ptr<float>();
+  check(g_lib.balance_forward(&o.p, o.pointers.data(), f + loss_at(num_experts), counts.data_ptr<int64_t>(), f, workspace.data_ptr(), bytes,
+                              on.stream));
+  return {values, counts};
 }
 
-// the gradients of all layers' logits, pieces of one buffer
-std::vector<Tensor> balance_backward_launch(const Tensor& grad, at::TensorList logits, const optional<Tensor>& attention_mask,
-                                            const Tensor& coef, int64_t num_experts, int64_t top_k, double lse_square_scale) {
+// the gradients of all layers' logits: [layers, tokens, experts]
+Tensor balance_backward_launch(const Tensor& grad, at::TensorList logits, const optional<Tensor>& attention_mask, const Tensor& values,
+                               int64_t num_experts, int64_t top_k, double lse_square_scale) {
   OnDevice on(logits[0]);
   const BalanceOperands o = balance_operands(logits, num_experts, top_k, attention_mask.value_or(Tensor()), lse_square_scale);
   const Tensor up = grad.to(at::kFloat).contiguous();
   Tensor all = at::empty({o.p.n_layers, o.p.n_tokens, num_experts}, logits[0].options().memory_format(at::MemoryFormat::Contiguous));
-  check(g_lib.balance_backward(&o.p, o.pointers.data(), coef.const_data_ptr<float>(), up.const_data_ptr<float>(), all.data_ptr(),
+  check(g_lib.balance_backward(&o.p, o.pointers.data(), values.const_data_ptr<float>(), up.const_data_ptr<float>(), all.data_ptr(),
                                on.stream));
-  std::vector<Tensor> out;
-  out.reserve(logits.size());
-  for (size_t l = 0; l < logits.size(); ++l)
-    out.push_back(piece_of(all, static_cast<int64_t>(l) * o.p.n_tokens * num_experts, logits[l].sizes()));
-  return out;
+  return all;
 }
 
-std::vector<Tensor> balance_backward(const Tensor& grad, at::TensorList logits, const optional<Tensor>& attention_mask, const Tensor& coef,
-                                     int64_t num_experts, int64_t top_k, double lse_square_scale) {
+Tensor balance_backward(const Tensor& grad, at::TensorList logits, const optional<Tensor>& attention_mask, const Tensor& values,
+                        int64_t num_experts, int64_t top_k, double lse_square_scale) {
   static const auto next = operator_of<decltype(balance_backward_launch)>("liger_b200::_load_balancing_loss_backward");
-  variable_list out;
+  variable_list out(1);
   {
     at::AutoDispatchBelowAutograd below;
-    out = next.call(grad, logits, attention_mask, coef, num_experts, top_k, lse_square_scale);
+    out[0] = next.call(grad, logits, attention_mask, values, num_experts, top_k, lse_square_scale);
   }
-  return once_differentiable(std::move(out), grad, logits);
+  return once_differentiable(std::move(out), grad, logits)[0];
+}
+
+// Whether nobody but autograd sees what is done with the tensors: no tracer, no mode, no transform, no wrapper around them.
+bool is_plain(at::TensorList tensors) {
+  using c10::DispatchKey;
+  static const c10::DispatchKeySet usual =
+      c10::DispatchKeySet({DispatchKey::CUDA, DispatchKey::CPU, DispatchKey::BackendSelect, DispatchKey::ADInplaceOrView,
+                           DispatchKey::AutogradCUDA, DispatchKey::AutogradCPU, DispatchKey::AutocastCUDA, DispatchKey::AutocastCPU});
+  c10::DispatchKeySet keys = c10::impl::tls_local_dispatch_key_set().included_;
+  for (const Tensor& t : tensors) {
+    if (!t.is_cuda() && !t.is_cpu()) return false;
+    keys = keys | t.key_set();
+  }
+  return ((keys - usual).raw_repr() & ~c10::full_backend_mask) == 0;      // the difference keeps the backends' bits
 }
 
 struct BalanceBackward : public torch::autograd::Node {
   std::vector<SavedVariable> logits;
   SavedVariable mask;
-  Tensor coef;
+  Tensor values;
+  bool of_values = false;       // the node stands behind the buffer, not behind the loss cut from it
   int64_t num_experts = 0, top_k = 0;
   double lse_square_scale = 0;
 
@@ -401,57 +415,81 @@ struct BalanceBackward : public torch::autograd::Node {
   void release_variables() override {
     for (auto& t : logits) t.reset_data();
     mask.reset_data();
-    coef.reset();
+    values.reset();
   }
 
   variable_list apply(variable_list&& grads) override {
     static const auto backward = operator_of<decltype(balance_backward_launch)>("liger_b200::_load_balancing_loss_backward");
     std::lock_guard<std::mutex> lock(mutex_);
-    const Tensor& grad = grads[0];
-    if (!grad.defined()) return variable_list(logits.size());
+    if (!grads[0].defined()) return variable_list(logits.size());
+    const Tensor grad = of_values ? grads[0].select(0, loss_at(num_experts)) : grads[0];
     variable_list x;
     x.reserve(logits.size());
     for (auto& t : logits) x.push_back(t.unpack());
     const Tensor m = mask.unpack();
-    TORCH_CHECK(coef.defined(), torch::autograd::ERR_BACKWARD_TWICE);
-    variable_list out = backward.call(grad, x, m, coef, num_experts, top_k, lse_square_scale);
-    for (size_t l = 0; l < out.size(); ++l) {
-      if (!task_should_compute_output(l)) out[l] = Tensor();
+    TORCH_CHECK(values.defined(), torch::autograd::ERR_BACKWARD_TWICE);
+    const Tensor all = backward.call(grad, x, m, values, num_experts, top_k, lse_square_scale);
+    // The layers' pieces of it start on any boundary.  A compiler has to see where: through the dispatcher then, and also where
+    // the pieces need a history.
+    const bool quick = is_plain(all) && !all.requires_grad();
+    variable_list out(x.size());
+    for (size_t l = 0; l < x.size(); ++l) {
+      if (!task_should_compute_output(l)) continue;
+      out[l] = quick ? piece_of(all, static_cast<int64_t>(l) * all.stride(0), x[l].sizes())
+                     : all.select(0, static_cast<int64_t>(l)).view_symint(x[l].sym_sizes());
     }
     return out;
   }
 };
 
-std::tuple<Tensor, Tensor, Tensor, Tensor> balance(at::TensorList logits, int64_t num_experts, int64_t top_k,
-                                                   const optional<Tensor>& attention_mask, double lse_square_scale) {
-  static const auto next = operator_of<decltype(balance_launch)>("liger_b200::_load_balancing_loss");
-  for (const Tensor& t : logits) refuse_tangent(t);
-  Tensor loss, z_loss, counts, coef;
-  {
-    at::AutoDispatchBelowAutograd below;
-    std::tie(loss, z_loss, counts, coef) = next.call(logits, num_experts, top_k, attention_mask, lse_square_scale);
-  }
-  if (torch::autograd::compute_requires_grad(logits)) {
-    auto node = std::shared_ptr<BalanceBackward>(new BalanceBackward(), torch::autograd::deleteNode);
-    node->set_next_edges(torch::autograd::collect_next_edges(logits));
-    node->logits.reserve(logits.size());
-    for (const Tensor& t : logits) node->logits.emplace_back(t, false);
-    node->mask = SavedVariable(attention_mask.value_or(Tensor()), false);
-    node->coef = coef;
-    node->num_experts = num_experts;
-    node->top_k = top_k;
-    node->lse_square_scale = lse_square_scale;
-    torch::autograd::set_history(loss, node);
-  }
-  return {loss, z_loss, counts, coef};
+void set_balance_history(const Tensor& result, bool of_values, const Tensor& values, at::TensorList logits, int64_t num_experts,
+                         int64_t top_k, const optional<Tensor>& attention_mask, double lse_square_scale) {
+  auto node = std::shared_ptr<BalanceBackward>(new BalanceBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(logits));
+  node->logits.reserve(logits.size());
+  for (const Tensor& t : logits) node->logits.emplace_back(t, false);
+  node->mask = SavedVariable(attention_mask.value_or(Tensor()), false);
+  node->values = of_values ? values.detach() : values;
+  node->of_values = of_values;
+  node->num_experts = num_experts;
+  node->top_k = top_k;
+  node->lse_square_scale = lse_square_scale;
+  torch::autograd::set_history(result, node);
 }
 
-// loss, its lse^2 term, counts [layers, experts]: a composite, without a kernel of its own
+std::tuple<Tensor, Tensor> balance(at::TensorList logits, int64_t num_experts, int64_t top_k, const optional<Tensor>& attention_mask,
+                                   double lse_square_scale) {
+  static const auto next = operator_of<decltype(balance_launch)>("liger_b200::_load_balancing_loss");
+  for (const Tensor& t : logits) refuse_tangent(t);
+  Tensor values, counts;
+  {
+    at::AutoDispatchBelowAutograd below;
+    std::tie(values, counts) = next.call(logits, num_experts, top_k, attention_mask, lse_square_scale);
+  }
+  if (torch::autograd::compute_requires_grad(logits))
+    set_balance_history(values, true, values, logits, num_experts, top_k, attention_mask, lse_square_scale);
+  return {values, counts};
+}
+
+// loss, its lse^2 term, counts [layers, experts]: a composite.  Where nobody looks on, the two numbers are cut out without the
+// dispatcher and the node stands right behind the loss.
 std::tuple<Tensor, Tensor, Tensor> load_balancing_loss(at::TensorList logits, int64_t num_experts, int64_t top_k,
                                                        const optional<Tensor>& attention_mask, double lse_square_scale) {
   static const auto forward = operator_of<decltype(balance_launch)>("liger_b200::_load_balancing_loss");
   TORCH_CHECK_VALUE(!logits.empty(), "expected the router logits of at least one layer");      // the dispatch goes by their device
-  auto [loss, z_loss, counts, coef] = forward.call(logits, num_experts, top_k, attention_mask, lse_square_scale);
+  if (!is_plain(logits)) {
+    auto [values, counts] = forward.call(logits, num_experts, top_k, attention_mask, lse_square_scale);
+    return {values.select(0, loss_at(num_experts)), values.detach().select(0, loss_at(num_experts) + 1), counts};
+  }
+  for (const Tensor& t : logits) refuse_tangent(t);
+  Tensor values, counts;
+  {
+    at::AutoDispatchBelowAutograd below;
+    std::tie(values, counts) = forward.call(logits, num_experts, top_k, attention_mask, lse_square_scale);
+  }
+  const Tensor loss = piece_of(values, loss_at(num_experts), {}), z_loss = piece_of(values, loss_at(num_experts) + 1, {});
+  if (torch::autograd::compute_requires_grad(logits))
+    set_balance_history(loss, false, values, logits, num_experts, top_k, attention_mask, lse_square_scale);
   return {loss, z_loss, counts};
 }
 
@@ -464,9 +502,9 @@ TORCH_LIBRARY(liger_b200, m) {
   m.def("_norm_backward(Tensor grad, Tensor x, Tensor? weight, Tensor? bias, Tensor statistics, int kind, float eps, float offset, "
         "bool round_xhat, bool need_weight, bool need_bias) -> (Tensor, Tensor, Tensor)");
   m.def("_load_balancing_loss(Tensor[] logits, int num_experts, int top_k, Tensor? attention_mask, float lse_square_scale) -> "
-        "(Tensor, Tensor, Tensor, Tensor)");
-  m.def("_load_balancing_loss_backward(Tensor grad, Tensor[] logits, Tensor? attention_mask, Tensor coefficients, int num_experts, "
-        "int top_k, float lse_square_scale) -> Tensor[]");
+        "(Tensor, Tensor)");
+  m.def("_load_balancing_loss_backward(Tensor grad, Tensor[] logits, Tensor? attention_mask, Tensor values, int num_experts, "
+        "int top_k, float lse_square_scale) -> Tensor");
 }
 
 // Tensors on the CPU get as far as require_device, which knows whether the library computes there.

@@ -62,12 +62,13 @@ def _describe_to_tracers():
     @fake("liger_b200::_load_balancing_loss")
     def _(logits, num_experts, top_k, attention_mask, lse_square_scale):
         x = logits[0]
-        return (x.new_empty((), dtype=torch.float32), x.new_empty((), dtype=torch.float32),
-                x.new_empty((len(logits), num_experts), dtype=torch.int64), x.new_empty((num_experts + 1,), dtype=torch.float32))
+        return (x.new_empty((num_experts + 3,), dtype=torch.float32),
+                x.new_empty((len(logits), num_experts), dtype=torch.int64))
 
     @fake("liger_b200::_load_balancing_loss_backward")
-    def _(grad, logits, attention_mask, coefficients, num_experts, top_k, lse_square_scale):
-        return [t.new_empty(t.shape) for t in logits]
+    def _(grad, logits, attention_mask, values, num_experts, top_k, lse_square_scale):
+        x = logits[0]
+        return x.new_empty((len(logits), x.numel() // num_experts, num_experts))
 
 
 def _refusing(message):

@@ -37,3 +37,11 @@ def test_functional_gradients(name):
 
 def test_second_derivative_is_refused():
     cases.case_second_derivative_is_refused("cuda")
+
+
+def test_outputs_are_as_described():
+    cases.case_outputs_are_as_described("cuda")
+
+
+def test_plain_calls_take_the_short_way():
+    cases.case_plain_calls_take_the_short_way("cuda")

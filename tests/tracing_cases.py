@@ -156,3 +156,47 @@ def case_second_derivative_is_refused(device):
         args = _inputs(device, 6, 11)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             torch.func.grad(lambda x: torch.func.grad(lambda t: f(t, *args[1:]).square().sum())(x).sum())(args[0])
+
+
+def case_outputs_are_as_described(device):
+    """What the launching operators return against what tracers are told: shapes, types, strides, storage, alignment.  A compiled graph
+    takes an operator's results for tensors of their own that start on 16-byte boundaries; the gradients of several layers in one
+    buffer are cut from it where the compiler sees it."""
+    op = torch.ops.liger_b200
+    x, w, b = _inputs(device, 7, 1)
+    y, statistics = op._norm_with_statistics(x, w, b, 0, 1e-6, 0.0, False)
+    checks = ("test_schema", "test_autograd_registration", "test_faketensor", "test_aot_dispatch_dynamic")
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    torch.library.opcheck(op.norm.default, (*leaves, 0, 1e-6, 0.0, False), test_utils=checks)
+    torch.library.opcheck(op.norm.default, (x, None, None, 1, 1e-6, 0.0, True), test_utils=checks)
+    torch.library.opcheck(op._norm_with_statistics.default, (*leaves, 0, 1e-6, 0.0, False), test_utils=checks)
+    torch.library.opcheck(op._norm_backward.default, (y, x, w, b, statistics, 0, 1e-6, 0.0, False, True, False), test_utils=checks)
+    up, coefficients = torch.ones((), device=device), torch.ones(61, device=device)
+    for dtype, rows in ((torch.float32, 7), (torch.float16, 5)):          # 5 x 60 x 2 bytes are no whole vectors
+        logits = [torch.randn(rows, 60, device=device).to(dtype) for _ in range(3)]
+        for given in (logits, [logits[0], *(t.clone().requires_grad_(True) for t in logits[1:])]):
+            torch.library.opcheck(op._load_balancing_loss.default, (given, 60, 4, None, 1e-3), test_utils=checks)
+        torch.library.opcheck(op._load_balancing_loss_backward.default, (up, logits, None, coefficients, 60, 4, 0.0), test_utils=checks)
+        for t in (*op._load_balancing_loss(logits, 60, 4, None, 0.0), op._load_balancing_loss_backward(up, logits, None, coefficients, 60, 4, 0.0)):
+            assert t.numel() == 1 or t.data_ptr() % 16 == 0
+        traced = make_fx(lambda *t: torch.autograd.grad(op.load_balancing_loss([v.requires_grad_(True) for v in t], 60, 4, None, 0.0)[0], t))(
+            *[t.clone() for t in logits])
+        assert any(n.target is op._load_balancing_loss_backward.default for n in traced.graph.nodes)
+        want = [t.clone().requires_grad_(True) for t in logits]
+        want = torch.autograd.grad(op.load_balancing_loss(want, 60, 4, None, 0.0)[0], want)
+        for got, ref in zip(traced(*logits), want):
+            assert got.shape == ref.shape == (rows, 60) and torch.equal(got, ref)
+
+
+def case_plain_calls_take_the_short_way(device):
+    """Without a tracer the loss and the layers' gradients are cut from their buffers without further operators."""
+    import liger_kernel_b200 as lk
+
+    logits = [t.requires_grad_(True) for t in torch.randn(3, 6, EXPERTS).to(device)]
+    loss = lk.liger_load_balancing_loss(tuple(logits), EXPERTS)
+    assert loss.grad_fn.name() == "LigerLoadBalancingLossBackward" and not loss._is_view()
+    grads = torch.autograd.grad(loss, logits)
+    assert not any(g._is_view() for g in grads)
+    assert [g.storage_offset() for g in grads] == [i * 6 * EXPERTS for i in range(3)]
+    with torch.autocast(device):
+        assert lk.liger_load_balancing_loss(logits[0], EXPERTS).grad_fn.name() == "LigerLoadBalancingLossBackward"
