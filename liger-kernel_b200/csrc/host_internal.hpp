@@ -38,7 +38,7 @@ inline int element_size(int dtype) { return dtype == FLCE_FP32 ? 4 : 2; }
 
 // A launch that may start while the kernel in front of it drains; the kernel calls wait_for_previous_kernel() first.
 template <auto kKernel, class... Args>
-int launch_dependent(dim3 grid, dim3 block, cudaStream_t stream, const Args&... args) {
+static int launch_dependent(dim3 grid, dim3 block, cudaStream_t stream, const Args&... args) {
 #ifndef FLCE_HOST_EMULATION
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
@@ -57,10 +57,11 @@ int launch_dependent(dim3 grid, dim3 block, cudaStream_t stream, const Args&... 
 }
 
 // A launch with `bytes` of dynamic shared memory; the permission for more than 48 KB is asked for once per kernel
-// and device (kKernel names the instantiation).
+// and device (kKernel names the instantiation).  The function is static so that what it remembers belongs to this library: the
+// permission is one for the kernel in this library, not for that of another copy in the process.
 constexpr int kMostDynamicShared = 220 * 1024;      // beside what such a kernel declares statically: 227 KB in all
 template <auto kKernel, class... Args>
-int launch_with_shared(dim3 grid, unsigned block, size_t bytes, cudaStream_t stream, const Args&... args) {
+static int launch_with_shared(dim3 grid, unsigned block, size_t bytes, cudaStream_t stream, const Args&... args) {
 #ifndef FLCE_HOST_EMULATION
   static std::atomic<bool> allowed[64];
   int device = 0;
