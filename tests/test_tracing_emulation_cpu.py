@@ -51,3 +51,7 @@ def test_outputs_are_as_described():
 
 def test_plain_calls_take_the_short_way():
     cases.case_plain_calls_take_the_short_way("cpu")
+
+
+def test_lazy_negatives():
+    cases.case_lazy_negatives("cpu")

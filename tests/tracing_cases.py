@@ -200,3 +200,23 @@ def case_plain_calls_take_the_short_way(device):
     assert [g.storage_offset() for g in grads] == [i * 6 * EXPERTS for i in range(3)]
     with torch.autocast(device):
         assert lk.liger_load_balancing_loss(logits[0], EXPERTS).grad_fn.name() == "LigerLoadBalancingLossBackward"
+
+
+def case_lazy_negatives(device):
+    """Tensors whose negation is still pending (torch's views of a conjugate's imaginary part) count with their values, as inputs, as
+    parameters and as upstream gradients."""
+    import liger_kernel_b200 as lk
+
+    def pending(t):
+        lazy = torch.complex(torch.zeros_like(t), -t).conj().imag
+        assert lazy.is_neg() and torch.equal(lazy, t)
+        return lazy
+
+    x, w, b = _inputs(device, 6, 13)
+    for name, f in _operators().items():
+        assert torch.equal(f(pending(x), pending(w), pending(b)), f(x, w, b)), name
+        lazy, plain = pending(x).requires_grad_(True), x.clone().requires_grad_(True)
+        up = torch.rand_like(f(x, w, b))
+        (got,), (want,) = (torch.autograd.grad(f(t, w, b), t, u) for t, u in ((lazy, pending(up)), (plain, up)))
+        assert torch.equal(got, want), name
+    assert torch.equal(lk.liger_load_balancing_loss((x, pending(x)), EXPERTS), lk.liger_load_balancing_loss((x, x), EXPERTS))
