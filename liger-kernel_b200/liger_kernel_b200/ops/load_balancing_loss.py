@@ -9,7 +9,10 @@ elementary operations.  Here it is one read of the logits forward and one read a
 * softmax, sums and the loss are fp32 or wider whatever the logits' type; the loss is fp32.
 * equal logits are chosen by index, lowest first.  The choice is made on the logits: probabilities that round to the same value
   stay apart.
-* tokens that the mask leaves out are not read; if it leaves none, the loss and all gradients are zero.
+* tokens that the mask leaves out (elements equal to 0; any other element keeps its token, as one token) are not read; if it leaves
+  none, the loss and all gradients are zero.
+* a gradient of the gradient, inputs with a forward-mode tangent and vmap are refused; torch.compile, torch.export and make_fx record
+  the launches as operators.
 """
 
 from dataclasses import dataclass

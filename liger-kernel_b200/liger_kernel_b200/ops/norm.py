@@ -11,7 +11,8 @@ Call surface of the reference's ``LigerLayerNormFunction`` (``src/liger_kernel/o
 * ``in_place`` and ``row_mode`` of the reference's RMSNorm are accepted and mean nothing here: the gradient of the input is
   always a tensor of its own, and the launch shape follows from the row's length.
 * Any leading dimensions, any row pitch (a slice of a wider tensor is read where it lies), any length of the last dimension from
-  one element.  A gradient of the gradient is refused by autograd.
+  one element.  A gradient of the gradient is refused by autograd, and so are inputs with a forward-mode tangent.
+* torch.compile, torch.export and make_fx record the launches as operators; torch.func's grad, vjp and vmap apply.
 """
 
 from .. import _lib
@@ -30,7 +31,8 @@ class LigerLayerNormFunction:
 
 class LigerRMSNormFunction:
     """``apply(X, W, eps, offset=0.0, casting_mode="llama", in_place=True, row_mode=None)``: ``x * rstd * (offset + W)``; ``W``
-    may be None.  Casting "llama" rounds ``x * rstd`` to the input's type before it meets the weight, "gemma" does not."""
+    may be None.  Casting "llama" rounds ``x * rstd`` to the input's type before it meets the weight, "gemma" does not; the
+    reference's "none", which computes in the input's type, is refused."""
 
     @staticmethod
     def apply(X, W, eps, offset=0.0, casting_mode="llama", in_place=True, row_mode=None):

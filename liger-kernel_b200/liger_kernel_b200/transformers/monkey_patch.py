@@ -36,7 +36,7 @@ def _report_unhandled(**flags):
     for name, on in flags.items():
         if on and name not in _reported:
             _reported.add(name)
-            logger.info("liger_kernel_b200 only provides the fused linear cross-entropy path; '%s=True' is ignored", name)
+            logger.info("liger_kernel_b200 patches the loss of a model's head; '%s=True' is ignored", name)
 
 
 def _patch_cross_entropy():
@@ -239,6 +239,7 @@ def install(cross_entropy: bool = False, fused_linear_jsd: bool = False, fused_l
     ``liger_kernel.transformers.functional``, ``liger_kernel.transformers.fused_linear_cross_entropy``), and on request
     the stand-alone cross-entropy, fused linear JSD, fused linear scaled cross-entropy, layer norm and RMSNorm operators at theirs;
     ``chunked_loss=True`` also rebinds the DPO / ORPO / SimPO / CPO / KTO / GRPO / JSD / cosine-similarity classes of ``liger_kernel.chunked_loss``.
+    RMSNorm here has the casting modes "llama" and "gemma": callers with another one raise after ``rms_norm=True``.
     Returns False when no ``liger_kernel`` is installed."""
     from ..ops.cross_entropy import LigerCrossEntropyFunction
     from ..ops.fused_linear_jsd import LigerFusedLinearJSDFunction
