@@ -85,7 +85,7 @@ const void* elements(const Tensor& t, const char* what) {
 // Tangents of forward-mode differentiation would be lost below autograd, and with them a part of the derivative.
 void refuse_tangent(const Tensor& t) {
   TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(),
-                              "liger_kernel_b200 has no forward-mode derivatives: the input carries a forward gradient");
+                              "liger_kernel_b200 has no forward-mode derivatives: an input or an upstream gradient carries a forward gradient");
 }
 
 // A gradient of a gradient would need the graph of the kernels' own arithmetic, which does not exist: what backward returns
@@ -212,6 +212,7 @@ std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& grad, const Tenso
                                                  const optional<Tensor>& bias, const Tensor& stats, int64_t kind, double eps, double offset,
                                                  bool round_xhat, bool need_w, bool need_b) {
   static const auto next = operator_of<decltype(norm_backward_launch)>("liger_b200::_norm_backward");
+  refuse_tangent(grad);
   variable_list out(3);
   {
     at::AutoDispatchBelowAutograd below;
@@ -380,6 +381,7 @@ Tensor balance_backward_launch(const Tensor& grad, at::TensorList logits, const 
 Tensor balance_backward(const Tensor& grad, at::TensorList logits, const optional<Tensor>& attention_mask, const Tensor& values,
                         int64_t num_experts, int64_t top_k, double lse_square_scale) {
   static const auto next = operator_of<decltype(balance_backward_launch)>("liger_b200::_load_balancing_loss_backward");
+  refuse_tangent(grad);
   variable_list out(1);
   {
     at::AutoDispatchBelowAutograd below;

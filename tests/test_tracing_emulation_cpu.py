@@ -55,3 +55,7 @@ def test_plain_calls_take_the_short_way():
 
 def test_lazy_negatives():
     cases.case_lazy_negatives("cpu")
+
+
+def test_forward_over_reverse():
+    cases.case_forward_over_reverse("cpu")

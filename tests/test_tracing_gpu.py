@@ -49,3 +49,7 @@ def test_plain_calls_take_the_short_way():
 
 def test_lazy_negatives():
     cases.case_lazy_negatives("cuda")
+
+
+def test_forward_over_reverse():
+    cases.case_forward_over_reverse("cuda")

@@ -220,3 +220,19 @@ def case_lazy_negatives(device):
         (got,), (want,) = (torch.autograd.grad(f(t, w, b), t, u) for t, u in ((lazy, pending(up)), (plain, up)))
         assert torch.equal(got, want), name
     assert torch.equal(lk.liger_load_balancing_loss((x, pending(x)), EXPERTS), lk.liger_load_balancing_loss((x, x), EXPERTS))
+
+
+def case_forward_over_reverse(device):
+    """A tangent that only the upstream gradient carries is refused as well: the input's gradient would lose it."""
+    import pytest
+    import torch.autograd.forward_ad as fa
+
+    for f in _operators().values():
+        x, w, b = _inputs(device, 4, 21)
+        x.requires_grad_(True)
+        y = f(x, w, b)
+        with fa.dual_level():
+            up = fa.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(NotImplementedError, match="forward"):
+                torch.autograd.grad(y, x, up, retain_graph=True)
+        torch.autograd.grad(y, x, torch.ones_like(y))
