@@ -192,7 +192,14 @@ std::tuple<Tensor, Tensor, Tensor> norm_backward_launch(const Tensor& grad, cons
   const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
   OnDevice on(x);
   const NormOperands o = norm_operands(kind, x, w, b, eps, offset, round_xhat);
-  const Tensor dy = as_rows(grad, o.p.hidden);
+  TORCH_CHECK_VALUE(grad.sizes() == x.sizes() && grad.scalar_type() == x.scalar_type() && grad.device() == x.device(),
+                    "the gradient must agree with the input in shape, type and device");
+  const int64_t planes = kind == FLCE_LAYER_NORM ? 2 : 1;
+  TORCH_CHECK_VALUE(stats.dim() == 2 && stats.size(0) == planes && stats.size(1) == o.p.n_rows && stats.scalar_type() == at::kFloat &&
+                        stats.device() == x.device(),
+                    "the statistics must be [", planes, ", ", o.p.n_rows, "] in fp32 on the input's device");
+  TORCH_CHECK_VALUE((w.defined() || !need_w) && (b.defined() || !need_b), "the gradient of a parameter that is not given");
+  const Tensor dy = as_rows(grad, o.p.hidden), kept = stats.contiguous();
   Tensor dx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous)), dw, db, workspace;
   size_t bytes = 0;
   if (need_w) dw = at::empty_like(o.w);
@@ -201,7 +208,7 @@ std::tuple<Tensor, Tensor, Tensor> norm_backward_launch(const Tensor& grad, cons
     bytes = g_lib.norm_workspace_bytes(&o.p);
     workspace = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
   }
-  const float* rstd = stats.const_data_ptr<float>();
+  const float* rstd = kept.const_data_ptr<float>();
   check(g_lib.norm_backward(&o.p, elements(dy, "the gradient"), dy.stride(0), kind == FLCE_LAYER_NORM ? rstd + o.p.n_rows : nullptr, rstd,
                             dx.data_ptr(), need_w ? dw.data_ptr() : nullptr, need_b ? db.data_ptr() : nullptr,
                             workspace.defined() ? workspace.data_ptr() : nullptr, bytes, on.stream));
@@ -371,9 +378,13 @@ Tensor balance_backward_launch(const Tensor& grad, at::TensorList logits, const 
                                int64_t num_experts, int64_t top_k, double lse_square_scale) {
   OnDevice on(logits[0]);
   const BalanceOperands o = balance_operands(logits, num_experts, top_k, attention_mask.value_or(Tensor()), lse_square_scale);
-  const Tensor up = grad.to(at::kFloat).contiguous();
+  TORCH_CHECK_VALUE(grad.numel() == 1 && grad.device() == logits[0].device(), "the gradient must be one number on the logits' device");
+  TORCH_CHECK_VALUE(values.dim() == 1 && values.size(0) > num_experts && values.scalar_type() == at::kFloat &&
+                        values.device() == logits[0].device(),
+                    "the coefficients must be ", num_experts + 1, " fp32 numbers or more on the logits' device");
+  const Tensor up = grad.to(at::kFloat).contiguous(), coef = values.contiguous();
   Tensor all = at::empty({o.p.n_layers, o.p.n_tokens, num_experts}, logits[0].options().memory_format(at::MemoryFormat::Contiguous));
-  check(g_lib.balance_backward(&o.p, o.pointers.data(), values.const_data_ptr<float>(), up.const_data_ptr<float>(), all.data_ptr(),
+  check(g_lib.balance_backward(&o.p, o.pointers.data(), coef.const_data_ptr<float>(), up.const_data_ptr<float>(), all.data_ptr(),
                                on.stream));
   return all;
 }

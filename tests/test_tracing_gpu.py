@@ -53,3 +53,7 @@ def test_lazy_negatives():
 
 def test_forward_over_reverse():
     cases.case_forward_over_reverse("cuda")
+
+
+def test_operators_check_what_belongs_together():
+    cases.case_operators_check_what_belongs_together("cuda")

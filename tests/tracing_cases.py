@@ -236,3 +236,46 @@ def case_forward_over_reverse(device):
             with pytest.raises(NotImplementedError, match="forward"):
                 torch.autograd.grad(y, x, up, retain_graph=True)
         torch.autograd.grad(y, x, torch.ones_like(y))
+
+
+def case_operators_check_what_belongs_together(device):
+    """The launching operators by themselves: a gradient, statistics or coefficients that do not fit the input are refused before a
+    kernel reads them; what fits but lies otherwise in memory is taken."""
+    import pytest
+
+    op = torch.ops.liger_b200
+    x, w, b = _inputs(device, 6, 31)
+    y, stats = op._norm_with_statistics(x, w, b, 0, 1e-6, 0.0, False)
+
+    def backward(grad=y, statistics=stats, kind=0, need_weight=True, need_bias=True, weight=w, bias=b):
+        return op._norm_backward(grad, x, weight, bias, statistics, kind, 1e-6, 0.0, False, need_weight, need_bias)
+
+    want = backward()
+    for grad in (y[:5], y[:, :12], y.reshape(12, 12), y.reshape(2, 3, EXPERTS), y.half(), torch.ones((), device=device)):
+        with pytest.raises(ValueError, match="gradient"):
+            backward(grad)
+    for statistics in (stats[:1], stats[:, :5], stats.t(), stats.reshape(-1), stats.half(), stats.double()):
+        with pytest.raises(ValueError, match="statistics"):
+            backward(statistics=statistics)
+    with pytest.raises(ValueError, match="statistics"):
+        backward(kind=1, bias=None, need_bias=False)                       # RMSNorm has one row of them
+    for missing in (dict(weight=None), dict(bias=None)):
+        with pytest.raises(ValueError, match="gradient of a parameter"):
+            backward(**missing)
+    for got, ref in zip(backward(y.t().contiguous().t(), stats.t().contiguous().t()), want):
+        assert torch.equal(got, ref)
+
+    logits = [x, y]
+    values, counts = op._load_balancing_loss(logits, EXPERTS, TOP_K, None, 0.0)
+
+    def balance_backward(grad=torch.ones((), device=device), v=values):
+        return op._load_balancing_loss_backward(grad, logits, None, v, EXPERTS, TOP_K, 0.0)
+
+    want = balance_backward()
+    assert want.shape == (2, 6, EXPERTS) and torch.equal(balance_backward(v=torch.stack([values, values]).t()[:, 0]), want)
+    for v in (values[:EXPERTS], values.half(), values[None], values[:0]):
+        with pytest.raises(ValueError, match="coefficients"):
+            balance_backward(v=v)
+    for grad in (torch.ones(2, device=device), torch.ones(0, device=device)):
+        with pytest.raises(ValueError, match="gradient"):
+            balance_backward(grad)
